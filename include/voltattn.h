@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define VA_ABI_VERSION 4
+#define VA_ABI_VERSION 5
 
 /* Status codes. */
 enum {
@@ -322,6 +322,125 @@ size_t va_page_scale_bytes(va_fmt fmt, int Hkv, int page_rows, int D, int G);
 int va_append_kv(va_fmt fmt, const uint16_t* x, int n, const int32_t* start,
                  const int32_t* block_table, const va_paged_shape* shape, void* pages,
                  uint16_t* scales, void* stream);
+
+/* ---- prompts, drafted tokens and the page pool ----
+ * What a serving loop does around the decode step; no counterpart in the
+ * reference. Query head i attends KV head i / (Hq / Hkv), as above. */
+
+/* Prompts packed one behind the other: rows cu[b] .. cu[b+1] - 1 are sequence
+ * b. Row strides (*_row) and head strides (*_head) count fp16 elements, so q, k
+ * and v may be slices of one fused projection: multiples of 8; k_row and v_row
+ * in [D, 2^24), the others >= 0. out is contiguous [total][Hq][D]. */
+typedef struct {
+    int B;             /* sequences, >= 1 */
+    int total;         /* rows of q, k, v and out, >= 0 */
+    int Hq, Hkv;       /* Hq % Hkv == 0 */
+    int D;             /* 64 or 128 */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+} va_prefill_shape;
+
+/* Device buffers: q, k, v fp16, 16-byte aligned; cu int32 [B+1], 4-byte aligned;
+ * out fp16, 16-byte aligned. */
+typedef struct {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const int32_t*  cu;    /* not descending, within 0 .. total */
+    uint16_t*       out;
+} va_prefill_bufs;
+
+/* Causal attention of every prompt of the batch: row i of a sequence attends
+ * its rows 0 .. i, softmax(q.K^T / sqrt(D)) V per query head. Rows of out in no
+ * sequence (before cu[0], from cu[B] on) become zero. A bound below its
+ * predecessor counts as equal to it, one above total as total. A row whose
+ * scores are all -inf is zero; NaN or an infinity in row j of k or v may reach
+ * any row of its 128-row block before j, and no row of another sequence.
+ * Asynchronous on `stream`; needs no workspace. */
+int va_prefill(const va_prefill_bufs* b, const va_prefill_shape* shape, void* stream);
+
+/* Device buffers of one verification step of drafted tokens. Alignment as
+ * va_paged_bufs; tree_mask 8 bytes; out 8 bytes; ws 16 bytes. */
+typedef struct {
+    const void*     k;             /* page pools, as va_paged_bufs */
+    const void*     v;
+    const uint16_t* sk;
+    const uint16_t* sv;
+    const int32_t*  block_table;   /* [B][max_pages] */
+    const int32_t*  ctx_lens;      /* [B] positions of context, >= 0 */
+    const int32_t*  tree_sizes;    /* [B] drafts of each sequence, 0 .. T; NULL: T each */
+    const uint64_t* tree_mask;     /* [B][T]: bit j of entry i: draft i attends draft j */
+    const uint16_t* q;             /* [B][T][Hq][D] fp16 */
+    uint16_t*       out;           /* [B][T][Hq][D] fp16 */
+    float*          ws;            /* va_tree_ws_bytes bytes; needs no zeroing */
+} va_tree_bufs;
+
+/* Attention of T drafted tokens per sequence (1 <= T <= VA_TREE_MAX) over a
+ * paged cache: draft i of sequence b attends positions 0 .. ctx_lens[b] - 1 and
+ * the drafts j < tree_sizes[b] whose bit its mask has (its own and its ancestors',
+ * for a tree; bits 0 .. i for a chain). Draft j's K/V rows are position
+ * ctx_lens[b] + j of the cache, written there before (va_append_kv). A draft to
+ * which nothing is visible, and drafts from tree_sizes[b] on, give zeros. A
+ * sequence with ctx + size above max_seq_len, or a length or size out of range,
+ * gives NaN for all T drafts; a page id outside the pool on one of its positions
+ * NaN for its drafts. V values whose scale exceeds 1023 (q8), 16383 (q4) or 32767
+ * (q3), beyond any cache made from fp16 values, may overflow to infinities. The
+ * tiled formats only. The last bits of a sequence's sums depend on the
+ * lengths of the whole batch; the same batch gives the same bits. Asynchronous
+ * on `stream`; concurrent calls need distinct ws. */
+#define VA_TREE_MAX 64
+int va_decode_tree(va_fmt fmt, const va_tree_bufs* b, const va_paged_shape* shape, int T, void* stream);
+
+/* Workspace of va_decode_tree; 0 for invalid arguments. */
+size_t va_tree_ws_bytes(va_fmt fmt, const va_paged_shape* shape, int T);
+
+/* The page pools of a cache (sk, sv: quantized formats). Alignment as
+ * va_append_kv: k, v 16 bytes (4 for quantized formats), sk, sv 2 bytes. */
+typedef struct {
+    void*     k;
+    void*     v;
+    uint16_t* sk;
+    uint16_t* sv;
+} va_pools;
+
+/* Moves kept rows together, in place: for i < counts[b], row base[b] + i of
+ * sequence b becomes what row base[b] + keep[b][i] was before the call, in every
+ * KV head of K and V (the accepted drafts after a verification step, with base
+ * the context's length). counts[b] is limited to 0 .. n; keep [B][n], n <=
+ * VA_TREE_MAX, in any order, repetitions allowed. A row whose source or
+ * destination lies before or past the block table, or on a page outside the
+ * pool, is not written. Sequences must not share the pages written. Any format
+ * and any page_rows >= 1 (as va_append_kv). Asynchronous on `stream`. */
+int va_compact_kv(va_fmt fmt, const va_pools* pools, const va_paged_shape* shape, const int32_t* block_table,
+                  const int32_t* base, const int32_t* keep, const int32_t* counts, int n, void* stream);
+
+/* Page ownership, on the device: refs[p] counts the sequences that hold page p;
+ * a page is free when its count is 0. A sequence of n positions holds the first
+ * ceil(n / page_rows) entries of its block-table row, and free pages are handed
+ * out lowest id first, in (sequence, entry) order; an entry for which none was
+ * left is -1 (rows appended there are dropped, decoding it gives NaN) and counts
+ * in *missing (device memory, may be NULL). Lengths are limited to 0 ..
+ * max_pages * page_rows; page ids outside the pool are carried along and never
+ * counted, read or written. max_pages * page_rows < 2^31, num_pages <= 2^30.
+ *
+ * va_fork_pages: the sequences of the next step, child c continuing sequence
+ * parents[c] (beam search's reordering, several samples of one prompt); outside
+ * 0 .. B-1: an empty sequence. Full pages are shared. The partly filled last
+ * page stays with a parent's first child and is copied, its rows in use, for
+ * each further one, so that every child may append. Sequences without a child
+ * give up their pages, before any is handed out. new_table [children][max_pages]
+ * (not block_table itself; entries a child does not hold are -1), new_lens
+ * [children]; refs is updated, and the pools get the copied rows. */
+int va_fork_pages(va_fmt fmt, const va_pools* pools, const va_paged_shape* shape, const int32_t* block_table,
+                  const int32_t* seq_lens, const int32_t* parents, int children, int32_t* refs,
+                  int32_t* new_table, int32_t* new_lens, int32_t* missing, void* stream);
+
+/* va_resize_pages: every sequence from old_lens[b] to new_lens[b] positions:
+ * entries no longer held are given up and become -1 (new_lens[b] = 0 frees the
+ * sequence), then the missing ones are handed out. A page that another sequence
+ * still holds stays shared: a sequence cut back into such a page must not append
+ * to it. block_table and refs are updated in place. */
+int va_resize_pages(int B, int page_rows, int max_pages, int num_pages, int32_t* block_table, int32_t* refs,
+                    const int32_t* old_lens, const int32_t* new_lens, int32_t* missing, void* stream);
 
 /* ---- runtime shims (the reference calls the CUDA runtime directly:
  *      cudaMalloc/cudaMemcpy/cudaFree/cudaEvent*, src/voltattn.cu:863-895, 936-955,

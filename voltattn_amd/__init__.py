@@ -30,6 +30,8 @@ __all__ = [
     "Stream", "Graph", "sync", "lib", "LIB_PATH", "fmt_bits", "is_f16", "check",
     "PagedShape", "PagedBufs", "decode_gqa", "pick_splits_gqa", "decode_paged",
     "pick_splits_paged", "page_bytes", "page_scale_bytes", "append_kv", "row_bytes",
+    "PrefillShape", "PrefillBufs", "prefill", "TreeBufs", "decode_tree", "tree_ws_bytes", "TREE_MAX",
+    "Pools", "compact_kv", "fork_pages", "resize_pages",
 ]
 
 LIB_PATH = Path(__file__).resolve().parent / "libvoltattn_hip.so"
@@ -78,6 +80,24 @@ class _PagedBufs(C.Structure):
                 ("seq_lens", _P), ("q", _P), ("out", _P), ("ws", _P)]
 
 
+class _PrefillShape(C.Structure):
+    _fields_ = [("B", _I), ("total", _I), ("Hq", _I), ("Hkv", _I), ("D", _I)] + [
+        (n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+
+
+class _PrefillBufs(C.Structure):
+    _fields_ = [(n, _P) for n in ("q", "k", "v", "cu", "out")]
+
+
+class _TreeBufs(C.Structure):
+    _fields_ = [(n, _P) for n in ("k", "v", "sk", "sv", "block_table", "ctx_lens", "tree_sizes", "tree_mask",
+                                  "q", "out", "ws")]
+
+
+class _Pools(C.Structure):
+    _fields_ = [(n, _P) for n in ("k", "v", "sk", "sv")]
+
+
 class _DevInfo(C.Structure):
     _fields_ = [("name", C.c_char * 256), ("arch", C.c_char * 64), ("compute_units", _I),
                 ("clock_khz", _I), ("mem_clock_khz", _I), ("mem_bus_bits", _I),
@@ -117,6 +137,12 @@ _sig("va_pick_splits_paged", _I, _I, C.POINTER(_PagedShape), C.POINTER(_I))
 _sig("va_page_bytes", _SZ, _I, _I, _I, _I)
 _sig("va_page_scale_bytes", _SZ, _I, _I, _I, _I, _I)
 _sig("va_append_kv", _I, _I, _P, _I, _P, _P, C.POINTER(_PagedShape), _P, _P, _P)
+_sig("va_prefill", _I, C.POINTER(_PrefillBufs), C.POINTER(_PrefillShape), _P)
+_sig("va_decode_tree", _I, _I, C.POINTER(_TreeBufs), C.POINTER(_PagedShape), _I, _P)
+_sig("va_tree_ws_bytes", _SZ, _I, C.POINTER(_PagedShape), _I)
+_sig("va_compact_kv", _I, _I, C.POINTER(_Pools), C.POINTER(_PagedShape), _P, _P, _P, _P, _I, _P)
+_sig("va_fork_pages", _I, _I, C.POINTER(_Pools), C.POINTER(_PagedShape), _P, _P, _P, _I, _P, _P, _P, _P, _P)
+_sig("va_resize_pages", _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P)
 _sig("va_device_count", _I, C.POINTER(_I))
 _sig("va_set_device", _I, _I)
 _sig("va_device_info", _I, C.POINTER(_DevInfo))
@@ -314,6 +340,115 @@ def append_kv(f: Fmt, x: int, n: int, start: int, block_table: int, shape: Paged
     cs = shape._c()
     check(lib.va_append_kv(int(f), x, n, start, block_table, C.byref(cs), pages, scales or None,
                            _stream(stream)))
+
+
+TREE_MAX = 64        # VA_TREE_MAX: drafted tokens per sequence
+
+
+@dataclass
+class PrefillShape:
+    """va_prefill_shape: B prompts of `total` rows together. Strides count fp16 elements;
+    0 stands for the contiguous [total][heads][D] layout."""
+    B: int
+    total: int
+    Hq: int
+    Hkv: int
+    D: int
+    q_row: int = 0
+    q_head: int = 0
+    k_row: int = 0
+    k_head: int = 0
+    v_row: int = 0
+    v_head: int = 0
+
+    def _c(self) -> _PrefillShape:
+        return _PrefillShape(self.B, self.total, self.Hq, self.Hkv, self.D,
+                             self.q_row or self.Hq * self.D, self.q_head or self.D,
+                             self.k_row or self.Hkv * self.D, self.k_head or self.D,
+                             self.v_row or self.Hkv * self.D, self.v_head or self.D)
+
+
+@dataclass
+class PrefillBufs:
+    """va_prefill_bufs: device pointers as ints (0 = NULL)."""
+    q: int = 0
+    k: int = 0
+    v: int = 0
+    cu: int = 0
+    out: int = 0
+
+
+def prefill(b: PrefillBufs, shape: PrefillShape, stream=None) -> None:
+    """Causal attention of packed prompts (rows cu[i] .. cu[i+1] - 1 are prompt i)."""
+    cb, cs = _PrefillBufs(*((getattr(b, n) or None) for n in ("q", "k", "v", "cu", "out"))), shape._c()
+    check(lib.va_prefill(C.byref(cb), C.byref(cs), _stream(stream)))
+
+
+@dataclass
+class TreeBufs:
+    """va_tree_bufs: device pointers as ints (0 = NULL; tree_sizes 0: T drafts each)."""
+    K: int = 0
+    V: int = 0
+    scK: int = 0
+    scV: int = 0
+    block_table: int = 0
+    ctx_lens: int = 0
+    tree_sizes: int = 0
+    tree_mask: int = 0
+    q: int = 0
+    out: int = 0
+    ws: int = 0
+
+    def _c(self) -> _TreeBufs:
+        return _TreeBufs(*(x or None for x in (self.K, self.V, self.scK, self.scV, self.block_table, self.ctx_lens,
+                                               self.tree_sizes, self.tree_mask, self.q, self.out, self.ws)))
+
+
+def decode_tree(f: Fmt, b: TreeBufs, shape: PagedShape, T: int, stream=None) -> None:
+    """Attention of T drafted tokens per sequence over a paged cache (q/out [B][T][Hq][D])."""
+    cb, cs = b._c(), shape._c()
+    check(lib.va_decode_tree(int(f), C.byref(cb), C.byref(cs), T, _stream(stream)))
+
+
+def tree_ws_bytes(f: Fmt, shape: PagedShape, T: int) -> int:
+    cs = shape._c()
+    return lib.va_tree_ws_bytes(int(f), C.byref(cs), T)
+
+
+@dataclass
+class Pools:
+    """va_pools: the page pools of a cache, device pointers as ints (0 = NULL)."""
+    K: int = 0
+    V: int = 0
+    scK: int = 0
+    scV: int = 0
+
+    def _c(self) -> _Pools:
+        return _Pools(self.K or None, self.V or None, self.scK or None, self.scV or None)
+
+
+def compact_kv(f: Fmt, pools: Pools, shape: PagedShape, block_table: int, base: int, keep: int, counts: int, n: int,
+               stream=None) -> None:
+    """Rows base[b] + keep[b][i] of every sequence move to base[b] + i, i < counts[b] (keep [B][n])."""
+    cp, cs = pools._c(), shape._c()
+    check(lib.va_compact_kv(int(f), C.byref(cp), C.byref(cs), block_table or None, base or None, keep or None,
+                            counts or None, n, _stream(stream)))
+
+
+def fork_pages(f: Fmt, pools: Pools, shape: PagedShape, block_table: int, seq_lens: int, parents: int, children: int,
+               refs: int, new_table: int, new_lens: int, missing: int = 0, stream=None) -> None:
+    """The next step's sequences: child c continues sequence parents[c] (va_fork_pages)."""
+    cp, cs = pools._c(), shape._c()
+    check(lib.va_fork_pages(int(f), C.byref(cp), C.byref(cs), block_table or None, seq_lens or None, parents or None,
+                            children, refs or None, new_table or None, new_lens or None, missing or None,
+                            _stream(stream)))
+
+
+def resize_pages(B: int, page_rows: int, max_pages: int, num_pages: int, block_table: int, refs: int, old_lens: int,
+                 new_lens: int, missing: int = 0, stream=None) -> None:
+    """Pages given up and handed out so that sequence b holds new_lens[b] positions (va_resize_pages)."""
+    check(lib.va_resize_pages(B, page_rows, max_pages, num_pages, block_table or None, refs or None, old_lens or None,
+                              new_lens or None, missing or None, _stream(stream)))
 
 
 def row_bytes(f: Fmt, D: int) -> int:

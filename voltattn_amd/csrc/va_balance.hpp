@@ -37,30 +37,6 @@ namespace va {
 constexpr int balance_tile(int TB) { return TB >= 128 ? TB : 128; }
 constexpr int BIG = 1 << 30;
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_rows_i(int old, int x) {
-    return __builtin_amdgcn_update_dpp(old, x, CTRL, ROWS, 0xF, false);
-}
-// Inclusive sum over the lanes (row shifts, then the row broadcasts).
-__device__ __forceinline__ int wave_scan(int x) {
-    x += dpp_rows_i<0x111, 0xF>(0, x);
-    x += dpp_rows_i<0x112, 0xF>(0, x);
-    x += dpp_rows_i<0x114, 0xF>(0, x);
-    x += dpp_rows_i<0x118, 0xF>(0, x);
-    x += dpp_rows_i<0x142, 0xA>(0, x);
-    x += dpp_rows_i<0x143, 0xC>(0, x);
-    return x;
-}
-__device__ __forceinline__ int wave_scan_max(int x) {           // x >= 0; lane 63 holds the maximum
-    x = max(x, dpp_rows_i<0x111, 0xF>(0, x));
-    x = max(x, dpp_rows_i<0x112, 0xF>(0, x));
-    x = max(x, dpp_rows_i<0x114, 0xF>(0, x));
-    x = max(x, dpp_rows_i<0x118, 0xF>(0, x));
-    x = max(x, dpp_rows_i<0x142, 0xA>(0, x));
-    x = max(x, dpp_rows_i<0x143, 0xC>(0, x));
-    return x;
-}
-
 template <int BT, int COST, int MIN_RUN, int QG>
 struct Balance : Runs<COST, MIN_RUN> {
     using R = Runs<COST, MIN_RUN>;

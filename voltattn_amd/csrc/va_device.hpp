@@ -241,4 +241,29 @@ __device__ __forceinline__ float column_max(float x) {
     return rows_max(x);
 }
 
+// ---------------------------------------------------------------- wave scans --
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_rows_i(int old, int x) {
+    return __builtin_amdgcn_update_dpp(old, x, CTRL, ROWS, 0xF, false);
+}
+// Inclusive sum over the lanes (row shifts, then the row broadcasts).
+__device__ __forceinline__ int wave_scan(int x) {
+    x += dpp_rows_i<0x111, 0xF>(0, x);
+    x += dpp_rows_i<0x112, 0xF>(0, x);
+    x += dpp_rows_i<0x114, 0xF>(0, x);
+    x += dpp_rows_i<0x118, 0xF>(0, x);
+    x += dpp_rows_i<0x142, 0xA>(0, x);
+    x += dpp_rows_i<0x143, 0xC>(0, x);
+    return x;
+}
+__device__ __forceinline__ int wave_scan_max(int x) {           // x >= 0; lane 63 holds the maximum
+    x = max(x, dpp_rows_i<0x111, 0xF>(0, x));
+    x = max(x, dpp_rows_i<0x112, 0xF>(0, x));
+    x = max(x, dpp_rows_i<0x114, 0xF>(0, x));
+    x = max(x, dpp_rows_i<0x118, 0xF>(0, x));
+    x = max(x, dpp_rows_i<0x142, 0xA>(0, x));
+    x = max(x, dpp_rows_i<0x143, 0xC>(0, x));
+    return x;
+}
+
 } // namespace va

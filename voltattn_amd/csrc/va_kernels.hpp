@@ -197,6 +197,73 @@ struct AppendArgs {
 };
 hipError_t launch_append(int bits, int G, const AppendArgs& a, hipStream_t stream);
 
+// Causal attention of packed prompts (va_prefill.hip). Rows are `*_row` elements
+// apart, heads `*_head`; out is contiguous [total][hq][D].
+struct PrefillArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const int32_t*  cu;           // [B + 1] bounds of the sequences
+    uint16_t*       out;
+    long long q_row, q_head, k_row, k_head, v_row, v_head;
+    int   B, total, hq, group;    // group: query heads per K/V head
+    float qscale;                 // log2(e) / sqrt(D)
+    int   items;                  // row tiles of the grid, set by launch_prefill
+};
+long long prefill_items(int total, int B);   // its row tiles at most
+hipError_t launch_prefill(int D, const PrefillArgs& a, hipStream_t stream);
+
+// Drafted tokens over a paged cache (va_tree.hpp).
+struct TreeArgs {
+    const uint8_t*  k;            // page pools, as DecodeArgs
+    const uint8_t*  v;
+    const uint16_t* sk;
+    const uint16_t* sv;
+    const int32_t*  block_table;  // [B][max_pages]
+    const int32_t*  ctx_lens;     // [B]
+    const int32_t*  sizes;        // [B] drafts of each sequence, or null: T
+    const uint64_t* mask;         // [B][T]
+    const uint16_t* q;            // [B][T][hkv * group][D]
+    uint16_t*       out;
+    float*          ws;           // tree_ws_floats
+    int   B, T, hkv, group;
+    int   max_pages, page_shift, num_pages;
+    int   cap;                    // ctx + drafts at most
+    float qscale;
+    int   nwg, min_share;         // work-groups, and the fewest tiles that one takes
+};
+// Query rows and K/V rows of a work-group's tile where a K/V head has `rows` query rows.
+int tree_rows(int rows);
+int tree_tile(int rows);
+int tree_groups_per_cu(int rows);
+hipError_t launch_tree(int kind, int D, int G, const TreeArgs& a, hipStream_t stream);
+
+// Page pool bookkeeping and row moves (va_pages.hip). Each launch uses the fields that
+// it needs.
+struct PageArgs {
+    uint8_t* k;                   // pools [num_pages][hkv][page_rows][row_bytes]
+    uint8_t* v;
+    uint8_t* sk;                  // scales, scale_bytes a row (0: none)
+    uint8_t* sv;
+    const int32_t* table;         // [B][max_pages]
+    const int32_t* lens;          // [B] positions (compaction: the first kept row's)
+    const int32_t* after;         // [B] positions after a resize
+    const int32_t* parents;       // [children]
+    const int32_t* keep;          // [B][n]
+    const int32_t* counts;        // [B]
+    int32_t* refs;                // [num_pages]
+    int32_t* new_table;           // fork: [children][max_pages]; resize: the table itself
+    int32_t* new_lens;            // [children]
+    int32_t* missing;             // may be null
+    int B, hkv, page_rows, max_pages, num_pages;
+    int children, n;
+    int row_bytes, scale_bytes;
+    bool wide;                    // rows are 16-byte words
+};
+hipError_t launch_compact(const PageArgs& a, hipStream_t stream);
+hipError_t launch_fork(const PageArgs& a, hipStream_t stream);
+hipError_t launch_resize(const PageArgs& a, hipStream_t stream);
+
 // fp32 -> fp16 (round to nearest even) over n values.
 hipError_t launch_f32_to_f16(const float* x, size_t n, uint16_t* out, hipStream_t stream);
 

@@ -17,6 +17,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <unordered_map>
 #include <vector>
@@ -787,6 +788,242 @@ int va_append_kv(va_fmt fmt, const uint16_t* x, int n, const int32_t* start,
     a.num_pages = sh->num_pages;
     const hipError_t e = va::launch_append(bits_of(fmt), is_f16(fmt) ? 32 : sh->G, a, as_stream(stream));
     if (e != hipSuccess) return hip_fail(e, "append launch");
+    return VA_OK;
+}
+
+int va_prefill(const va_prefill_bufs* b, const va_prefill_shape* sh, void* stream) {
+    if (!sh) return fail(VA_ENULL, "shape is NULL");
+    if (!b) return fail(VA_ENULL, "bufs is NULL");
+    if (sh->B < 1 || sh->Hkv < 1) return fail(VA_EINVAL, "B and Hkv must be >= 1");
+    if (sh->total < 0) return fail(VA_EINVAL, "total must be >= 0 (got %d)", sh->total);
+    if (sh->D != 64 && sh->D != 128) return fail(VA_EINVAL, "D must be 64 or 128 (got %d)", sh->D);
+    if (sh->Hq < 1 || sh->Hq % sh->Hkv)
+        return fail(VA_EINVAL, "Hq must be a positive multiple of Hkv (Hq=%d, Hkv=%d)", sh->Hq, sh->Hkv);
+    for (const int64_t s : {sh->q_row, sh->q_head, sh->k_row, sh->k_head, sh->v_row, sh->v_head})
+        if (s < 0 || s % 8) return fail(VA_EINVAL, "strides must be multiples of 8 and >= 0 (got %lld)", (long long)s);
+    for (const int64_t s : {sh->k_row, sh->v_row})
+        if (s < sh->D || s >= 1 << 24) return fail(VA_EINVAL, "k_row and v_row must be in [D, 2^24) (got %lld)", (long long)s);
+    if (va::prefill_items(sh->total, sh->B) * sh->Hq > 0x7FFFFFFFLL) return fail(VA_ERANGE, "B or total too large");
+    if (sh->total == 0) return VA_OK;
+    if (!b->q || !b->k || !b->v || !b->cu || !b->out) return fail(VA_ENULL, "q, k, v, cu and out must be non-NULL");
+    if (!aligned(b->q, 16) || !aligned(b->k, 16) || !aligned(b->v, 16) || !aligned(b->out, 16))
+        return fail(VA_EALIGN, "q, k, v and out must be 16-byte aligned");
+    if (!aligned(b->cu, 4)) return fail(VA_EALIGN, "cu must be 4-byte aligned");
+    va::PrefillArgs a{};
+    a.q = b->q;
+    a.k = b->k;
+    a.v = b->v;
+    a.cu = b->cu;
+    a.out = b->out;
+    a.q_row = sh->q_row;
+    a.q_head = sh->q_head;
+    a.k_row = sh->k_row;
+    a.k_head = sh->k_head;
+    a.v_row = sh->v_row;
+    a.v_head = sh->v_head;
+    a.B = sh->B;
+    a.total = sh->total;
+    a.hq = sh->Hq;
+    a.group = sh->Hq / sh->Hkv;
+    a.qscale = (float)(1.4426950408889634074 / std::sqrt((double)sh->D));
+    const hipError_t e = va::launch_prefill(sh->D, a, as_stream(stream));
+    if (e != hipSuccess) return hip_fail(e, "prefill launch");
+    return VA_OK;
+}
+
+} // extern "C"
+
+namespace {
+
+// Checks of va_decode_tree's shape; the number of work-groups on success.
+int validate_tree(va_fmt fmt, const va_paged_shape* sh, int T, int* nwg) {
+    const int rc = validate_shape(fmt, sh, true);
+    if (rc) return rc;
+    if (T < 1 || T > VA_TREE_MAX) return fail(VA_EINVAL, "T must be in [1, %d] (got %d)", VA_TREE_MAX, T);
+    const long long rows = (long long)T * (sh->Hq / sh->Hkv);
+    if (rows > 1 << 20 || (long long)sh->B * T * sh->Hq > 0x7FFFFFFFLL / 64) return fail(VA_ERANGE, "B*T*Hq too large");
+    const int bm = va::tree_rows((int)rows), bn = va::tree_tile((int)rows);
+    const long long blocks = (long long)sh->B * sh->Hkv * ((rows + bm - 1) / bm);
+    const long long tiles = blocks * std::max(1LL, ((long long)sh->max_seq_len + bn - 1) / bn);
+    if (tiles > 0x7FFFFFFFLL) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", tiles);
+    *nwg = (int)std::min(tiles, (long long)va::tree_groups_per_cu((int)rows) * cus_or_default());
+    return VA_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+size_t va_tree_ws_bytes(va_fmt fmt, const va_paged_shape* sh, int T) {
+    int nwg = 0;
+    if (validate_tree(fmt, sh, T, &nwg)) return 0;
+    return (size_t)2 * nwg * va::tree_rows(T * (sh->Hq / sh->Hkv)) * (sh->D + 2) * sizeof(float);
+}
+
+int va_decode_tree(va_fmt fmt, const va_tree_bufs* b, const va_paged_shape* sh, int T, void* stream) {
+    int nwg = 0;
+    const int rc = validate_tree(fmt, sh, T, &nwg);
+    if (rc) return rc;
+    if (!b) return fail(VA_ENULL, "bufs is NULL");
+    const bool quant = !is_f16(fmt);
+    if (!b->k || !b->v || !b->q || !b->out || !b->ws || !b->block_table || !b->ctx_lens || !b->tree_mask)
+        return fail(VA_ENULL, "k, v, q, out, ws, block_table, ctx_lens and tree_mask must be non-NULL");
+    if (quant && (!b->sk || !b->sv)) return fail(VA_ENULL, "quantized formats need sk and sv");
+    const size_t kal = kind_of(fmt) == 3 ? 4 : 16;
+    if (!aligned(b->k, kal) || !aligned(b->v, kal)) return fail(VA_EALIGN, "k and v must be %zu-byte aligned", kal);
+    if (!aligned(b->q, 16) || !aligned(b->ws, 16)) return fail(VA_EALIGN, "q and ws must be 16-byte aligned");
+    if (!aligned(b->out, 8) || !aligned(b->tree_mask, 8)) return fail(VA_EALIGN, "out and tree_mask must be 8-byte aligned");
+    if (!aligned(b->block_table, 4) || !aligned(b->ctx_lens, 4) || !aligned(b->tree_sizes, 4))
+        return fail(VA_EALIGN, "block_table, ctx_lens or tree_sizes misaligned");
+    if (quant) {
+        const size_t sal = (sh->D / sh->G) >= 2 ? 4 : 2;
+        if (!aligned(b->sk, sal) || !aligned(b->sv, sal))
+            return fail(VA_EALIGN, "sk and sv must be %zu-byte aligned", sal);
+    }
+    va::TreeArgs a{};
+    a.k = static_cast<const uint8_t*>(b->k);
+    a.v = static_cast<const uint8_t*>(b->v);
+    a.sk = b->sk;
+    a.sv = b->sv;
+    a.block_table = b->block_table;
+    a.ctx_lens = b->ctx_lens;
+    a.sizes = b->tree_sizes;
+    a.mask = b->tree_mask;
+    a.q = b->q;
+    a.out = b->out;
+    a.ws = b->ws;
+    a.B = sh->B;
+    a.T = T;
+    a.hkv = sh->Hkv;
+    a.group = sh->Hq / sh->Hkv;
+    a.max_pages = sh->max_pages;
+    a.page_shift = log2i(sh->page_rows);
+    a.num_pages = sh->num_pages;
+    a.cap = sh->max_seq_len;
+    a.qscale = (float)(1.4426950408889634074 / std::sqrt((double)sh->D));
+    a.nwg = nwg;
+    a.min_share = 1;
+    const hipError_t e = va::launch_tree(kind_of(fmt), sh->D, is_f16(fmt) ? 64 : sh->G, a, as_stream(stream));
+    if (e != hipSuccess) return hip_fail(e, "tree launch");
+    return VA_OK;
+}
+
+} // extern "C"
+
+namespace {
+
+int validate_pages(int page_rows, int max_pages, int num_pages) {
+    if ((long long)max_pages * page_rows > 0x7FFFFFFFLL) return fail(VA_ERANGE, "max_pages*page_rows must stay below 2^31");
+    if (num_pages > 1 << 30) return fail(VA_ERANGE, "num_pages must be at most 2^30 (got %d)", num_pages);
+    return VA_OK;
+}
+
+// Checks of the pools, and the launch arguments that they and the shape give.
+int page_args(va_fmt fmt, const va_pools* p, const va_paged_shape* sh, va::PageArgs* a) {
+    int rc = validate_shape(fmt, sh, false);
+    if (rc == VA_OK) rc = validate_pages(sh->page_rows, sh->max_pages, sh->num_pages);
+    if (rc) return rc;
+    const bool quant = !is_f16(fmt);
+    if (!p || !p->k || !p->v || (quant && (!p->sk || !p->sv))) return fail(VA_ENULL, "the pools (and scales) must be non-NULL");
+    if (!aligned(p->k, quant ? 4 : 16) || !aligned(p->v, quant ? 4 : 16)) return fail(VA_EALIGN, "pages misaligned");
+    if (quant && (!aligned(p->sk, 2) || !aligned(p->sv, 2))) return fail(VA_EALIGN, "scales must be 2-byte aligned");
+    a->k = static_cast<uint8_t*>(p->k);
+    a->v = static_cast<uint8_t*>(p->v);
+    a->sk = reinterpret_cast<uint8_t*>(p->sk);
+    a->sv = reinterpret_cast<uint8_t*>(p->sv);
+    a->B = sh->B;
+    a->hkv = sh->Hkv;
+    a->page_rows = sh->page_rows;
+    a->max_pages = sh->max_pages;
+    a->num_pages = sh->num_pages;
+    a->row_bytes = (int)row_bytes(fmt, sh->D);
+    a->scale_bytes = quant ? sh->D / sh->G * 2 : 0;
+    a->wide = a->row_bytes % 16 == 0 && aligned(p->k, 16) && aligned(p->v, 16) && kind_of(fmt) != 3;
+    return VA_OK;
+}
+
+bool aligned4(std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if (!aligned(p, 4)) return false;
+    return true;
+}
+
+} // namespace
+
+extern "C" {
+
+int va_compact_kv(va_fmt fmt, const va_pools* pools, const va_paged_shape* sh, const int32_t* block_table,
+                  const int32_t* base, const int32_t* keep, const int32_t* counts, int n, void* stream) {
+    va::PageArgs a{};
+    const int rc = page_args(fmt, pools, sh, &a);
+    if (rc) return rc;
+    if (n < 0 || n > VA_TREE_MAX) return fail(VA_EINVAL, "n must be in [0, %d] (got %d)", VA_TREE_MAX, n);
+    if ((long long)sh->B * sh->Hkv > 0x7FFFFFFFLL) return fail(VA_ERANGE, "B*Hkv too large");
+    if (n == 0) return VA_OK;
+    if (!block_table || !base || !keep || !counts) return fail(VA_ENULL, "block_table, base, keep and counts must be non-NULL");
+    if (!aligned4({block_table, base, keep, counts})) return fail(VA_EALIGN, "block_table, base, keep or counts misaligned");
+    a.table = block_table;
+    a.lens = base;
+    a.keep = keep;
+    a.counts = counts;
+    a.n = n;
+    const hipError_t e = va::launch_compact(a, as_stream(stream));
+    if (e != hipSuccess) return hip_fail(e, "compact launch");
+    return VA_OK;
+}
+
+int va_fork_pages(va_fmt fmt, const va_pools* pools, const va_paged_shape* sh, const int32_t* block_table,
+                  const int32_t* seq_lens, const int32_t* parents, int children, int32_t* refs,
+                  int32_t* new_table, int32_t* new_lens, int32_t* missing, void* stream) {
+    va::PageArgs a{};
+    const int rc = page_args(fmt, pools, sh, &a);
+    if (rc) return rc;
+    if (children < 1) return fail(VA_EINVAL, "children must be >= 1 (got %d)", children);
+    if ((long long)children * sh->Hkv > 0x7FFFFFFFLL || (long long)children + sh->B > 0x7FFFFFF0LL)
+        return fail(VA_ERANGE, "too many sequences");
+    if (!block_table || !seq_lens || !parents || !refs || !new_table || !new_lens)
+        return fail(VA_ENULL, "block_table, seq_lens, parents, refs, new_table and new_lens must be non-NULL");
+    if (!aligned4({block_table, seq_lens, parents, refs, new_table, new_lens, missing}))
+        return fail(VA_EALIGN, "block_table, seq_lens, parents, refs, new_table, new_lens or missing misaligned");
+    if (new_table == block_table || new_lens == seq_lens)
+        return fail(VA_EINVAL, "new_table and new_lens must not be block_table and seq_lens");
+    a.table = block_table;
+    a.lens = seq_lens;
+    a.parents = parents;
+    a.children = children;
+    a.refs = refs;
+    a.new_table = new_table;
+    a.new_lens = new_lens;
+    a.missing = missing;
+    const hipError_t e = va::launch_fork(a, as_stream(stream));
+    if (e != hipSuccess) return hip_fail(e, "fork launch");
+    return VA_OK;
+}
+
+int va_resize_pages(int B, int page_rows, int max_pages, int num_pages, int32_t* block_table, int32_t* refs,
+                    const int32_t* old_lens, const int32_t* new_lens, int32_t* missing, void* stream) {
+    if (B < 1 || page_rows < 1 || max_pages < 1 || num_pages < 1)
+        return fail(VA_EINVAL, "B, page_rows, max_pages and num_pages must be >= 1");
+    if (B > 0x7FFFFFF0) return fail(VA_ERANGE, "too many sequences");
+    const int rc = validate_pages(page_rows, max_pages, num_pages);
+    if (rc) return rc;
+    if (!block_table || !refs || !old_lens || !new_lens)
+        return fail(VA_ENULL, "block_table, refs, old_lens and new_lens must be non-NULL");
+    if (!aligned4({block_table, refs, old_lens, new_lens, missing}))
+        return fail(VA_EALIGN, "block_table, refs, old_lens, new_lens or missing misaligned");
+    va::PageArgs a{};
+    a.table = block_table;
+    a.new_table = block_table;
+    a.lens = old_lens;
+    a.after = new_lens;
+    a.refs = refs;
+    a.missing = missing;
+    a.B = B;
+    a.page_rows = page_rows;
+    a.max_pages = max_pages;
+    a.num_pages = num_pages;
+    const hipError_t e = va::launch_resize(a, as_stream(stream));
+    if (e != hipSuccess) return hip_fail(e, "resize launch");
     return VA_OK;
 }
 

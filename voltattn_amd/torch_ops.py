@@ -7,6 +7,15 @@ Importing this module registers
 * ``voltattn::decode_gqa(...)`` — Hq query heads over Hkv KV heads (va_decode_gqa);
 * ``voltattn::decode_paged(...)`` — a batch over a page pool (va_decode_paged);
 * ``voltattn::append_kv(...)`` — quantize-and-append new rows (va_append_kv; mutates the pools);
+* ``voltattn::prefill(q, k, v, cu_seqlens) -> out`` — causal attention of packed prompts
+  (va_prefill);
+* ``voltattn::decode_tree(...)`` — drafted tokens over a page pool (va_decode_tree);
+* ``voltattn::compact_kv(...)`` — accepted drafts' rows moved together (va_compact_kv; mutates
+  the pools);
+* ``voltattn::fork_pages(...) -> (block_table, seq_lens, missing)`` — the next step's sequences
+  (va_fork_pages; mutates refs and the pools);
+* ``voltattn::resize_pages(...) -> missing`` — pages given up and handed out (va_resize_pages;
+  mutates block_table and refs);
 * ``voltattn::quantize(x, bits, group) -> (packed, scales)`` (va_quantize; the reference's
   quantize(), src/voltattn.cu:705-745);
 * ``voltattn::dequantize(packed, scales, bits, group) -> x`` (va_dequantize; the reference's
@@ -29,9 +38,11 @@ from typing import Optional
 
 import torch
 
-from . import (Fmt, _Bufs, _PagedBufs, _PagedShape, check, fmt_bits, lib, ws_bytes)
+from . import (TREE_MAX, Fmt, _Bufs, _PagedBufs, _PagedShape, _Pools, _PrefillBufs, _PrefillShape, _TreeBufs, check,
+               fmt_bits, lib, ws_bytes)
 
-__all__ = ["decode", "decode_gqa", "decode_paged", "append_kv", "quantize", "dequantize"]
+__all__ = ["decode", "decode_gqa", "decode_paged", "append_kv", "quantize", "dequantize",
+           "prefill", "decode_tree", "compact_kv", "fork_pages", "resize_pages"]
 
 
 # What an op does on the host per call is most of a small call's time: the names are
@@ -357,6 +368,253 @@ def dequantize(packed: torch.Tensor, scales: torch.Tensor, bits: int, group: int
 def _(packed, scales, bits, group=32):
     D = _validate_dequantize(packed, scales, bits, group)
     return packed.new_empty(packed.shape[:-1] + (D,), dtype=torch.float32)
+
+
+# ------------------------------------- prompts, drafted tokens, page pool --
+
+def _on_device(t: torch.Tensor, *others):
+    """Every tensor on t's device, which must be the current one: the library launches there."""
+    for x in (t, *others):
+        if x is None:
+            continue
+        if not x.is_cuda:
+            _fail("ops need tensors on a gfx950 device (no CPU fallback)")
+        if x.device != t.device:
+            _fail(f"tensors on {t.device} and {x.device}")
+    if t.device.index != torch.cuda.current_device():
+        _fail(f"tensors on {t.device}, but the current device is cuda:{torch.cuda.current_device()} (torch.cuda.device)")
+
+
+def _contiguous(**ts):
+    for name, t in ts.items():
+        if t is not None and not t.is_contiguous():
+            _fail(f"{name} must be contiguous")
+
+
+def _validate_prefill(q, k, v, cu) -> None:
+    if q.dim() != 3:
+        _fail(f"q must be [T, Hq, D] (got {tuple(q.shape)})")
+    T, Hq, D = q.shape
+    _expect(q, "q", (T, Hq, D), torch.float16)
+    _check((D == 64) | (D == 128), lambda: f"D must be 64 or 128 (got {D})")
+    if k.dim() != 3:
+        _fail(f"k must be [T, Hkv, D] (got {tuple(k.shape)})")
+    Hkv = k.shape[1]
+    _check(Hkv >= 1, lambda: f"k must have at least one head (got {Hkv})")
+    _check(Hq >= 1, lambda: f"q must have at least one head (got {Hq})")
+    _check(Hq % Hkv == 0, lambda: f"query heads ({Hq}) must be a multiple of K/V heads ({Hkv})")
+    _expect(k, "k", (T, Hkv, D), torch.float16)
+    _expect(v, "v", (T, Hkv, D), torch.float16)
+    if cu.dim() != 1:
+        _fail(f"cu_seqlens must be [B + 1] (got {tuple(cu.shape)})")
+    _expect(cu, "cu_seqlens", (cu.shape[0],), torch.int32)
+    _check(cu.shape[0] >= 2, lambda: f"cu_seqlens must be [B + 1] with B >= 1 (got {tuple(cu.shape)})")
+
+
+def _strides(name: str, t: torch.Tensor):
+    """(row, head) strides; the last dimension must be dense. The stride of a dimension of one is free."""
+    T, H, D = t.shape
+    row, head, last = t.stride()
+    if last != 1:
+        _fail(f"{name} must be dense in its last dimension (stride {last})")
+    if H == 1:
+        head = 0
+    if T <= 1:
+        row = max(head * H, D)
+    return row, head
+
+
+@torch.library.custom_op("voltattn::prefill", mutates_args=())
+def prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor) -> torch.Tensor:
+    """q fp16 [T, Hq, D]; k, v fp16 [T, Hkv, D], dense in D only (slices of a fused projection);
+    cu_seqlens int32 [B + 1]: rows cu[b] .. cu[b+1] - 1 are prompt b. out [T, Hq, D], zeros in rows of no prompt."""
+    _validate_prefill(q, k, v, cu_seqlens)
+    _on_device(q, k, v, cu_seqlens)
+    _contiguous(cu_seqlens=cu_seqlens)
+    T, Hq, D = q.shape
+    out = torch.empty((T, Hq, D), dtype=torch.float16, device=q.device)
+    if T == 0:
+        return out
+    shape = _PrefillShape(cu_seqlens.shape[0] - 1, T, Hq, k.shape[1], D, *_strides("q", q), *_strides("k", k),
+                          *_strides("v", v))
+    b = _PrefillBufs(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr())
+    check(lib.va_prefill(C.byref(b), C.byref(shape), _stream(q)))
+    return out
+
+
+@prefill.register_fake
+def _(q, k, v, cu_seqlens):
+    _validate_prefill(q, k, v, cu_seqlens)
+    return q.new_empty(q.shape, dtype=torch.float16)
+
+
+def _validate_tree(q, kp, vp, ksp, vsp, block_table, ctx_lens, sizes, mask, f: Fmt, group: int) -> None:
+    if q.dim() != 4:
+        _fail(f"q must be [B, T, Hq, D] (got {tuple(q.shape)})")
+    B, T, Hq, D = q.shape
+    _validate_paged(q[:, 0] if T != 0 else q.new_empty((B, Hq, D)), kp, vp, ksp, vsp, block_table, ctx_lens, f, group)
+    _check((T >= 1) & (T <= TREE_MAX), lambda: f"T must be 1 .. {TREE_MAX} (got {T})")
+    if sizes is not None:
+        _expect(sizes, "tree_sizes", (B,), torch.int32)
+    _expect(mask, "tree_mask", (B, T), torch.int64)
+
+
+@torch.library.custom_op("voltattn::decode_tree", mutates_args=())
+def decode_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: Optional[torch.Tensor],
+                v_scale_pages: Optional[torch.Tensor], block_table: torch.Tensor, ctx_lens: torch.Tensor,
+                tree_sizes: Optional[torch.Tensor], tree_mask: torch.Tensor, fmt: str, max_seq_len: int,
+                group: int = 32) -> torch.Tensor:
+    """q fp16 [B, T, Hq, D]; pages [num_pages, Hkv, page_rows, ...]; ctx_lens int32 [B]; tree_sizes int32 [B] or
+    None (T each); tree_mask int64 [B, T]: bit j of entry i: draft i attends draft j, whose rows are position
+    ctx_lens[b] + j. max_seq_len >= every context and its drafts."""
+    f = _fmt(fmt)
+    _validate_tree(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask, f,
+                   group)
+    _on_device(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask)
+    _contiguous(q=q, k_pages=k_pages, v_pages=v_pages, k_scale_pages=k_scale_pages, v_scale_pages=v_scale_pages,
+                block_table=block_table, ctx_lens=ctx_lens, tree_sizes=tree_sizes, tree_mask=tree_mask)
+    B, T, Hq, D = q.shape
+    num_pages, Hkv, page_rows = k_pages.shape[:3]
+    shape = _PagedShape(B, Hq, Hkv, D, group, page_rows, block_table.shape[1], num_pages, max_seq_len)
+    nbytes = lib.va_tree_ws_bytes(int(f), C.byref(shape), T)
+    out = torch.empty_like(q)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
+    b = _TreeBufs(_ptr(k_pages), _ptr(v_pages), _ptr(k_scale_pages), _ptr(v_scale_pages), _ptr(block_table),
+                  _ptr(ctx_lens), _ptr(tree_sizes), _ptr(tree_mask), _ptr(q), _ptr(out), _ptr(ws))
+    check(lib.va_decode_tree(int(f), C.byref(b), C.byref(shape), T, _stream(q)))
+    return out
+
+
+@decode_tree.register_fake
+def _(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask, fmt,
+      max_seq_len, group=32):
+    _validate_tree(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask,
+                   _fmt(fmt), group)
+    return q.new_empty(q.shape, dtype=torch.float16)
+
+
+def _validate_pools(kp, vp, ksp, vsp, block_table, f: Fmt, group: int) -> None:
+    """Pools [num_pages, Hkv, page_rows, row] and block_table [B, max_pages]."""
+    if kp.dim() != 4:
+        _fail(f"k_pages must be [num_pages, Hkv, page_rows, row] (got {tuple(kp.shape)})")
+    row = kp.shape[-1]
+    D = row if fmt_bits(f) == 16 else row * 8 // fmt_bits(f)
+    _check_dg(f, D, group)
+    _check_kv(f, kp, vp, ksp, vsp, tuple(kp.shape[:3]), D, group)
+    if block_table.dim() != 2:
+        _fail(f"block_table must be [B, max_pages] (got {tuple(block_table.shape)})")
+    _expect(block_table, "block_table", tuple(block_table.shape), torch.int32)
+
+
+def _pools(kp, vp, ksp, vsp, block_table, f: Fmt, group: int):
+    """(va_pools, va_paged_shape) of checked tensors."""
+    num_pages, Hkv, page_rows, row = kp.shape
+    D = row if fmt_bits(f) == 16 else row * 8 // fmt_bits(f)
+    return (_Pools(_ptr(kp), _ptr(vp), _ptr(ksp), _ptr(vsp)),
+            _PagedShape(block_table.shape[0], Hkv, Hkv, D, group, page_rows, block_table.shape[1], num_pages, 0))
+
+
+def _validate_compact(kp, vp, ksp, vsp, block_table, base, keep, counts, f: Fmt, group: int) -> None:
+    _validate_pools(kp, vp, ksp, vsp, block_table, f, group)
+    B = block_table.shape[0]
+    _expect(base, "base", (B,), torch.int32)
+    if keep.dim() != 2:
+        _fail(f"keep must be [B={B}, n] (got {tuple(keep.shape)})")
+    _expect(keep, "keep", (B, keep.shape[1]), torch.int32)
+    _check(keep.shape[1] <= TREE_MAX, lambda: f"keep holds at most {TREE_MAX} rows a sequence (got {keep.shape[1]})")
+    _expect(counts, "counts", (B,), torch.int32)
+
+
+@torch.library.custom_op("voltattn::compact_kv", mutates_args=("k_pages", "v_pages", "k_scale_pages", "v_scale_pages"))
+def compact_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: Optional[torch.Tensor],
+               v_scale_pages: Optional[torch.Tensor], block_table: torch.Tensor, base: torch.Tensor,
+               keep: torch.Tensor, counts: torch.Tensor, fmt: str, group: int = 32) -> None:
+    """For i < counts[b], row base[b] + i of sequence b becomes what row base[b] + keep[b, i] was (K, V, scales)."""
+    f = _fmt(fmt)
+    _validate_compact(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, f, group)
+    _on_device(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts)
+    _contiguous(k_pages=k_pages, v_pages=v_pages, k_scale_pages=k_scale_pages, v_scale_pages=v_scale_pages,
+                block_table=block_table, base=base, keep=keep, counts=counts)
+    p, shape = _pools(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, f, group)
+    check(lib.va_compact_kv(int(f), C.byref(p), C.byref(shape), _ptr(block_table), _ptr(base), _ptr(keep),
+                            _ptr(counts), keep.shape[1], _stream(k_pages)))
+
+
+@compact_kv.register_fake
+def _(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, fmt, group=32):
+    _validate_compact(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, _fmt(fmt), group)
+    return None
+
+
+def _validate_fork(block_table, seq_lens, parents, refs, kp, vp, ksp, vsp, f: Fmt, group: int) -> None:
+    _validate_pools(kp, vp, ksp, vsp, block_table, f, group)
+    _expect(seq_lens, "seq_lens", (block_table.shape[0],), torch.int32)
+    if parents.dim() != 1:
+        _fail(f"parents must be [children] (got {tuple(parents.shape)})")
+    _expect(parents, "parents", tuple(parents.shape), torch.int32)
+    _expect(refs, "refs", (kp.shape[0],), torch.int32)
+
+
+@torch.library.custom_op("voltattn::fork_pages", mutates_args=("refs", "k_pages", "v_pages", "k_scale_pages",
+                                                               "v_scale_pages"))
+def fork_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor,
+               k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: Optional[torch.Tensor],
+               v_scale_pages: Optional[torch.Tensor], fmt: str,
+               group: int = 32) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The next step's sequences: child c continues sequence parents[c] (int32 [children]), sharing its full pages
+    (refs int32 [num_pages] counts the holders) and with a last page of its own. Returns (block_table
+    [children, max_pages], seq_lens [children], missing [1]: pages that the pool did not have)."""
+    f = _fmt(fmt)
+    _validate_fork(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, f, group)
+    _on_device(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    _contiguous(block_table=block_table, seq_lens=seq_lens, parents=parents, refs=refs, k_pages=k_pages,
+                v_pages=v_pages, k_scale_pages=k_scale_pages, v_scale_pages=v_scale_pages)
+    p, shape = _pools(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, f, group)
+    n = parents.shape[0]
+    table = block_table.new_empty((n, block_table.shape[1]))
+    lens, missing = block_table.new_empty((n,)), block_table.new_empty((1,))
+    check(lib.va_fork_pages(int(f), C.byref(p), C.byref(shape), _ptr(block_table), _ptr(seq_lens), _ptr(parents), n,
+                            _ptr(refs), _ptr(table), _ptr(lens), _ptr(missing), _stream(block_table)))
+    return table, lens, missing
+
+
+@fork_pages.register_fake
+def _(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, fmt, group=32):
+    _validate_fork(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, _fmt(fmt), group)
+    n = parents.shape[0]
+    return block_table.new_empty((n, block_table.shape[1])), block_table.new_empty((n,)), block_table.new_empty((1,))
+
+
+def _validate_resize(block_table, refs, old_lens, new_lens, page_rows) -> None:
+    if block_table.dim() != 2:
+        _fail(f"block_table must be [B, max_pages] (got {tuple(block_table.shape)})")
+    _expect(block_table, "block_table", tuple(block_table.shape), torch.int32)
+    if refs.dim() != 1:
+        _fail(f"refs must be [num_pages] (got {tuple(refs.shape)})")
+    _expect(refs, "refs", tuple(refs.shape), torch.int32)
+    _expect(old_lens, "old_lens", (block_table.shape[0],), torch.int32)
+    _expect(new_lens, "new_lens", (block_table.shape[0],), torch.int32)
+    _check(page_rows >= 1, lambda: f"page_rows must be >= 1 (got {page_rows})")
+
+
+@torch.library.custom_op("voltattn::resize_pages", mutates_args=("block_table", "refs"))
+def resize_pages(block_table: torch.Tensor, refs: torch.Tensor, old_lens: torch.Tensor, new_lens: torch.Tensor,
+                 page_rows: int) -> torch.Tensor:
+    """Every sequence from old_lens[b] to new_lens[b] positions: pages no longer held are given up (0 frees the
+    sequence), missing ones handed out, lowest free id (refs 0) first. Returns how many the pool did not have, [1]."""
+    _validate_resize(block_table, refs, old_lens, new_lens, page_rows)
+    _on_device(block_table, refs, old_lens, new_lens)
+    _contiguous(block_table=block_table, refs=refs, old_lens=old_lens, new_lens=new_lens)
+    missing = block_table.new_empty((1,))
+    check(lib.va_resize_pages(block_table.shape[0], page_rows, block_table.shape[1], refs.shape[0], _ptr(block_table),
+                              _ptr(refs), _ptr(old_lens), _ptr(new_lens), _ptr(missing), _stream(block_table)))
+    return missing
+
+
+@resize_pages.register_fake
+def _(block_table, refs, old_lens, new_lens, page_rows):
+    _validate_resize(block_table, refs, old_lens, new_lens, page_rows)
+    return block_table.new_empty((1,))
 
 
 def row_format_bits(fmt: str) -> int:
