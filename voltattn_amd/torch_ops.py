@@ -49,6 +49,7 @@ __all__ = ["decode", "decode_gqa", "decode_paged", "append_kv", "quantize", "deq
 # looked up once, plain sizes are compared without torch._check, and the stream handle
 # is read directly (decode_paged 45 -> 25 us per call, append_kv 35 -> 20).
 _FMTS = {f.label: f for f in Fmt}
+_BITS = [fmt_bits(f) for f in Fmt]
 
 
 def _fmt(name: str) -> Fmt:
@@ -94,6 +95,8 @@ def _check(cond, msg) -> None:
 
 
 def _expect(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> None:
+    if type(t) is torch.Tensor and t.shape == shape and t.dtype == dtype:
+        return                               # plain sizes only: a traced tensor has another type
     if t is None:
         _fail(f"{name} is required")
     if t.dim() != len(shape):
@@ -106,7 +109,7 @@ def _expect(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> Non
 
 def _check_dg(f: Fmt, D, group: int) -> None:
     _check((D == 64) | (D == 128), lambda: f"D must be 64 or 128 (got {D})")
-    if fmt_bits(f) != 16:
+    if _BITS[f] != 16:
         if group not in (32, 64):
             _fail(f"group must be 32 or 64 (got {group})")
         _check(D >= group, lambda: f"group must be <= D (got {group}, D={D})")
@@ -115,9 +118,9 @@ def _check_dg(f: Fmt, D, group: int) -> None:
 def _row_shape(f: Fmt, D) -> tuple[tuple, torch.dtype]:
     """Trailing shape and dtype of one K/V row of format f: fp16 [D] for the f16
     formats, uint8 [row bytes] for the quantized ones."""
-    if fmt_bits(f) == 16:
+    if _BITS[f] == 16:
         return (D,), torch.float16
-    return (D * fmt_bits(f) // 8,), torch.uint8
+    return (D * _BITS[f] // 8,), torch.uint8
 
 
 def _check_kv(f: Fmt, k, v, ks, vs, lead: tuple, D, group: int) -> None:
@@ -125,7 +128,7 @@ def _check_kv(f: Fmt, k, v, ks, vs, lead: tuple, D, group: int) -> None:
     tail, dt = _row_shape(f, D)
     _expect(k, "k", lead + tail, dt)
     _expect(v, "v", lead + tail, dt)
-    if fmt_bits(f) != 16:
+    if _BITS[f] != 16:
         _expect(ks, "k_scale", lead + (D // group,), torch.float16)
         _expect(vs, "v_scale", lead + (D // group,), torch.float16)
 
@@ -178,7 +181,7 @@ def _validate_append(x, start, block_table, pages, scale_pages, f: Fmt, group: i
     _check(Hp == Hkv, lambda: f"pages hold {Hp} K/V heads, x has {Hkv}")
     tail, dt = _row_shape(f, D)
     _expect(pages, "pages", (num_pages, Hkv, page_rows) + tail, dt)
-    if fmt_bits(f) != 16:
+    if _BITS[f] != 16:
         _expect(scale_pages, "scale_pages", (num_pages, Hkv, page_rows, D // group), torch.float16)
     _expect(start, "start", (B,), torch.int32)
     if block_table.dim() != 2:
@@ -372,23 +375,44 @@ def _(packed, scales, bits, group=32):
 
 # ------------------------------------- prompts, drafted tokens, page pool --
 
-def _on_device(t: torch.Tensor, *others):
-    """Every tensor on t's device, which must be the current one: the library launches there."""
-    for x in (t, *others):
-        if x is None:
-            continue
-        if not x.is_cuda:
-            _fail("ops need tensors on a gfx950 device (no CPU fallback)")
-        if x.device != t.device:
+# Registered through the dispatcher directly: per call torch.library.custom_op takes 15 us on
+# the host, more than most of these kernels run for, this 4. One implementation for every
+# device, so that CPU tensors meet the ops' own error.
+_LIBRARY = torch.library.Library("voltattn", "FRAGMENT")
+
+
+def _op(schema: str, fake):
+    """Registers the decorated function and its fake implementation; what it returns is the op."""
+    name = schema.split("(")[0]
+
+    def register(fn):
+        _LIBRARY.define(schema)
+        _LIBRARY.impl(name, fn, "CompositeExplicitAutograd")
+        torch.library.register_fake(f"voltattn::{name}", fake, lib=_LIBRARY)
+        op = getattr(torch.ops.voltattn, name)
+        op.__doc__ = fn.__doc__
+        return op
+
+    return register
+
+
+def _on_device(t: torch.Tensor, *others) -> int:
+    """The stream to launch on: every tensor is on t's device, which must be the current one."""
+    at = t.get_device()                                     # -1: not on a GPU
+    for x in others:
+        if x is not None and x.get_device() != at:
             _fail(f"tensors on {t.device} and {x.device}")
-    if t.device.index != torch.cuda.current_device():
-        _fail(f"tensors on {t.device}, but the current device is cuda:{torch.cuda.current_device()} (torch.cuda.device)")
+    if at < 0 or not t.is_cuda:
+        _fail("ops need tensors on a gfx950 device (no CPU fallback)")
+    if at != torch._C._cuda_getDevice():
+        _fail(f"tensors on {t.device}, but the current device is cuda:{torch._C._cuda_getDevice()} (torch.cuda.device)")
+    return torch._C._cuda_getCurrentRawStream(at)
 
 
-def _contiguous(**ts):
-    for name, t in ts.items():
+def _contiguous(*ts) -> None:
+    for t in ts:
         if t is not None and not t.is_contiguous():
-            _fail(f"{name} must be contiguous")
+            _fail(f"a tensor of shape {tuple(t.shape)} must be contiguous")
 
 
 def _validate_prefill(q, k, v, cu) -> None:
@@ -424,13 +448,18 @@ def _strides(name: str, t: torch.Tensor):
     return row, head
 
 
-@torch.library.custom_op("voltattn::prefill", mutates_args=())
+def _prefill_fake(q, k, v, cu_seqlens):
+    _validate_prefill(q, k, v, cu_seqlens)
+    return q.new_empty(q.shape, dtype=torch.float16)
+
+
+@_op("prefill(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens) -> Tensor", _prefill_fake)
 def prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor) -> torch.Tensor:
     """q fp16 [T, Hq, D]; k, v fp16 [T, Hkv, D], dense in D only (slices of a fused projection);
     cu_seqlens int32 [B + 1]: rows cu[b] .. cu[b+1] - 1 are prompt b. out [T, Hq, D], zeros in rows of no prompt."""
     _validate_prefill(q, k, v, cu_seqlens)
-    _on_device(q, k, v, cu_seqlens)
-    _contiguous(cu_seqlens=cu_seqlens)
+    stream = _on_device(q, k, v, cu_seqlens)
+    _contiguous(cu_seqlens)
     T, Hq, D = q.shape
     out = torch.empty((T, Hq, D), dtype=torch.float16, device=q.device)
     if T == 0:
@@ -438,28 +467,41 @@ def prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch
     shape = _PrefillShape(cu_seqlens.shape[0] - 1, T, Hq, k.shape[1], D, *_strides("q", q), *_strides("k", k),
                           *_strides("v", v))
     b = _PrefillBufs(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr())
-    check(lib.va_prefill(C.byref(b), C.byref(shape), _stream(q)))
+    check(lib.va_prefill(C.byref(b), C.byref(shape), stream))
     return out
-
-
-@prefill.register_fake
-def _(q, k, v, cu_seqlens):
-    _validate_prefill(q, k, v, cu_seqlens)
-    return q.new_empty(q.shape, dtype=torch.float16)
 
 
 def _validate_tree(q, kp, vp, ksp, vsp, block_table, ctx_lens, sizes, mask, f: Fmt, group: int) -> None:
     if q.dim() != 4:
         _fail(f"q must be [B, T, Hq, D] (got {tuple(q.shape)})")
     B, T, Hq, D = q.shape
-    _validate_paged(q[:, 0] if T != 0 else q.new_empty((B, Hq, D)), kp, vp, ksp, vsp, block_table, ctx_lens, f, group)
+    _expect(q, "q", (B, T, Hq, D), torch.float16)
     _check((T >= 1) & (T <= TREE_MAX), lambda: f"T must be 1 .. {TREE_MAX} (got {T})")
+    _check_dg(f, D, group)
+    if kp.dim() != 4:
+        _fail(f"k_pages must be [num_pages, Hkv, page_rows, row] (got {tuple(kp.shape)})")
+    num_pages, Hkv, page_rows, _ = kp.shape
+    _check(Hkv >= 1, lambda: f"k_pages must have at least one head (got {Hkv})")
+    _check(Hq % Hkv == 0, lambda: f"query heads ({Hq}) must be a multiple of K/V heads ({Hkv})")
+    _check_kv(f, kp, vp, ksp, vsp, (num_pages, Hkv, page_rows), D, group)
+    if block_table.dim() != 2:
+        _fail(f"block_table must be [B={B}, max_pages] (got {tuple(block_table.shape)})")
+    _expect(block_table, "block_table", (B, block_table.shape[1]), torch.int32)
+    _expect(ctx_lens, "ctx_lens", (B,), torch.int32)
     if sizes is not None:
         _expect(sizes, "tree_sizes", (B,), torch.int32)
     _expect(mask, "tree_mask", (B, T), torch.int64)
 
 
-@torch.library.custom_op("voltattn::decode_tree", mutates_args=())
+def _decode_tree_fake(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask, fmt,
+      max_seq_len, group=32):
+    _validate_tree(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask,
+                   _fmt(fmt), group)
+    return q.new_empty(q.shape, dtype=torch.float16)
+
+
+@_op("decode_tree(Tensor q, Tensor k_pages, Tensor v_pages, Tensor? k_scale_pages, Tensor? v_scale_pages, Tensor block_table, "
+     "Tensor ctx_lens, Tensor? tree_sizes, Tensor tree_mask, str fmt, SymInt max_seq_len, int group=32) -> Tensor", _decode_tree_fake)
 def decode_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: Optional[torch.Tensor],
                 v_scale_pages: Optional[torch.Tensor], block_table: torch.Tensor, ctx_lens: torch.Tensor,
                 tree_sizes: Optional[torch.Tensor], tree_mask: torch.Tensor, fmt: str, max_seq_len: int,
@@ -470,9 +512,9 @@ def decode_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k
     f = _fmt(fmt)
     _validate_tree(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask, f,
                    group)
-    _on_device(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask)
-    _contiguous(q=q, k_pages=k_pages, v_pages=v_pages, k_scale_pages=k_scale_pages, v_scale_pages=v_scale_pages,
-                block_table=block_table, ctx_lens=ctx_lens, tree_sizes=tree_sizes, tree_mask=tree_mask)
+    stream = _on_device(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask)
+    _contiguous(q, k_pages, v_pages, k_scale_pages, v_scale_pages,
+                block_table, ctx_lens, tree_sizes, tree_mask)
     B, T, Hq, D = q.shape
     num_pages, Hkv, page_rows = k_pages.shape[:3]
     shape = _PagedShape(B, Hq, Hkv, D, group, page_rows, block_table.shape[1], num_pages, max_seq_len)
@@ -481,16 +523,8 @@ def decode_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k
     ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
     b = _TreeBufs(_ptr(k_pages), _ptr(v_pages), _ptr(k_scale_pages), _ptr(v_scale_pages), _ptr(block_table),
                   _ptr(ctx_lens), _ptr(tree_sizes), _ptr(tree_mask), _ptr(q), _ptr(out), _ptr(ws))
-    check(lib.va_decode_tree(int(f), C.byref(b), C.byref(shape), T, _stream(q)))
+    check(lib.va_decode_tree(int(f), C.byref(b), C.byref(shape), T, stream))
     return out
-
-
-@decode_tree.register_fake
-def _(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask, fmt,
-      max_seq_len, group=32):
-    _validate_tree(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask,
-                   _fmt(fmt), group)
-    return q.new_empty(q.shape, dtype=torch.float16)
 
 
 def _validate_pools(kp, vp, ksp, vsp, block_table, f: Fmt, group: int) -> None:
@@ -498,7 +532,7 @@ def _validate_pools(kp, vp, ksp, vsp, block_table, f: Fmt, group: int) -> None:
     if kp.dim() != 4:
         _fail(f"k_pages must be [num_pages, Hkv, page_rows, row] (got {tuple(kp.shape)})")
     row = kp.shape[-1]
-    D = row if fmt_bits(f) == 16 else row * 8 // fmt_bits(f)
+    D = row if _BITS[f] == 16 else row * 8 // _BITS[f]
     _check_dg(f, D, group)
     _check_kv(f, kp, vp, ksp, vsp, tuple(kp.shape[:3]), D, group)
     if block_table.dim() != 2:
@@ -509,7 +543,7 @@ def _validate_pools(kp, vp, ksp, vsp, block_table, f: Fmt, group: int) -> None:
 def _pools(kp, vp, ksp, vsp, block_table, f: Fmt, group: int):
     """(va_pools, va_paged_shape) of checked tensors."""
     num_pages, Hkv, page_rows, row = kp.shape
-    D = row if fmt_bits(f) == 16 else row * 8 // fmt_bits(f)
+    D = row if _BITS[f] == 16 else row * 8 // _BITS[f]
     return (_Pools(_ptr(kp), _ptr(vp), _ptr(ksp), _ptr(vsp)),
             _PagedShape(block_table.shape[0], Hkv, Hkv, D, group, page_rows, block_table.shape[1], num_pages, 0))
 
@@ -525,25 +559,25 @@ def _validate_compact(kp, vp, ksp, vsp, block_table, base, keep, counts, f: Fmt,
     _expect(counts, "counts", (B,), torch.int32)
 
 
-@torch.library.custom_op("voltattn::compact_kv", mutates_args=("k_pages", "v_pages", "k_scale_pages", "v_scale_pages"))
+def _compact_kv_fake(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, fmt, group=32):
+    _validate_compact(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, _fmt(fmt), group)
+    return None
+
+
+@_op("compact_kv(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scale_pages, Tensor(d!)? v_scale_pages, "
+     "Tensor block_table, Tensor base, Tensor keep, Tensor counts, str fmt, int group=32) -> ()", _compact_kv_fake)
 def compact_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: Optional[torch.Tensor],
                v_scale_pages: Optional[torch.Tensor], block_table: torch.Tensor, base: torch.Tensor,
                keep: torch.Tensor, counts: torch.Tensor, fmt: str, group: int = 32) -> None:
     """For i < counts[b], row base[b] + i of sequence b becomes what row base[b] + keep[b, i] was (K, V, scales)."""
     f = _fmt(fmt)
     _validate_compact(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, f, group)
-    _on_device(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts)
-    _contiguous(k_pages=k_pages, v_pages=v_pages, k_scale_pages=k_scale_pages, v_scale_pages=v_scale_pages,
-                block_table=block_table, base=base, keep=keep, counts=counts)
+    stream = _on_device(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts)
+    _contiguous(k_pages, v_pages, k_scale_pages, v_scale_pages,
+                block_table, base, keep, counts)
     p, shape = _pools(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, f, group)
     check(lib.va_compact_kv(int(f), C.byref(p), C.byref(shape), _ptr(block_table), _ptr(base), _ptr(keep),
-                            _ptr(counts), keep.shape[1], _stream(k_pages)))
-
-
-@compact_kv.register_fake
-def _(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, fmt, group=32):
-    _validate_compact(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, _fmt(fmt), group)
-    return None
+                            _ptr(counts), keep.shape[1], stream))
 
 
 def _validate_fork(block_table, seq_lens, parents, refs, kp, vp, ksp, vsp, f: Fmt, group: int) -> None:
@@ -555,8 +589,14 @@ def _validate_fork(block_table, seq_lens, parents, refs, kp, vp, ksp, vsp, f: Fm
     _expect(refs, "refs", (kp.shape[0],), torch.int32)
 
 
-@torch.library.custom_op("voltattn::fork_pages", mutates_args=("refs", "k_pages", "v_pages", "k_scale_pages",
-                                                               "v_scale_pages"))
+def _fork_pages_fake(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, fmt, group=32):
+    _validate_fork(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, _fmt(fmt), group)
+    n = parents.shape[0]
+    return block_table.new_empty((n, block_table.shape[1])), block_table.new_empty((n,)), block_table.new_empty((1,))
+
+
+@_op("fork_pages(Tensor block_table, Tensor seq_lens, Tensor parents, Tensor(a!) refs, Tensor(b!) k_pages, Tensor(c!) v_pages, "
+     "Tensor(d!)? k_scale_pages, Tensor(e!)? v_scale_pages, str fmt, int group=32) -> (Tensor, Tensor, Tensor)", _fork_pages_fake)
 def fork_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor,
                k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: Optional[torch.Tensor],
                v_scale_pages: Optional[torch.Tensor], fmt: str,
@@ -566,23 +606,16 @@ def fork_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch
     [children, max_pages], seq_lens [children], missing [1]: pages that the pool did not have)."""
     f = _fmt(fmt)
     _validate_fork(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, f, group)
-    _on_device(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages)
-    _contiguous(block_table=block_table, seq_lens=seq_lens, parents=parents, refs=refs, k_pages=k_pages,
-                v_pages=v_pages, k_scale_pages=k_scale_pages, v_scale_pages=v_scale_pages)
+    stream = _on_device(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    _contiguous(block_table, seq_lens, parents, refs, k_pages,
+                v_pages, k_scale_pages, v_scale_pages)
     p, shape = _pools(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, f, group)
     n = parents.shape[0]
     table = block_table.new_empty((n, block_table.shape[1]))
     lens, missing = block_table.new_empty((n,)), block_table.new_empty((1,))
     check(lib.va_fork_pages(int(f), C.byref(p), C.byref(shape), _ptr(block_table), _ptr(seq_lens), _ptr(parents), n,
-                            _ptr(refs), _ptr(table), _ptr(lens), _ptr(missing), _stream(block_table)))
+                            _ptr(refs), _ptr(table), _ptr(lens), _ptr(missing), stream))
     return table, lens, missing
-
-
-@fork_pages.register_fake
-def _(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, fmt, group=32):
-    _validate_fork(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, _fmt(fmt), group)
-    n = parents.shape[0]
-    return block_table.new_empty((n, block_table.shape[1])), block_table.new_empty((n,)), block_table.new_empty((1,))
 
 
 def _validate_resize(block_table, refs, old_lens, new_lens, page_rows) -> None:
@@ -597,25 +630,24 @@ def _validate_resize(block_table, refs, old_lens, new_lens, page_rows) -> None:
     _check(page_rows >= 1, lambda: f"page_rows must be >= 1 (got {page_rows})")
 
 
-@torch.library.custom_op("voltattn::resize_pages", mutates_args=("block_table", "refs"))
+def _resize_pages_fake(block_table, refs, old_lens, new_lens, page_rows):
+    _validate_resize(block_table, refs, old_lens, new_lens, page_rows)
+    return block_table.new_empty((1,))
+
+
+@_op("resize_pages(Tensor(a!) block_table, Tensor(b!) refs, Tensor old_lens, Tensor new_lens, SymInt page_rows) -> Tensor", _resize_pages_fake)
 def resize_pages(block_table: torch.Tensor, refs: torch.Tensor, old_lens: torch.Tensor, new_lens: torch.Tensor,
                  page_rows: int) -> torch.Tensor:
     """Every sequence from old_lens[b] to new_lens[b] positions: pages no longer held are given up (0 frees the
     sequence), missing ones handed out, lowest free id (refs 0) first. Returns how many the pool did not have, [1]."""
     _validate_resize(block_table, refs, old_lens, new_lens, page_rows)
-    _on_device(block_table, refs, old_lens, new_lens)
-    _contiguous(block_table=block_table, refs=refs, old_lens=old_lens, new_lens=new_lens)
+    stream = _on_device(block_table, refs, old_lens, new_lens)
+    _contiguous(block_table, refs, old_lens, new_lens)
     missing = block_table.new_empty((1,))
     check(lib.va_resize_pages(block_table.shape[0], page_rows, block_table.shape[1], refs.shape[0], _ptr(block_table),
-                              _ptr(refs), _ptr(old_lens), _ptr(new_lens), _ptr(missing), _stream(block_table)))
+                              _ptr(refs), _ptr(old_lens), _ptr(new_lens), _ptr(missing), stream))
     return missing
 
 
-@resize_pages.register_fake
-def _(block_table, refs, old_lens, new_lens, page_rows):
-    _validate_resize(block_table, refs, old_lens, new_lens, page_rows)
-    return block_table.new_empty((1,))
-
-
 def row_format_bits(fmt: str) -> int:
-    return fmt_bits(_fmt(fmt))
+    return _BITS[_fmt(fmt)]
