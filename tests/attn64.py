@@ -8,6 +8,8 @@ result may be off, each rounding by at most half a step of its type:
   weight is off by that share twice (its own score's and the maximum's), and by 2^-22 for exp2;
 * a weight (times V's group scale) is rounded to fp16: 2^-11 of it, or 2^-25 absolutely where
   fp16 has no finer step, in units of the largest weight, which is at least 1;
+* where a kernel rounds V's values to fp16 (v_rounded: code times scale, a product of 8 and 11 bits,
+  in 11), each is off by 2^-11 of itself, the sum of weights times values by 2^-11 of sum p|v| more;
 * the sums over n positions are off by 2^-24 of sum p|v| for each addition;
 * the result is rounded to fp16: 2^-11 of it, or 2^-25.
 """
@@ -16,7 +18,7 @@ import math
 import torch
 
 
-def attend(q, k, v, seen, scale_v=None):
+def attend(q, k, v, seen, scale_v=None, v_rounded=False):
     """q [R, D], k and v [n, D] (exact values), seen [R, n] booleans; scale_v [n, D]: the group scale
     under each value of v (1 where there are none). float64 (out, bound), zeros where nothing is seen."""
     q, k, v = q.double(), k.double(), v.double()
@@ -34,7 +36,7 @@ def attend(q, k, v, seen, scale_v=None):
     sv = torch.ones_like(v) if scale_v is None else scale_v.double()
     code = torch.where(sv == 0, torch.zeros_like(v), v / sv).abs()
     fine = seen.double() @ code * 2.0 ** -25 / total                 # weights below fp16's smallest normal one
-    bound = (2.0 ** -11 + 2.0 ** -24 * (n + 64) + e_score) * size + fine + 2.0 ** -11 * out.abs() + 2.0 ** -25
+    bound = (2.0 ** -11 * (2 if v_rounded else 1) + 2.0 ** -24 * (n + 64) + e_score) * size + fine + 2.0 ** -11 * out.abs() + 2.0 ** -25
     return out, bound
 
 

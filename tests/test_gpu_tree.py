@@ -81,6 +81,8 @@ class Case:
 
     def check(self, got, skip=()):
         g = self.Hq // self.Hkv
+        # over 64 query rows to a K/V head the kernel rounds dequantized V values to fp16
+        rounded = self.bits != 16 and self.T * g > 64
         for b in range(len(self.ctx)):
             n, c = self.sizes[b], self.ctx[b]
             if b in skip:
@@ -92,7 +94,7 @@ class Case:
                 k, _ = self._rows(self.k, self.ks, b, h)
                 v, sv = self._rows(self.v, self.vs, b, h)
                 for i in range(h * g, h * g + g):
-                    attn64.check(got[b, :n, i], *attn64.attend(self.q[b, :n, i], k, v, seen, sv), (b, i))
+                    attn64.check(got[b, :n, i], *attn64.attend(self.q[b, :n, i], k, v, seen, sv, rounded), (b, i))
 
 
 @pytest.mark.parametrize("fmt", list(BITS))

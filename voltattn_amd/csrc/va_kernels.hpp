@@ -235,7 +235,7 @@ struct TreeArgs {
 // Query rows and K/V rows of a work-group's tile where a K/V head has `rows` query rows.
 int tree_rows(int rows);
 int tree_tile(int rows);
-int tree_groups_per_cu(int rows);
+int tree_groups_per_cu(int D, int rows);
 hipError_t launch_tree(int kind, int D, int G, const TreeArgs& a, hipStream_t stream);
 
 // Page pool bookkeeping and row moves (va_pages.hip). Each launch uses the fields that

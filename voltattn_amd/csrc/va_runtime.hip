@@ -846,7 +846,7 @@ int validate_tree(va_fmt fmt, const va_paged_shape* sh, int T, int* nwg) {
     const long long blocks = (long long)sh->B * sh->Hkv * ((rows + bm - 1) / bm);
     const long long tiles = blocks * std::max(1LL, ((long long)sh->max_seq_len + bn - 1) / bn);
     if (tiles > 0x7FFFFFFFLL) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", tiles);
-    *nwg = (int)std::min(tiles, (long long)va::tree_groups_per_cu((int)rows) * cus_or_default());
+    *nwg = (int)std::min(tiles, (long long)(getenv("VA_WG") ? atoi(getenv("VA_WG")) : va::tree_groups_per_cu(sh->D, (int)rows)) * cus_or_default());
     return VA_OK;
 }
 
@@ -902,7 +902,7 @@ int va_decode_tree(va_fmt fmt, const va_tree_bufs* b, const va_paged_shape* sh, 
     a.cap = sh->max_seq_len;
     a.qscale = (float)(1.4426950408889634074 / std::sqrt((double)sh->D));
     a.nwg = nwg;
-    a.min_share = 1;
+    a.min_share = getenv("VA_MS") ? atoi(getenv("VA_MS")) : 1;
     const hipError_t e = va::launch_tree(kind_of(fmt), sh->D, is_f16(fmt) ? 64 : sh->G, a, as_stream(stream));
     if (e != hipSuccess) return hip_fail(e, "tree launch");
     return VA_OK;

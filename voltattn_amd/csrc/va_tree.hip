@@ -8,20 +8,22 @@ static int tree_qw(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 
 int tree_rows(int rows) { return 32 * tree_qw(rows); }
 int tree_tile(int rows) { return tree_qw(rows) == 1 ? TreeTile<1>::BN : TreeTile<2>::BN; }
-int tree_groups_per_cu(int) { return 2; }
+int tree_groups_per_cu(int D, int rows) { return tree_waves(D, tree_qw(rows)); }
 
 template <int KIND, int D, int G>
 static hipError_t launch(const TreeArgs& a, hipStream_t stream) {
     const dim3 grid((unsigned)a.nwg), block(256);
-    const long long rows = (long long)a.B * a.T * a.hkv * a.group;
-    const dim3 mgrid((unsigned)((rows + 3) / 4));
+    const bool few = (long long)a.B * a.T * a.hkv * a.group <= 8192;   // 32 to a work-group would leave CUs idle
+    const int mr = few ? 8 : 32;
+    const dim3 mgrid((unsigned)((size_t)a.B * a.hkv * ((a.T * a.group + mr - 1) / mr)));
     hipError_t e;
 #define VA_TREE(QW)                                                                        \
     do {                                                                                   \
         hipLaunchKernelGGL((tree_attend<KIND, D, G, QW>), grid, block, 0, stream, a);      \
         e = hipGetLastError();                                                             \
         if (e == hipSuccess) {                                                             \
-            hipLaunchKernelGGL((tree_merge<D, QW>), mgrid, block, 0, stream, a);           \
+            if (few) hipLaunchKernelGGL((tree_merge<D, QW, 4>), mgrid, block, 0, stream, a); \
+            else hipLaunchKernelGGL((tree_merge<D, QW, 1>), mgrid, block, 0, stream, a);   \
             e = hipGetLastError();                                                         \
         }                                                                                  \
     } while (0)

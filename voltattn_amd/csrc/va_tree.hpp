@@ -95,6 +95,13 @@ __device__ __forceinline__ void unpack_unit(const Words<Unit<KIND>::W>& u, f16x8
     }
 }
 
+template <int AUX> __device__ __forceinline__ u32x4 load128(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, AUX);
+}
+template <int AUX> __device__ __forceinline__ u32x3 load96(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_amdgcn_raw_buffer_load_b96(r, off, 0, AUX);
+}
+
 // p and p * scale stay within fp16: the weights start at 2^OFF and may grow by 2^SLACK
 // before the maximum follows. A scale of a cache of fp16 values is at most 65504/127 (q8),
 // 65504/7 (q4), 65504/3 (q3).
@@ -104,6 +111,10 @@ template <> struct WeightRange<KQ8>  { static constexpr float off = 3.f, slack =
 template <> struct WeightRange<KQ4>  { static constexpr float off = 0.f, slack = 2.f; };
 template <> struct WeightRange<KQ3>  { static constexpr float off = 0.f, slack = 1.f; };
 
+__device__ __forceinline__ f16x4 lds_scales(const lds_u8* p, uint32_t at) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) f16x4*>(p + at);
+}
+
 // ------------------------------------------------------------- work split --
 // A sequence's part in the numbering: nothing for one without drafts or with lengths
 // out of range (whose rows tree_merge fills).
@@ -111,56 +122,79 @@ struct TreeSeq {
     int ctx, n, len;      // len = ctx + n
     int tiles, blocks;    // K/V tiles, row blocks per K/V head
     bool bad;
+    int first;            // the sequence's first tile in the numbering
 };
-template <int BM, int BN>
-__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
-    TreeSeq s;
-    s.ctx = a.ctx_lens[b];
-    s.n = a.sizes ? a.sizes[b] : a.T;
-    s.bad = s.ctx < 0 || s.n < 0 || s.n > a.T || s.ctx > a.cap - s.n;
-    s.len = s.bad ? 0 : s.ctx + s.n;
-    s.tiles = (s.len + BN - 1) / BN;
-    s.blocks = s.bad ? 0 : (s.n * a.group + BM - 1) / BM;
-    return s;
-}
-template <int BM, int BN>
-__device__ __forceinline__ int tree_units(const TreeArgs& a, int b) {
-    if (b >= a.B) return 0;
-    const TreeSeq s = tree_seq<BM, BN>(a, b);
-    return s.tiles * s.blocks * a.hkv;
-}
-// Sum over the sequences below `upto` (all: a.B); every wave by itself.
-template <int BM, int BN>
-__device__ __forceinline__ int tree_units_below(const TreeArgs& a, int upto) {
-    int sum = 0;
-    for (int b0 = 0; b0 < upto; b0 += 64) {
-        const int b = b0 + (int)__lane_id();
-        sum += __builtin_amdgcn_readlane(wave_scan(b < upto ? tree_units<BM, BN>(a, b) : 0), 63);
+// The numbering, by one wave: lane i has sequence b0 + i of the current 64.
+template <int BM, int BN> struct TreePlan {
+    const TreeArgs& a;
+    int b0 = -1, ctx, n, upto = 0;               // upto: tiles up to and with the lane's sequence
+    int total = 0;                               // of the batch
+    __device__ __forceinline__ void make(TreeSeq& s) const {
+        s.bad = s.ctx < 0 || s.n < 0 || s.n > a.T || s.ctx > a.cap - s.n;
+        s.len = s.bad ? 0 : s.ctx + s.n;
+        s.tiles = (s.len + BN - 1) / BN;
+        s.blocks = s.bad ? 0 : (s.n * a.group + BM - 1) / BM;
     }
-    return sum;
-}
-__device__ __forceinline__ int tree_share(const TreeArgs& a, int units) {
-    return max((units + a.nwg - 1) / a.nwg, a.min_share);
-}
-// Tile `at` of the numbering: its sequence and the number of that sequence's first tile.
-template <int BM, int BN>
-__device__ __forceinline__ bool tree_find(const TreeArgs& a, int at, int& seq, int& first) {
-    int before = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int b = b0 + (int)__lane_id(), u = tree_units<BM, BN>(a, b), upto = before + wave_scan(u);
-        const uint64_t hit = __ballot(upto > at);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            seq = b0 + l;
-            first = __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(u, l);
-            return true;
+    __device__ __forceinline__ void load(int from, int before) {
+        const int b = from + (int)__lane_id();
+        TreeSeq s{};
+        if (b < a.B) {
+            s.ctx = a.ctx_lens[b];
+            s.n = a.sizes ? a.sizes[b] : a.T;
         }
-        before = __builtin_amdgcn_readlane(upto, 63);
+        make(s);
+        b0 = from;
+        ctx = s.ctx;
+        n = s.n;
+        upto = before + wave_scan(b < a.B ? s.tiles * s.blocks * a.hkv : 0);
     }
-    return false;
-}
+    __device__ __forceinline__ explicit TreePlan(const TreeArgs& args) : a(args) {
+        for (int from = 0; from < a.B; from += 64) {
+            load(from, total);
+            total = __builtin_amdgcn_readlane(upto, 63);
+        }
+    }
+    // Brings in the 64 that sequence b is among, or that tile `at` is in (b < 0).
+    __device__ __forceinline__ void seek(int b, int at) {
+        if (a.B <= 64) return;
+        int before = 0;
+        for (int from = 0; from < a.B; from += 64) {
+            load(from, before);
+            before = __builtin_amdgcn_readlane(upto, 63);
+            if (b >= 0 ? b < from + 64 : at < before) return;
+        }
+    }
+    __device__ __forceinline__ TreeSeq lane(int l) const {
+        TreeSeq s;
+        s.ctx = __builtin_amdgcn_readlane(ctx, l);
+        s.n = __builtin_amdgcn_readlane(n, l);
+        make(s);
+        s.first = __builtin_amdgcn_readlane(upto, l) - s.tiles * s.blocks * a.hkv;
+        return s;
+    }
+    __device__ __forceinline__ TreeSeq sequence(int b) {
+        seek(b, 0);
+        return lane(b - b0);
+    }
+    // The sequence that tile at < total is in.
+    __device__ __forceinline__ TreeSeq at(int tile, int& b) {
+        seek(-1, tile);
+        const int l = __builtin_ctzll(__ballot(upto > tile));
+        b = b0 + l;
+        return lane(l);
+    }
+    __device__ __forceinline__ int share() const { return max((total + a.nwg - 1) / a.nwg, a.min_share); }
+};
 
 // --------------------------------------------------------------- kernel --
+#ifndef KVAUX
+#define KVAUX 0
+#endif
+#ifndef PART_AUX
+#define PART_AUX 16
+#endif
+// Work-groups that fit a CU (waves to a SIMD): their registers decide.
+constexpr int tree_waves(int D, int qw) { return qw < 4 ? 2 : D == 128 ? 3 : 4; }
 template <int QW> struct TreeTile {
     static constexpr int BM = 32 * QW, KW = 4 / QW;
     static constexpr int BN = QW == 1 ? 128 : 64;
@@ -168,53 +202,71 @@ template <int QW> struct TreeTile {
 };
 
 template <int KIND, int D, int G, int QW>
-__global__ __launch_bounds__(256, KIND == KF16 && QW == 1 ? 1 : 2) void tree_attend(TreeArgs a) {
+__global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a) {
     using T = TreeTile<QW>;
     constexpr int BM = T::BM, BN = T::BN, KW = T::KW, KB = T::KB;
     constexpr int KS = D / 16, DB = D / 32;
     constexpr int NG = KIND == KF16 ? 1 : D / G;            // scale groups of a row
-    constexpr bool SCALED = KIND != KF16;
+    constexpr bool EXACT2 = KIND != KF16 && QW == 4;        // K as two fp16 terms
+    constexpr bool SCALED = KIND != KF16 && !EXACT2;
     constexpr int ROWB = RowBytes<KIND, D>::value;
     constexpr int UPR = D / Unit<KIND>::UE;                 // units per row
     constexpr int UNITS = BN * UPR;                         // of one tensor's tile
     constexpr int UPT = (UNITS + 255) / 256;                // per lane
     constexpr int TILE = BN * 2 * D;
+    // A tile is fetched while its predecessor is computed, or, by the widest row blocks, when it is
+    // its turn: three work-groups fit a CU without its registers and cover each other's waits
+    constexpr bool AHEAD = QW != 4;
+    constexpr int AUX = QW == 4 ? KVAUX : VA_LOAD_AUX;      // the row blocks of a K/V head read the same rows
+    using WR = WeightRange<SCALED ? KIND : KF16>;
+    constexpr int GP = QW == 1 ? 1 : NG > 2 ? 2 : NG, VP = GP;   // scale groups that are in registers at once
     constexpr int HALVES = BN / 64;                         // a page holds at least 64 rows
     constexpr int RSRCS = 256 / UPR > 64 ? 1 : HALVES;      // halves that a wave fetches from
     constexpr int SCB = SCALED ? NG * BN * 2 : 0;           // bytes of a tile's scales, [group][row]
-    constexpr int COMB = KW > 1 ? 4 * 32 * (D + 4) * 4 : 0; // the KW partial sums, over the tiles
-    constexpr int LDS = 2 * TILE + 2 * SCB > COMB ? 2 * TILE + 2 * SCB : COMB;
+    constexpr int TILES = (EXACT2 ? 3 : 2) * TILE + 2 * SCB;
+    constexpr int ES = 68;                                  // epilogue: 64 columns of a row, the next four banks on
+    constexpr int EPI = 4 * 32 * ES * 4;
+    constexpr int LDS = TILES > EPI + 1024 ? TILES : EPI + 1024;
     __shared__ __align__(1024) uint8_t lds[LDS];
 
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), half = lane >> 5;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    // the thread's number, made anew: what is computed from it is not held across loops
+    auto fresh_tid = [&]() {
+        int x = tid;
+        asm volatile("" : "+v"(x));
+        return x;
+    };
     const int qw = wave % QW, kw = wave / QW;
     lds_u8* kt = (lds_u8*)lds;
     lds_u8* vt = kt + TILE;
-    lds_u8* skt = vt + TILE;
+    lds_u8* skt = vt + TILE;                                // scales, or K's second terms
     lds_u8* svt = skt + SCB;
-    WideAddr<D> ad;
-    ad.init(lane);
+    const float qs = a.qscale * (EXACT2 ? 2.f : 1.f);       // K and V are halved there
+    WideAddr<D> ad0;
+    ad0.init(lane, kw * KB * 32);
 
-    const int units = tree_units_below<BM, BN>(a, a.B);
-    const int share = tree_share(a, units);
     // consecutive shares on one XCD (work-groups are dealt to the eight in turn): the row
     // blocks of a K/V head lie next to each other and read the same rows
     const int wg = (a.nwg & 7) == 0 ? (int)(blockIdx.x & 7) * (a.nwg >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
-    int at = wg * share;
-    const int end = min(units, at + share);
-    while (at < end) {
-        int b, first;
-        if (!tree_find<BM, BN>(a, at, b, first)) return;
-        b = uniform(b);
-        const TreeSeq sq = tree_seq<BM, BN>(a, b);
-        const int in = at - first, blk = in / sq.tiles;     // (K/V head, row block) of the sequence
+    int at = 0, end = 0;
+    do {                                                    // the pieces of the share; each finds its place anew
+        const int lane = fresh_tid() & 63, half = lane >> 5;
+        TreePlan<BM, BN> plan(a);                           // (holding the plan would cost the loop's registers)
+        if (end == 0) {
+            at = wg * plan.share();
+            end = min(plan.total, at + plan.share());
+            if (at >= end) return;
+        }
+        int b;
+        const TreeSeq sq = plan.at(at, b);
+        const int in = at - sq.first, blk = in / sq.tiles;  // (K/V head, row block) of the sequence
         const int hk = uniform(blk / sq.blocks), rb = uniform(blk - hk * sq.blocks);
         const int t0 = uniform(in - blk * sq.tiles), t1 = uniform(min(sq.tiles, t0 + (end - at)));
+        const uint32_t sat = (uint32_t)((kw * KB * 32 + 4 * half) * 2);   // the lane's scales in a group
         const int rows = sq.n * a.group;
         const int row = rb * BM + qw * 32 + (lane & 31);
         const int rc = min(row, rows - 1), node = rc / a.group, hq = hk * a.group + (rc - node * a.group);
-        uint64_t mask = a.mask[(size_t)b * a.T + node];
-        if (sq.n < 64) mask &= (1ull << sq.n) - 1;
+        const uint64_t bits = a.mask[(size_t)b * a.T + node];
         f16x8 q[KS];
         {
             const uint16_t* qp = a.q + (((size_t)b * a.T + node) * a.hkv * a.group + hq) * D + 8 * half;
@@ -225,8 +277,10 @@ __global__ __launch_bounds__(256, KIND == KF16 && QW == 1 ? 1 : 2) void tree_att
 
         Words<Unit<KIND>::W> kr[UPT], vr[UPT];
         uint32_t scr[2] = {0, 0};                           // lane's scales of K (lanes 0..127) or V
+        uint32_t ksu[UPT], vsu[UPT];                        // EXACT2: of its units
         bool bad = false;
         auto fetch = [&](int t) {
+            const int tid = fresh_tid(), lane = tid & 63;
             // the rows of each half of the tile, 64 to a page at least: pool row and how many there are
             size_t first_row[HALVES];
             int left[HALVES];
@@ -241,7 +295,7 @@ __global__ __launch_bounds__(256, KIND == KF16 && QW == 1 ? 1 : 2) void tree_att
                 }
                 first_row[x] = (((size_t)page * a.hkv + hk) << a.page_shift) + (size_t)(j & ((1 << a.page_shift) - 1));
             }
-            __amdgpu_buffer_rsrc_t rk[RSRCS], rv[RSRCS];
+            __amdgpu_buffer_rsrc_t rk[RSRCS], rv[RSRCS], rsk[RSRCS], rsv[RSRCS];
 #pragma unroll
             for (int x = 0; x < RSRCS; ++x) {
                 const bool up = RSRCS < HALVES ? wave >= 2 : x == 1;
@@ -249,6 +303,10 @@ __global__ __launch_bounds__(256, KIND == KF16 && QW == 1 ? 1 : 2) void tree_att
                 const uint32_t bytes = (uint32_t)(uniform(up ? left[HALVES - 1] : left[0]) * ROWB);
                 rk[x] = make_rsrc(a.k + r * ROWB, bytes);
                 rv[x] = make_rsrc(a.v + r * ROWB, bytes);
+                if constexpr (EXACT2) {
+                    rsk[x] = make_rsrc(a.sk + r * NG, bytes / ROWB * NG * 2);
+                    rsv[x] = make_rsrc(a.sv + r * NG, bytes / ROWB * NG * 2);
+                }
             }
 #pragma unroll
             for (int i = 0; i < UPT; ++i) {
@@ -256,13 +314,18 @@ __global__ __launch_bounds__(256, KIND == KF16 && QW == 1 ? 1 : 2) void tree_att
                 const uint32_t off = (uint32_t)((r & 63) * ROWB + (u % UPR) * Unit<KIND>::UB);
                 if (UNITS % 256 == 0 || u < UNITS) {
                     if constexpr (Unit<KIND>::W == 4) {
-                        const u32x4 ka = ld128(rk[x], off, 0), va = ld128(rv[x], off, 0);
+                        const u32x4 ka = load128<AUX>(rk[x], off), va = load128<AUX>(rv[x], off);
                         kr[i] = {{ka.x, ka.y, ka.z, ka.w}};
                         vr[i] = {{va.x, va.y, va.z, va.w}};
                     } else {
-                        const u32x3 ka = ld96(rk[x], off, 0), va = ld96(rv[x], off, 0);
+                        const u32x3 ka = load96<AUX>(rk[x], off), va = load96<AUX>(rv[x], off);
                         kr[i] = {{ka.x, ka.y, ka.z}};
                         vr[i] = {{va.x, va.y, va.z}};
+                    }
+                    if constexpr (EXACT2) {
+                        const uint32_t so = (uint32_t)(((r & 63) * NG + (u % UPR) * Unit<KIND>::UE / G) * 2);
+                        ksu[i] = ld16(rsk[x], so, 0);
+                        vsu[i] = ld16(rsv[x], so, 0);
                     }
                 }
             }
@@ -280,19 +343,33 @@ __global__ __launch_bounds__(256, KIND == KF16 && QW == 1 ? 1 : 2) void tree_att
             }
         };
         auto stage = [&]() {
+            const int tid = fresh_tid();
 #pragma unroll
             for (int i = 0; i < UPT; ++i) {
                 const int u = i * 256 + tid, r = u / UPR, c = (u % UPR) * (Unit<KIND>::UE / 8);
                 if (UNITS % 256 == 0 || u < UNITS) {
-                    f16x8 x[Unit<KIND>::UE / 8], y[Unit<KIND>::UE / 8];
+                    f16x8 x[Unit<KIND>::UE / 8];
                     unpack_unit<KIND>(kr[i], x);
-                    unpack_unit<KIND>(vr[i], y);
+                    const f16x8 ks = EXACT2 ? f16x8(__builtin_bit_cast(_Float16, (uint16_t)ksu[i])) * (_Float16)0.5f : f16x8{};
 #pragma unroll
                     for (int e = 0; e < Unit<KIND>::UE / 8; ++e) {
                         const int to = r * 2 * D + (((c + e) ^ swz<D>(r)) << 4);
+                        if constexpr (EXACT2) {
+                            const f16x8 hi = x[e] * ks;
+                            *reinterpret_cast<lds_f16x8*>(skt + to) = __builtin_elementwise_fma(x[e], ks, -hi);
+                            x[e] = hi;
+                        }
                         *reinterpret_cast<lds_f16x8*>(kt + to) = x[e];
-                        *reinterpret_cast<lds_f16x8*>(vt + to) = y[e];
                     }
+                    if (!AHEAD) __builtin_amdgcn_sched_barrier(0);   // one operand's values in registers at a time
+                    unpack_unit<KIND>(vr[i], x);
+                    const f16x8 vs = EXACT2 ? f16x8(__builtin_bit_cast(_Float16, (uint16_t)vsu[i])) * (_Float16)0.5f : f16x8{};
+#pragma unroll
+                    for (int e = 0; e < Unit<KIND>::UE / 8; ++e) {
+                        const int to = r * 2 * D + (((c + e) ^ swz<D>(r)) << 4);
+                        *reinterpret_cast<lds_f16x8*>(vt + to) = EXACT2 ? x[e] * vs : x[e];
+                    }
+                    if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if constexpr (SCALED) {
@@ -307,36 +384,80 @@ __global__ __launch_bounds__(256, KIND == KF16 && QW == 1 ? 1 : 2) void tree_att
             }
         };
 
+        // keeps the operands' loads ahead of the arithmetic that covers their latency; with few
+        // query rows the fetches bound, and the registers are theirs
+        auto order = []() {
+            if constexpr (QW == 2) __builtin_amdgcn_sched_barrier(0);
+        };
         f32x16 o[DB] = {};
         float m = -__builtin_inff(), l = 0.f;               // m: raw scores; p = exp2((s - m) qscale + OFF)
-        fetch(t0);
+        if constexpr (AHEAD) fetch(t0);
+        const uint64_t mask = sq.n < 64 ? bits & ((1ull << sq.n) - 1) : bits;
         for (int t = t0; t < t1; ++t) {
-            __syncthreads();                                // the last tile (or sum) is read
+            __syncthreads();                                // the last tile, or sums, are read
+            if constexpr (!AHEAD) fetch(t);
             stage();
-            if (t + 1 < t1) fetch(t + 1);
+            if (AHEAD && t + 1 < t1) fetch(t + 1);
             __syncthreads();
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                const int r32 = (kw * KB + kb) * 32;        // the block's first row in the tile
-                const int j = t * BN + r32;
+                const int j = t * BN + (kw * KB + kb) * 32;
+                const WideAddr<D> ad = ad0.fresh();
+                const uint32_t at32 = (uint32_t)(kb * 64 * D);   // the block's rows, in bytes
                 f32x16 s = {};
+                f16x8 kf[KS];
+                if constexpr (QW != 4) {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) kf[i] = lds_row8(kt, ad.k(i) + at32);
+                }
+                order();
                 if constexpr (SCALED) {
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        f32x16 acc = {};
+                    for (int g0 = 0; g0 < NG; g0 += GP) {
+                        f32x16 acc[GP] = {};
 #pragma unroll
-                        for (int i = g * G / 16; i < (g + 1) * G / 16; ++i)
-                            acc = mfma_32x32x16(lds_row8(kt + r32 * 2 * D, ad.k[i]), q[i], acc);
+                        for (int i = 0; i < G / 16; ++i)
 #pragma unroll
-                        for (int v4 = 0; v4 < 4; ++v4) {
-                            const f16x4 sc = *reinterpret_cast<__attribute__((address_space(3))) f16x4*>(skt + (g * BN + r32 + 8 * v4 + 4 * half) * 2);
+                            for (int g = 0; g < GP; ++g) acc[g] = mfma_32x32x16(kf[(g0 + g) * G / 16 + i], q[(g0 + g) * G / 16 + i], acc[g]);
+                        order();
+                        f16x4 sc[GP][4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) s[4 * v4 + e] = __builtin_fmaf(acc[4 * v4 + e], (float)sc[e], s[4 * v4 + e]);
-                        }
+                        for (int g = 0; g < GP; ++g)
+#pragma unroll
+                            for (int v4 = 0; v4 < 4; ++v4) sc[g][v4] = lds_scales(skt, sat + (uint32_t)(((g0 + g) * BN + kb * 32 + 8 * v4) * 2));
+#pragma unroll
+                        for (int g = 0; g < GP; ++g)
+#pragma unroll
+                            for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(acc[g][v], (float)sc[g][v / 4][v % 4], s[v]);
                     }
                 } else {
-                    s = wide_scores<D>(kt + r32 * 2 * D, ad, q);
+                    if constexpr (EXACT2) {
+#pragma unroll
+                        for (int i = 0; i < KS; ++i) s = mfma_32x32x16(lds_row8(skt, ad.k(i) + at32), q[i], s);
+                    }
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) s = mfma_32x32x16(QW == 4 ? lds_row8(kt, ad.k(i) + at32) : kf[i], q[i], s);
                 }
+                // V's operands are on their way while the weights are made
+                order();
+                f16x8 vf[2][DB];
+                if constexpr (QW != 4) {
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                        for (int db = 0; db < DB; ++db) {
+                            const uint32_t to = at32 + (uint32_t)(tt * 32 * D);
+                            vf[tt][db] = lds_tr8(vt, ad.v(db, 0) + to, ad.v(db, 1) + to);
+                        }
+                }
+                f16x4 vsc[NG][4];
+                if constexpr (SCALED) {
+#pragma unroll
+                    for (int g = 0; g < VP; ++g)
+#pragma unroll
+                        for (int v4 = 0; v4 < 4; ++v4) vsc[g][v4] = lds_scales(svt, sat + (uint32_t)((g * BN + kb * 32 + 8 * v4) * 2));
+                }
+                order();
                 if (j + 32 > sq.ctx) {                      // drafts, or rows behind the sequence
                     const int d = sq.ctx - j;               // below 32: where the drafts begin
                     uint32_t seen = d > 0 ? ((1u << d) - 1u) | (uint32_t)(mask << d) : d > -64 ? (uint32_t)(mask >> -d) : 0u;
@@ -348,161 +469,218 @@ __global__ __launch_bounds__(256, KIND == KF16 && QW == 1 ? 1 : 2) void tree_att
 #pragma unroll
                 for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
                 top = halves_max(top);
-                if (__any((top - m) * a.qscale > WeightRange<KIND>::slack)) {   // also the first one: m = -inf
+                if (__any((top - m) * qs > WR::slack)) {   // also the first one: m = -inf
                     const float to = fmaxf(m, top);
-                    const float f = to == m ? 1.f : fast_exp2((m - to) * a.qscale);
+                    const float f = to == m ? 1.f : fast_exp2((m - to) * qs);
                     m = to;
                     l *= f;
 #pragma unroll
                     for (int db = 0; db < DB; ++db) o[db] *= f;
                 }
-                const float base = m == -__builtin_inff() ? 0.f : m * a.qscale - WeightRange<KIND>::off;
+                const float base = m == -__builtin_inff() ? 0.f : m * qs - WR::off;
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    s[v] = fast_exp2(__builtin_fmaf(s[v], a.qscale, -base));
+                    s[v] = fast_exp2(__builtin_fmaf(s[v], qs, -base));
                     l += s[v];
                 }
-                lds_u8* vb = vt + r32 * 2 * D;
-                if constexpr (SCALED) {
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        f16x8 p[2];
-#pragma unroll
-                        for (int v4 = 0; v4 < 4; ++v4) {
-                            const f16x4 sc = *reinterpret_cast<__attribute__((address_space(3))) f16x4*>(svt + (g * BN + r32 + 8 * v4 + 4 * half) * 2);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) p[v4 / 2][4 * (v4 & 1) + e] = (_Float16)(s[4 * v4 + e] * (float)sc[e]);
-                        }
-#pragma unroll
-                        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                            for (int db = g * G / 32; db < (g + 1) * G / 32; ++db) {
-                                const uint32_t to = (uint32_t)(tt * 16 * 2 * D);
-                                o[db] = mfma_32x32x16(lds_tr8(vb, ad.v[db][0] + to, ad.v[db][1] + to), p[tt], o[db]);
-                            }
-                    }
-                } else {
-                    f16x8 p[2];
+                f16x8 p[2];
+                if constexpr (!SCALED) {
 #pragma unroll
                     for (int v = 0; v < 16; ++v) p[v / 8][v % 8] = (_Float16)s[v];
-                    wide_values<D>(vb, ad, p, o);
+                }
+                if constexpr (QW == 4) {
+                    wide_values<D>(vt + at32, ad, p, o);
+                    continue;
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    if constexpr (SCALED) {
+                        if (g + VP < NG)
+#pragma unroll
+                            for (int v4 = 0; v4 < 4; ++v4) vsc[g + VP][v4] = lds_scales(svt, sat + (uint32_t)(((g + VP) * BN + kb * 32 + 8 * v4) * 2));
+#pragma unroll
+                        for (int v = 0; v < 16; ++v)    // + 0: one instruction, the product rounded to fp16 once
+                            p[v / 8][v % 8] = (_Float16)__builtin_fmaf(s[v], (float)vsc[g][v / 4][v % 4], 0.f);
+                    }
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                        for (int db = g * DB / NG; db < (g + 1) * DB / NG; ++db) o[db] = mfma_32x32x16(vf[tt][db], p[tt], o[db]);
                 }
             }
         }
         l = halves_sum(l);
         if (bad) l = __builtin_nanf("");
 
+        // The sums, 64 columns at a time, go through LDS: the KW waves of the same rows are joined
+        // there, and a row leaves in one piece (a row per lane leaves 32 bytes at a time: one
+        // sequence, 16 drafts over 4096 positions q8, 26.4 us with it).
         const bool whole = t0 == 0 && t1 == sq.tiles;
         const int slot = 2 * wg + (t0 == 0 ? 1 : 0);
-        float* part = a.ws + (size_t)slot * BM * (D + 2);   // [BM][D] sums, then [BM][2] (m, l)
-        const int r = qw * 32 + (lane & 31);
-        uint16_t* out = a.out + (((size_t)b * a.T + node) * a.hkv * a.group + hq) * D;
-        auto finish = [&](float mm, float ll, int d, float x0, float x1, float x2, float x3) {
-            if (row >= rows) return;
-            if (whole) {
-                const float inv = ll == 0.f ? 0.f : 1.f / ll;
-                const bool none = ll == 0.f;
-                f16x4 w = {(_Float16)(none ? 0.f : x0 * inv), (_Float16)(none ? 0.f : x1 * inv),
-                           (_Float16)(none ? 0.f : x2 * inv), (_Float16)(none ? 0.f : x3 * inv)};
-                *reinterpret_cast<f16x4*>(out + d) = w;
-            } else {
-                *reinterpret_cast<f32x4*>(part + (size_t)r * D + d) = f32x4{x0, x1, x2, x3};
-                if (d == 0) *reinterpret_cast<u32x2*>(part + (size_t)BM * D + 2 * r) =
-                    u32x2{__builtin_bit_cast(uint32_t, mm * a.qscale), __builtin_bit_cast(uint32_t, ll)};
-            }
-        };
-        if constexpr (KW == 1) {
+        // [BM][D] sums, then [BM][2] (m, l); written through to memory: what is dirty in the L2s is
+        // written back when the kernel ends, at a fraction of the rate
+        const __amdgpu_buffer_rsrc_t part = make_rsrc(a.ws + (size_t)uniform(slot) * BM * (D + 2), BM * (D + 2) * 4);
+        __attribute__((address_space(3))) float* es = (__attribute__((address_space(3))) float*)lds;
+        __attribute__((address_space(3))) float* ml = es + EPI / 4;     // [wave][32][2]
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    finish(m, l, 32 * db + 8 * g + 4 * half, o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]);
-        } else {
-            // the KW waves of these rows: sums side by side in LDS, then each wave joins a part of the columns
+        for (int c0 = 0; c0 < D; c0 += 64) {
+            const int tid = fresh_tid(), lane = tid & 63, half = lane >> 5;
             __syncthreads();
-            __attribute__((address_space(3))) float* cs = (__attribute__((address_space(3))) float*)lds;
-            constexpr int RS = D + 4;                       // row stride: rows four banks apart
-            __attribute__((address_space(3))) float* mine = cs + (wave * 32 + (lane & 31)) * RS;
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
+            for (int db = 0; db < 2; ++db)
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(mine + 32 * db + 8 * g + 4 * half) =
-                        f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-            if (half == 0) {
-                mine[D] = m;
-                mine[D + 1] = l;
-            }
-            __syncthreads();
-            float mm = -__builtin_inff();
-#pragma unroll
-            for (int k = 0; k < KW; ++k) mm = fmaxf(mm, cs[((k * QW + qw) * 32 + (lane & 31)) * RS + D]);
-            float ll = 0.f, f[KW];
-#pragma unroll
-            for (int k = 0; k < KW; ++k) {
-                const __attribute__((address_space(3))) float* x = cs + ((k * QW + qw) * 32 + (lane & 31)) * RS;
-                f[k] = x[D] == mm ? 1.f : fast_exp2((x[D] - mm) * a.qscale);
-                ll = __builtin_fmaf(f[k], x[D + 1], ll);
-            }
-            // (K/V-row wave kw, half) of 2 KW: columns 4 (kw 2 + half) + 8 KW i
-#pragma unroll
-            for (int i = 0; i < D / (8 * KW); ++i) {
-                const int d = 4 * (kw * 2 + half) + 8 * KW * i;
-                f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < KW; ++k) {
-                    const f32x4 x = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(cs + ((k * QW + qw) * 32 + (lane & 31)) * RS + d);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(f[k], x[e], s[e]);
+                for (int g = 0; g < 4; ++g) {
+                    const f32x16& x = o[c0 / 32 + db];
+                    *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(es + (wave * 32 + (lane & 31)) * ES + 32 * db + 8 * g + 4 * half) =
+                        f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
                 }
-                finish(mm, ll, d, s[0], s[1], s[2], s[3]);
+            if (c0 == 0 && half == 0) {
+                ml[(wave * 32 + lane) * 2] = m;
+                ml[(wave * 32 + lane) * 2 + 1] = l;
+            }
+            __syncthreads();
+            const int c = (tid & 15) * 4;
+#pragma unroll 1
+            for (int r0 = 0; r0 < BM; r0 += 16) {
+                const int r = r0 + (tid >> 4), at0 = r & 31, w0 = r >> 5;
+                float mm = ml[(w0 * 32 + at0) * 2], ll = ml[(w0 * 32 + at0) * 2 + 1];
+                f32x4 x = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(es + (w0 * 32 + at0) * ES + c);
+                if constexpr (KW > 1) {
+                    const float m0 = mm;
+#pragma unroll
+                    for (int k = 1; k < KW; ++k) mm = fmaxf(mm, ml[((k * QW + w0) * 32 + at0) * 2]);
+                    const float f0 = m0 == mm ? 1.f : fast_exp2((m0 - mm) * qs);
+                    ll *= f0;
+                    x *= f0;
+#pragma unroll
+                    for (int k = 1; k < KW; ++k) {
+                        const int w = (k * QW + w0) * 32 + at0;
+                        const float mk = ml[w * 2], f = mk == mm ? 1.f : fast_exp2((mk - mm) * qs);
+                        const f32x4 y = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(es + w * ES + c);
+                        ll = __builtin_fmaf(f, ml[w * 2 + 1], ll);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(f, y[e], x[e]);
+                    }
+                }
+                const int to = rb * BM + r;
+                if (to >= rows) continue;
+                if (EXACT2) x *= 2.f;
+                if (whole) {
+                    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+                    f16x4 y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = (_Float16)(ll == 0.f ? 0.f : x[e] * inv);
+                    const int nd = to / a.group;
+                    *reinterpret_cast<f16x4*>(a.out + (((size_t)b * a.T + nd) * a.hkv * a.group + hk * a.group + (to - nd * a.group)) * D + c0 + c) = y;
+                } else {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), part, (uint32_t)(r * D + c0 + c) * 4, 0, PART_AUX);
+                    if (c0 == 0 && c == 0)
+                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, (f32x2{mm * qs, ll})), part, (uint32_t)(BM * D + 2 * r) * 4, 0, PART_AUX);
+                }
             }
         }
         at += t1 - t0;
-    }
+    } while (at < end);
 }
 
 // Joins the pieces of the row blocks that several shares cut, and fills the rows that no
 // work-group has: zeros for drafts behind a sequence's last one and for sequences of
-// length 0, NaN for sequences whose lengths are out of range. A wave per output row.
-template <int D, int QW>
+// length 0, NaN for sequences whose lengths are out of range. A work-group has 32/PW rows of
+// one (sequence, K/V head), eight lanes to a row with D/8 columns each; PW of its waves
+// share the pieces of the same rows (few rows, many pieces), joined through LDS.
+template <int D, int QW, int PW>
 __global__ __launch_bounds__(256) void tree_merge(TreeArgs a) {
-    constexpr int BM = TreeTile<QW>::BM, BN = TreeTile<QW>::BN, E = D / 64;
-    const int lane = (int)__lane_id();
-    const int hq = a.hkv * a.group;
-    const long long n = (long long)a.B * a.T * hq;
-    const long long i = (long long)blockIdx.x * 4 + uniform((int)threadIdx.x >> 6);
-    if (i >= n) return;
-    const int b = (int)(i / (a.T * hq)), in = (int)(i - (long long)b * a.T * hq), node = in / hq, h = in - node * hq;
-    uint16_t* out = a.out + (size_t)i * D + lane * E;
-    const TreeSeq sq = tree_seq<BM, BN>(a, b);
-    float x[E] = {};
-    if (sq.bad) {
+    constexpr int BM = TreeTile<QW>::BM, BN = TreeTile<QW>::BN, V = D / 32, MR = 32 / PW;
+    constexpr int U = 4;                                    // pieces in flight
+    __shared__ float s_part[PW > 1 ? 4 * 8 * D : 1], s_ml[PW > 1 ? 4 * 8 * 2 : 1];
+    const int lane = (int)__lane_id(), wave = uniform((int)threadIdx.x >> 6);
+    const int all = a.T * a.group, per = (all + MR - 1) / MR;   // rows of a K/V head, work-groups
+    const int bh = (int)blockIdx.x / per, b = bh / a.hkv, hk = bh - b * a.hkv;
+    const int base = ((int)blockIdx.x - bh * per) * MR;     // MR rows never leave a row block
+    const int row = base + (PW > 1 ? 0 : wave * 8) + (lane >> 3), r = row % BM, pw = PW > 1 ? wave : 0;
+    TreePlan<BM, BN> plan(a);
+    const TreeSeq sq = plan.sequence(b);
+    const int rows = sq.bad ? 0 : sq.n * a.group;
+    const int share = plan.share(), t0 = sq.first + (hk * sq.blocks + base / BM) * sq.tiles;
+    const int w0 = t0 / share, w1 = (t0 + sq.tiles - 1) / share;
+    if (base + MR <= rows && w0 == w1) return;              // finished by their work-group
+    constexpr size_t STEP = (size_t)BM * (D + 2);
+    const float* col = a.ws + (size_t)r * D + (lane & 7) * 4;
+    const float* ml = a.ws + (size_t)BM * D + 2 * r;
+    float m = -__builtin_inff(), l = 0.f;
+    f32x4 x[V] = {};
+    if (w0 != w1 && base < rows) {
+        for (int p0 = w0 + pw; p0 <= w1; p0 += U * PW) {
+            f32x2 s[U];
+            f32x4 y[U][V];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = __builtin_nanf("");
-    } else if (node < sq.n) {
-        const int hk = h / a.group, r = node * a.group + (h - hk * a.group);
-        const int share = tree_share(a, tree_units_below<BM, BN>(a, a.B));
-        const int t0 = tree_units_below<BM, BN>(a, b) + (hk * sq.blocks + r / BM) * sq.tiles;
-        const int w0 = t0 / share, w1 = (t0 + sq.tiles - 1) / share;
-        if (w0 == w1) return;                               // finished by its work-group
-        float m = -__builtin_inff(), l = 0.f;
-        for (int w = w0; w <= w1; ++w) {
-            const float* part = a.ws + (size_t)(2 * w + (w == w0 ? 1 : 0)) * BM * (D + 2);
-            const float mw = part[(size_t)BM * D + 2 * (r % BM)], lw = part[(size_t)BM * D + 2 * (r % BM) + 1];
-            const float to = fmaxf(m, mw);
-            const float f = m == to ? 1.f : fast_exp2(m - to), g = mw == to ? 1.f : fast_exp2(mw - to);
+            for (int u = 0; u < U; ++u) {
+                const int p = min(p0 + u * PW, w1);         // the last one again: not used
+                const size_t at = (size_t)(2 * p + (p == w0 ? 1 : 0)) * STEP;
+                s[u] = *reinterpret_cast<const f32x2*>(ml + at);
+#pragma unroll
+                for (int v = 0; v < V; ++v) y[u][v] = *reinterpret_cast<const f32x4*>(col + at + 32 * v);
+            }
+            float to = m;
+#pragma unroll
+            for (int u = 0; u < U; ++u) to = fmaxf(to, s[u].x);
+            const float f = m == to ? 1.f : fast_exp2(m - to);
             m = to;
-            l = __builtin_fmaf(g, lw, l * f);
+            l *= f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = __builtin_fmaf(g, part[(size_t)(r % BM) * D + lane * E + e], x[e] * f);
+            for (int v = 0; v < V; ++v) x[v] *= f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p0 + u * PW > w1) continue;
+                const float g = s[u].x == to ? 1.f : fast_exp2(s[u].x - to);
+                l = __builtin_fmaf(g, s[u].y, l);
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[v][e] = __builtin_fmaf(g, y[u][v][e], x[v][e]);
+            }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = l == 0.f ? 0.f : x[e] * inv;
     }
+    if constexpr (PW > 1) {
+        float* mine = s_part + (wave * 8 + (lane >> 3)) * D + (lane & 7) * 4;
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = f2h_rne(x[e]);
+        for (int v = 0; v < V; ++v) *reinterpret_cast<f32x4*>(mine + 32 * v) = x[v];
+        if ((lane & 7) == 0) {
+            s_ml[(wave * 8 + (lane >> 3)) * 2] = m;
+            s_ml[(wave * 8 + (lane >> 3)) * 2 + 1] = l;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        float to = m;
+#pragma unroll
+        for (int w = 1; w < PW; ++w) to = fmaxf(to, s_ml[(w * 8 + (lane >> 3)) * 2]);
+        const float f = m == to ? 1.f : fast_exp2(m - to);
+        l *= f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] *= f;
+#pragma unroll
+        for (int w = 1; w < PW; ++w) {
+            const float mw = s_ml[(w * 8 + (lane >> 3)) * 2], g = mw == to ? 1.f : fast_exp2(mw - to);
+            l = __builtin_fmaf(g, s_ml[(w * 8 + (lane >> 3)) * 2 + 1], l);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const f32x4 y = *reinterpret_cast<const f32x4*>(mine + w * 8 * D + 32 * v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[v][e] = __builtin_fmaf(g, y[e], x[v][e]);
+            }
+        }
+    }
+    if (row >= all || (row < rows && w0 == w1)) return;
+    const int node = row / a.group;
+    uint16_t* out = a.out + (((size_t)b * a.T + node) * a.hkv * a.group + hk * a.group + (row - node * a.group)) * D + (lane & 7) * 4;
+    const float inv = l == 0.f ? 0.f : 1.f / l, none = sq.bad ? __builtin_nanf("") : 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        f16x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (_Float16)(row >= rows ? none : l == 0.f ? 0.f : x[v][e] * inv);
+        *reinterpret_cast<f16x4*>(out + 32 * v) = y;
+    }
 }
 
 } // namespace va

@@ -28,6 +28,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short    s16x4 __attribute__((ext_vector_type(4)));
+typedef float    f32x2 __attribute__((ext_vector_type(2)));
 typedef float    f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -57,25 +58,29 @@ __device__ __forceinline__ float halves_sum(float x) {
 }
 
 // LDS addresses of a wave's operands in a K tile and a V tile (byte offsets from
-// the tile's start). Rows 32 apart differ by 64D bytes in the address only.
+// the tile's start). Rows 32 apart differ by 64D bytes in the address only, and the
+// chunks of one row by an XOR, so that three registers are enough; fresh() keeps the
+// compiler from holding all their XORs across a loop.
 template <int D> struct WideAddr {
-    uint32_t k[D / 16];      // K chunk of step s of this lane's row
-    uint32_t v[D / 32][2];   // V^T block db, rows 8r + ..
-    __device__ __forceinline__ void init(int lane) {
+    uint32_t k0, v0[2];
+    // row0: the tile's row that the wave's blocks begin at, a multiple of 32
+    __device__ __forceinline__ void init(int lane, int row0 = 0) {
         const int h = lane >> 5, row = lane & 31;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) k[s] = (uint32_t)(row * 2 * D + (((2 * s + h) ^ swz<D>(row)) << 4));
+        k0 = (uint32_t)((row0 + row) * 2 * D + ((h ^ swz<D>(row)) << 4));
         const int i = lane & 15;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int key = 8 * r + 4 * h + (i >> 2);
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db) {
-                const int chunk = db * 4 + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-                v[db][r] = (uint32_t)(key * 2 * D + ((chunk ^ swz<D>(key)) << 4) + (i & 1) * 8);
-            }
+            const int key = 8 * r + 4 * h + (i >> 2), chunk = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+            v0[r] = (uint32_t)((row0 + key) * 2 * D + ((chunk ^ swz<D>(key)) << 4) + (i & 1) * 8);
         }
     }
+    __device__ __forceinline__ WideAddr fresh() const {
+        WideAddr a = *this;
+        asm volatile("" : "+v"(a.k0), "+v"(a.v0[0]), "+v"(a.v0[1]));
+        return a;
+    }
+    __device__ __forceinline__ uint32_t k(int s) const { return k0 ^ (uint32_t)(s << 5); }          // chunk of step s of this lane's row
+    __device__ __forceinline__ uint32_t v(int db, int r) const { return v0[r] ^ (uint32_t)(db << 6); }   // V^T block db, rows 8r + ..
 };
 
 __device__ __forceinline__ f16x8 lds_row8(const lds_u8* p, uint32_t at) {
@@ -92,7 +97,7 @@ template <int D>
 __device__ __forceinline__ f32x16 wide_scores(const lds_u8* k, const WideAddr<D>& ad, const f16x8 (&q)[D / 16]) {
     f32x16 s = {};
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) s = mfma_32x32x16(lds_row8(k, ad.k[i]), q[i], s);
+    for (int i = 0; i < D / 16; ++i) s = mfma_32x32x16(lds_row8(k, ad.k(i)), q[i], s);
     return s;
 }
 
@@ -104,7 +109,7 @@ __device__ __forceinline__ void wide_values(lds_u8* v, const WideAddr<D>& ad, co
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) {
             const uint32_t at = (uint32_t)(t * 16 * 2 * D);
-            o[db] = mfma_32x32x16(lds_tr8(v, ad.v[db][0] + at, ad.v[db][1] + at), p[t], o[db]);
+            o[db] = mfma_32x32x16(lds_tr8(v, ad.v(db, 0) + at, ad.v(db, 1) + at), p[t], o[db]);
         }
 }
 
