@@ -106,7 +106,7 @@ template <int AUX> __device__ __forceinline__ u32x3 load96(__amdgpu_buffer_rsrc_
 // before the maximum follows. A scale of a cache of fp16 values is at most 65504/127 (q8),
 // 65504/7 (q4), 65504/3 (q3).
 template <int KIND> struct WeightRange;
-template <> struct WeightRange<KF16> { static constexpr float off = 4.f, slack = 8.f; };
+template <> struct WeightRange<KF16> { static constexpr float off = WIDE_OFF, slack = WIDE_SLACK; };
 template <> struct WeightRange<KQ8>  { static constexpr float off = 3.f, slack = 3.f; };
 template <> struct WeightRange<KQ4>  { static constexpr float off = 0.f, slack = 2.f; };
 template <> struct WeightRange<KQ3>  { static constexpr float off = 0.f, slack = 1.f; };

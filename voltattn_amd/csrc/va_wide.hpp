@@ -45,6 +45,11 @@ template <int D> __device__ __forceinline__ int swz(int row) {
     return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 2) << 1) | ((row >> 2) & 3);
 }
 
+// The running maximum that weights are relative to follows lazily: weights start at
+// 2^WIDE_OFF (fp16 keeps their digits down to 2^-14, and some to 2^-24) and may grow by
+// 2^WIDE_SLACK before sums and output are rescaled, which a wave then rarely does.
+constexpr float WIDE_OFF = 4.f, WIDE_SLACK = 8.f;
+
 // x combined over the two half-waves (lanes l and l^32).
 __device__ __forceinline__ float halves_max(float x) {
     unsigned a = __builtin_bit_cast(unsigned, x), b = a;
@@ -90,6 +95,18 @@ __device__ __forceinline__ f16x8 lds_tr8(lds_u8* p, uint32_t a, uint32_t b) {
     const f16x4 x = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(p + a)));
     const f16x4 y = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(p + b)));
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Order for the scheduler of N matrix products with R LDS reads each, in the scheduling
+// region that this call ends: the reads of the next DEEP products are always on their way.
+template <int N, int R, int DEEP> __device__ __forceinline__ void feed_mfma() {
+    __builtin_amdgcn_sched_group_barrier(0x100, DEEP * R, 0);
+#pragma unroll
+    for (int i = 0; i < N - DEEP; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, DEEP, 0);
 }
 
 // S^T of one 32-row K block at `k` (its first row's LDS address).
