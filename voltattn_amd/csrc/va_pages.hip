@@ -13,6 +13,7 @@ namespace va {
 
 constexpr int PLAN_T = 1024;          // threads of the planning work-group
 constexpr int PLAN_IDS = 8;           // page counts that one of its threads looks at at once
+constexpr int PLAN_ONE = 128;         // sequences (parents and children) that it plans by itself
 
 __device__ __forceinline__ int pages_of(int n, int page_rows) { return n <= 0 ? 0 : (n - 1) / page_rows + 1; }
 __device__ __forceinline__ bool in_pool(const PageArgs& a, int id) { return id >= 0 && id < a.num_pages; }
@@ -45,136 +46,165 @@ __device__ __forceinline__ int count_parents(const int32_t* parents, int n, int 
     return kids;
 }
 
-// A child's block-table row and length, by one wave. The entry of a page that it needs of
-// its own (a later child's copy of the partly filled last page) is -2.
-__device__ __forceinline__ void fork_child(const PageArgs& a, int c) {
-    const int p = a.parents[c], lane = (int)__lane_id();
+// A child's block-table row and length, by one wave; true, and the entry, if it needs a page
+// of its own there (a later child's copy of the partly filled last page): the entry is -2.
+__device__ __forceinline__ bool fork_child(const PageArgs& a, const int32_t* parents, const int32_t* lens, int c, int& full) {
+    const int p = parents[c], lane = (int)__lane_id();
     const bool has = p >= 0 && p < a.B;
     const int cap = a.max_pages * a.page_rows;
-    const int len = has ? max(0, min(a.lens[p], cap)) : 0;
-    const int own = pages_of(len, a.page_rows), full = len / a.page_rows;
-    const bool later = has && count_parents(a.parents, c, p) > 0;
+    const int len = has ? max(0, min(lens[p], cap)) : 0, own = pages_of(len, a.page_rows);
+    full = len / a.page_rows;
+    const bool later = has && count_parents(parents, c, p) > 0;
     const int32_t* from = a.table + (size_t)(has ? p : 0) * a.max_pages;
     int32_t* to = a.new_table + (size_t)c * a.max_pages;
+    bool asks = false;
     for (int i = lane; i < a.max_pages; i += 64) {
         int id = i < own ? from[i] : -1;
-        if (later && i == full && in_pool(a, id)) id = -2;          // i < own here: the page in part
+        if (later && i == full && in_pool(a, id)) {         // i < own here: the page in part
+            id = -2;
+            asks = true;
+        }
         to[i] = id;
     }
     if (lane == 0) a.new_lens[c] = len;
+    return __any(asks);
 }
 // The counts of a parent's pages: every child more holds the full ones, the first child
 // keeps the last one, and without children all are given up.
-__device__ __forceinline__ void fork_parent(const PageArgs& a, int p) {
+template <int SCOPE>
+__device__ __forceinline__ void fork_parent(const PageArgs& a, const int32_t* parents, const int32_t* lens, int p) {
     const int cap = a.max_pages * a.page_rows;
-    const int len = max(0, min(a.lens[p], cap));
+    const int len = max(0, min(lens[p], cap));
     const int own = pages_of(len, a.page_rows), full = len / a.page_rows;
-    const int kids = count_parents(a.parents, a.children, p);
+    const int kids = count_parents(parents, a.children, p);
     const int32_t* from = a.table + (size_t)p * a.max_pages;
     for (int i = (int)__lane_id(); i < own; i += 64) {
         const int id = from[i], more = (i < full ? kids : min(kids, 1)) - 1;
-        if (more != 0 && in_pool(a, id)) atomicAdd(a.refs + id, more);
+        if (more != 0 && in_pool(a, id)) __hip_atomic_fetch_add(a.refs + id, more, __ATOMIC_RELAXED, SCOPE);
     }
 }
-// Sequence b's entries given up and asked for, by one wave.
-__device__ __forceinline__ void resize_row(const PageArgs& a, int b) {
+// Sequence b's entries given up and asked for, by one wave; how many are asked for.
+template <int SCOPE>
+__device__ __forceinline__ int resize_row(const PageArgs& a, int b, int before, int after, int& first) {
     const int cap = a.max_pages * a.page_rows;
-    const int n0 = pages_of(min(a.lens[b], cap), a.page_rows), n1 = pages_of(min(a.after[b], cap), a.page_rows);
+    const int n0 = pages_of(min(before, cap), a.page_rows), n1 = pages_of(min(after, cap), a.page_rows);
     int32_t* row = a.new_table + (size_t)b * a.max_pages;
     for (int i = min(n0, n1) + (int)__lane_id(); i < max(n0, n1); i += 64) {
         if (i < n0) {
             const int id = row[i];
-            if (in_pool(a, id)) atomicAdd(a.refs + id, -1);
+            if (in_pool(a, id)) __hip_atomic_fetch_add(a.refs + id, -1, __ATOMIC_RELAXED, SCOPE);
         }
         row[i] = -1;
     }
-}
-// The pages that row b of new_table asks for: `first` and how many.
-template <bool FORK>
-__device__ __forceinline__ int asked(const PageArgs& a, int b, int& first) {
-    const int cap = a.max_pages * a.page_rows;
-    if (FORK) {
-        const int len = a.new_lens[b];
-        first = len / a.page_rows;
-        return first < a.max_pages && a.new_table[(size_t)b * a.max_pages + first] == -2;
-    }
-    first = pages_of(min(a.lens[b], cap), a.page_rows);
-    return max(0, pages_of(min(a.after[b], cap), a.page_rows) - first);
+    first = n0;
+    return max(0, n1 - n0);
 }
 
 // Rows and counts of a large batch, a wave to a sequence: children, then parents.
 template <bool FORK>
 __global__ __launch_bounds__(256) void pages_rows(PageArgs a) {
     const int i = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
+    int first;
     if (FORK) {
-        if (i < a.children) fork_child(a, i);
-        else if (i < a.children + a.B) fork_parent(a, i - a.children);
+        if (i < a.children) (void)fork_child(a, a.parents, a.lens, i, first);
+        else if (i < a.children + a.B) fork_parent<__HIP_MEMORY_SCOPE_AGENT>(a, a.parents, a.lens, i - a.children);
     } else if (i < a.B) {
-        resize_row(a, i);
+        (void)resize_row<__HIP_MEMORY_SCOPE_AGENT>(a, i, a.lens[i], a.after[i], first);
     }
 }
 
-// Hands out the lowest free pages, in (sequence, index) order: one work-group. ALL: it
-// also does pages_rows' part first. Counts changed by this launch's atomics are read from
-// the coherence point, never from a line cached before.
+// Hands out the lowest free pages, in (sequence, index) order: one work-group, which a round
+// looks through PLAN_T * PLAN_IDS counts, lists the free ids and deals them to the sequences, a
+// wave to each. ALL: it also does pages_rows' part first, every sequence's chain of loads at once.
 template <bool FORK, bool ALL>
 __global__ __launch_bounds__(PLAN_T) void pages_take(PageArgs a) {
-    __shared__ int s_scan[PLAN_T / 64];
-    __shared__ int s_upto[PLAN_T];
-    const int tid = (int)threadIdx.x, wave = tid >> 6;
-    if (ALL) {
-        if (FORK) {
-            for (int c = wave; c < a.children; c += PLAN_T / 64) fork_child(a, c);
-            for (int p = wave; p < a.B; p += PLAN_T / 64) fork_parent(a, p);
-        } else {
-            for (int b = wave; b < a.B; b += PLAN_T / 64) resize_row(a, b);
+    constexpr int WAVES = PLAN_T / 64;
+    __shared__ int s_scan[WAVES];
+    __shared__ int s_upto[PLAN_T], s_first[PLAN_T], s_need[ALL ? PLAN_ONE : 1], s_in[ALL ? 2 * PLAN_ONE : 1];
+    __shared__ int s_free[PLAN_T * PLAN_IDS];
+    const int tid = (int)threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
+    const int rows = FORK ? a.children : a.B;
+    if constexpr (ALL) {                                    // at most PLAN_ONE sequences
+        int* in0 = s_in;                                    // parents, or lengths before
+        int* in1 = s_in + PLAN_ONE;                         // lengths, or lengths after
+        if (tid < rows) in0[tid] = FORK ? a.parents[tid] : a.lens[tid];
+        else if (tid >= PLAN_ONE && tid < PLAN_ONE + a.B) in1[tid - PLAN_ONE] = (FORK ? a.lens : a.after)[tid - PLAN_ONE];
+        __syncthreads();
+        for (int i = wave; i < rows + (FORK ? a.B : 0); i += WAVES) {
+            int first = 0, need = 0;
+            if (FORK && i >= rows) {
+                fork_parent<__HIP_MEMORY_SCOPE_WORKGROUP>(a, in0, in1, i - rows);
+                continue;
+            }
+            if (FORK) need = fork_child(a, in0, in1, i, first);
+            else need = resize_row<__HIP_MEMORY_SCOPE_WORKGROUP>(a, i, in0[i], in1[i], first);
+            if (lane == 0) {
+                s_first[i] = first;
+                s_need[i] = need;
+            }
         }
-        __threadfence();
+        // the counts are read below, for the first time in this launch, when all are changed
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
-    const int rows = FORK ? a.children : a.B;
     int cursor = 0, missing = 0;                            // every page below cursor is taken
     for (int b0 = 0; b0 < rows; b0 += PLAN_T) {
         const int b = b0 + tid;
-        int first = 0, total;
-        const int need = b < rows ? asked<FORK>(a, b, first) : 0;
+        int need = 0, total;
+        if (b < rows) {
+            if constexpr (ALL) {
+                need = s_need[b];
+            } else {
+                const int cap = a.max_pages * a.page_rows;
+                int first;
+                if (FORK) {
+                    first = a.new_lens[b] / a.page_rows;
+                    need = first < a.max_pages && a.new_table[(size_t)b * a.max_pages + first] == -2;
+                } else {
+                    first = pages_of(min(a.lens[b], cap), a.page_rows);
+                    need = max(0, pages_of(min(a.after[b], cap), a.page_rows) - first);
+                }
+                s_first[tid] = first;
+            }
+        }
         const int upto = block_scan<PLAN_T>(need, s_scan, total);
         s_upto[tid] = upto;
-        __syncthreads();
         int got = 0;                                        // of these sequences' requests
         while (got < total && cursor < a.num_pages) {
             const int id0 = cursor + tid * PLAN_IDS;
             int n = 0, found;
             uint32_t free = 0;
+            const __amdgpu_buffer_rsrc_t r = make_rsrc(a.refs + cursor, (uint32_t)min(a.num_pages - cursor, PLAN_T * PLAN_IDS) * 4u);
 #pragma unroll
-            for (int k = 0; k < PLAN_IDS; ++k)
-                if (id0 + k < a.num_pages && (int)load_dev(reinterpret_cast<const unsigned*>(a.refs) + id0 + k) == 0) {
-                    free |= 1u << k;
-                    ++n;
-                }
-            int rank = got + block_scan<PLAN_T>(n, s_scan, found) - n;
-            for (; free && rank < total; free &= free - 1, ++rank) {
-                const int id = id0 + __builtin_ctz(free);
-                int lo = 0, hi = PLAN_T - 1;                // the sequence whose requests end behind `rank`
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (s_upto[mid] > rank) hi = mid; else lo = mid + 1;
-                }
-                int at;
-                asked<FORK>(a, b0 + lo, at);
-                at += rank - (lo ? s_upto[lo - 1] : 0);
-                a.new_table[(size_t)(b0 + lo) * a.max_pages + at] = id;
-                store_dev(reinterpret_cast<unsigned*>(a.refs) + id, 1u);
+            for (int k = 0; k < PLAN_IDS; k += 4) {
+                const u32x4 c = __builtin_amdgcn_raw_buffer_load_b128(r, (uint32_t)(tid * PLAN_IDS + k) * 4u, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c[e] == 0 && id0 + k + e < a.num_pages) {
+                        free |= 1u << (k + e);
+                        ++n;
+                    }
             }
-            const bool more = got + found < total;
-            got = min(total, got + found);
-            if (more) cursor += PLAN_T * PLAN_IDS;
-            __threadfence();
+            int rank = block_scan<PLAN_T>(n, s_scan, found) - n;   // among this round's
+            for (; free && got + rank < total; free &= free - 1, ++rank) {
+                const int id = id0 + __builtin_ctz(free);
+                s_free[rank] = id;
+                a.refs[id] = 1;
+            }
             __syncthreads();
+            const int end = min(total, got + found);
+            for (int j = wave; j < min(PLAN_T, rows - b0); j += WAVES) {
+                const int lo = j ? s_upto[j - 1] : 0, hi = min(s_upto[j], end);
+                for (int k = max(lo, got) + lane; k < hi; k += 64)
+                    a.new_table[(size_t)(b0 + j) * a.max_pages + s_first[j] + (k - lo)] = s_free[k - got];
+            }
+            if (got + found < total) cursor += PLAN_T * PLAN_IDS;
+            got = end;
+            __syncthreads();                                // s_free is read
         }
         missing += total - got;
-        if (FORK && need && upto > got) a.new_table[(size_t)b * a.max_pages + first] = -1;
-        __syncthreads();                                    // s_upto is read
+        if (FORK && need && upto > got) a.new_table[(size_t)b * a.max_pages + s_first[tid]] = -1;
+        __syncthreads();                                    // s_upto and s_first are read
     }
     if (tid == 0 && a.missing) *a.missing = missing;
 }
@@ -277,7 +307,7 @@ hipError_t launch_compact(const PageArgs& a, hipStream_t stream) {
 }
 
 // One launch plans a small batch; a large one's rows are dealt over the device first.
-static bool plan_in_one(const PageArgs& a, int rows) { return rows <= 128 && (long long)rows * a.max_pages <= 1 << 15; }
+static bool plan_in_one(const PageArgs& a, int rows) { return rows <= PLAN_ONE && (long long)rows * a.max_pages <= 1 << 15; }
 
 hipError_t launch_resize(const PageArgs& a, hipStream_t stream) {
     if (plan_in_one(a, a.B)) {
