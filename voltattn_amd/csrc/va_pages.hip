@@ -294,7 +294,7 @@ __global__ __launch_bounds__(256) void compact_rows(PageArgs a) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int at = i * 256 + tid, r = at / w;
-        if (r < n && s_from[r] >= 0 && s_to[r] >= 0) reinterpret_cast<U*>(pool + s_to[r] * a.row_bytes)[at - r * w] = x[i];
+        if (r < n && s_from[r] >= 0 && s_to[r] >= 0) __builtin_nontemporal_store(x[i], reinterpret_cast<U*>(pool + s_to[r] * a.row_bytes) + (at - r * w));
     }
     if (sr < n && s_from[sr] >= 0 && s_to[sr] >= 0) sp[s_to[sr] * ng + (tid - sr * ng)] = sc;
 }
