@@ -191,3 +191,40 @@ def test_c_abi_writes_its_rows_only():
 def test_empty_batch():
     q = torch.empty((0, 4, 128), dtype=torch.float16, device="cuda")
     assert ops.prefill(q, q[:, :2], q[:, :2], _int([0, 0])).shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,at", [(1, 0), (50, 0), (50, 49), (130, 127), (130, 128), (300, 130), (700, 65), (700, 511)])
+def test_infinite_and_nan_values_reach_the_rows_that_see_them_only(n, at, D):
+    """Row `at` of V holds inf, -inf, NaN and finite values, as does row at + 3 (another order): a column's
+    outputs are the values' sum from that row on, and as if both rows were finite before it."""
+    q, k, v = _inputs(n, 2, 2, D, n + at)
+    cu = _int([0, n])
+    want = ops.prefill(q, k, v, cu)
+    bad, kinds = v.clone(), torch.tensor([float("inf"), -float("inf"), float("nan"), 1.0], device="cuda").half()
+    rows = [(at, 0)] + ([(at + 3, 1)] if at + 3 < n else [])
+    for row, turn in rows:
+        bad[row, 0] = kinds.roll(turn).repeat(D // 4)
+    got = ops.prefill(q, k, bad, cu)
+    assert torch.equal(got[:, 1], want[:, 1]) and torch.equal(got[:at], want[:at])
+    odd = torch.zeros((n, D), dtype=torch.float64, device="cuda")
+    for row, turn in rows:
+        x = bad[row, 0].double()
+        odd[row:] += torch.where(x.isfinite(), torch.zeros_like(x), x)
+    x = got[:, 0].double()
+    assert torch.equal(x.isnan(), odd.isnan())
+    assert torch.equal(x == float("inf"), odd == float("inf")) and torch.equal(x == -float("inf"), odd == -float("inf"))
+
+
+def test_infinite_and_nan_keys_reach_the_rows_that_see_them_only():
+    for at in (0, 63, 140):
+        q, k, v = _inputs(200, 2, 1, 128, at)
+        cu = _int([0, 200])
+        for x in (float("nan"), float("inf")):
+            bad = k.clone()
+            bad[at, 0, 5] = x
+            got = ops.prefill(q, bad, v, cu)
+            # not bit for bit: 32 rows take a new maximum together (an infinite score of one of them makes
+            # them), which rounds a sum anew; what that may be off is part of the bound
+            _check(got[:at], q[:at], k[:at], v[:at], [(0, at)])
+            assert got[at:][(q[at:, :, 5] > 0)].isnan().all()        # a score of NaN, or of inf

@@ -222,3 +222,37 @@ def test_other_stream_graph_and_repeat():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager), i
+
+
+@pytest.mark.parametrize("fmt", list(BITS))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,group", [(5, 4), (12, 4), (33, 4)])
+def test_infinite_and_nan_drafts_reach_the_rows_that_see_them_only(fmt, D, T, group):
+    """A draft whose values (quantized: one group's scale) are infinite or NaN: the drafts that do not see
+    it are as without, those that do get the values' kind in its columns. The whole context is one piece,
+    and many."""
+    for ctx in (0, 100, 5000):
+        c = Case(fmt, [ctx], T, 2 * group, 2, D, seed=T + ctx)
+        want = c.run()
+        c.sizes[0] = T
+        at = T // 2
+        page, row = c.table[0][(ctx + at) // c.page], (ctx + at) % c.page
+        sees = torch.tensor([bool(m >> at & 1) for m in c.masks[0]], device="cuda")
+        for kind in (float("inf"), -float("inf"), float("nan")):
+            v = (c.v if c.bits == 16 else c.vs).clone()
+            if c.bits == 16:
+                v[page, 0, row, 8:40] = kind
+                got = c.run(v=v)
+                lo, sign = 8, torch.ones(32, device="cuda", dtype=torch.double)
+            else:
+                lo, x = 32, c.v[page:page + 1, 0, row:row + 1]
+                ones = torch.ones((1, 1, D // 32), device="cuda", dtype=torch.half)
+                sign = ops.dequantize(x.contiguous(), ones, c.bits, 32)[0, 0, 32:64].double()      # the codes: 0 times inf is NaN
+                v[page, 0, row, 1] = kind
+                got = c.run(vs=v)
+            assert torch.equal(got[0, ~sees], want[0, ~sees]) and torch.equal(got[0, :, group:], want[0, :, group:])
+            odd = (sign * kind).expand(int(sees.sum()), group, 32)
+            x = got[0, sees][:, :group, lo:lo + 32].double()
+            assert torch.equal(x.isnan(), odd.isnan()) and torch.equal(x > 65504, odd > 65504) and torch.equal(x < -65504, odd < -65504)
+            rest = [i for i in range(D) if not lo <= i < lo + 32]
+            assert torch.equal(got[0, sees][..., rest], want[0, sees][..., rest])

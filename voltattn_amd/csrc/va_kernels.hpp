@@ -230,12 +230,14 @@ struct TreeArgs {
     int   max_pages, page_shift, num_pages;
     int   cap;                    // ctx + drafts at most
     float qscale;
-    int   nwg, min_share;         // work-groups, and the fewest tiles that one takes
+    int   nwg, qw;                // of its TreeForm
 };
-// Query rows and K/V rows of a work-group's tile where a K/V head has `rows` query rows.
-int tree_rows(int rows);
-int tree_tile(int rows);
-int tree_groups_per_cu(int D, int rows);
+// Row blocks of 32 qw query rows, K/V tiles of the batch at most, and work-groups.
+struct TreeForm {
+    int qw;
+    long long tiles, groups;
+};
+TreeForm tree_form(int kind, int D, int B, int hkv, int rows, int cap, int cus);   // rows: of a K/V head
 hipError_t launch_tree(int kind, int D, int G, const TreeArgs& a, hipStream_t stream);
 
 // Page pool bookkeeping and row moves (va_pages.hip). Each launch uses the fields that

@@ -14,7 +14,6 @@
 namespace va {
 
 constexpr int PF_BM = 128;         // query rows per work-group
-constexpr int PF_BN = 64;          // K/V rows per tile
 
 // Rows [begin, begin + n) of the packed batch; keys: whether they are a sequence (the
 // rows before the first and behind the last sequence are in none, and get zeros).
@@ -52,27 +51,11 @@ __device__ __forceinline__ bool prefill_span(const int32_t* __restrict__ cu, int
     return false;
 }
 
-// 16 bytes per lane to LDS, lane l's at `to` + 16 l; zeros where the offset is out of range.
-__device__ __forceinline__ void fetch_lds(__amdgpu_buffer_rsrc_t r, lds_u8* to, uint32_t off, uint32_t soff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to, 16, off, sgpr(soff), 0, 0);
-}
-
-// A barrier that waits for this wave's LDS reads and all but the last N of its loads to LDS.
-// (__syncthreads would wait for every load.)
-template <int N> __device__ __forceinline__ void barrier_but() {
-    static_assert(N == 0 || N == 2 || N == 4, "loads per operand");
-    if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if constexpr (N == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 template <int D>
 __global__ __launch_bounds__(256, 3) void prefill_causal(PrefillArgs a) {
     constexpr int KS = D / 16, DB = D / 32;
-    constexpr int TILE = PF_BN * 2 * D;                     // bytes of a K (or V) tile
-    constexpr int RPI = 1024 / (2 * D);                     // rows that one wave's 16-byte load covers
-    constexpr int LPW = TILE / 1024 / 4;                    // loads per wave and tile
-    __shared__ __align__(1024) uint8_t lds[3 * TILE];       // K of two tiles, V of one
+    __shared__ __align__(1024) uint8_t lds[3 * WideFetch<D>::TILE + 4];
+    lds_int* odd = (lds_int*)((lds_u8*)lds + 3 * WideFetch<D>::TILE);   // infinite or NaN values were left out
 
     const int lane = (int)__lane_id(), wave = uniform((int)threadIdx.x >> 6), half = lane >> 5;
     const int item = (int)(a.items - 1 - blockIdx.x / (unsigned)a.hq);
@@ -98,81 +81,28 @@ __global__ __launch_bounds__(256, 3) void prefill_causal(PrefillArgs a) {
     const int hk = head / a.group;
     const uint16_t* kp = a.k + (size_t)sp.begin * a.k_row + (size_t)hk * a.k_head;
     const uint16_t* vp = a.v + (size_t)sp.begin * a.v_row + (size_t)hk * a.v_head;
-    // Load i of the wave covers rows (wave LPW + i) RPI + lane / (D/8); its lanes fetch the chunks
-    // that swz() puts in their places: those of load 0 with another XOR.
-    const int lr = wave * LPW * RPI + lane / (D / 8);
-    const uint32_t kr = (uint32_t)lr * (uint32_t)a.k_row * 2u, vr = (uint32_t)lr * (uint32_t)a.v_row * 2u;
-    const uint32_t lc = (uint32_t)((lane % (D / 8)) ^ swz<D>(lr));
-    WideAddr<D> ad0;
-    ad0.init(lane);
-    lds_u8* kt = (lds_u8*)lds;
-    lds_u8* vt = kt + 2 * TILE;
-    // Loads go straight to LDS (4 per wave and operand); a wave waits for its own, the barrier
-    // behind the wait for everybody's. K is fetched a tile ahead, V during its tile's scores.
-    auto fetch = [&](const uint16_t* rows, long long stride, uint32_t lane_row, int j0, lds_u8* to) {
-        const int n = min(PF_BN, sp.n - j0);
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(rows + (size_t)j0 * stride, (uint32_t)(((n - 1) * (size_t)stride + D) * 2));
-#pragma unroll
-        for (int i = 0; i < LPW; ++i)
-            fetch_lds(r, to + (wave * LPW + i) * 1024, lane_row + ((lc ^ (uint32_t)(D == 128 ? i : 2 * i)) << 4), (uint32_t)(i * RPI * 2) * (uint32_t)stride);
+    WideAddr<D> ad;
+    ad.init(lane);
+    const WideFetch<D> load_k(wave, lane, (uint32_t)a.k_row * 2u), load_v(wave, lane, (uint32_t)a.v_row * 2u);
+    auto tile = [&](const WideFetch<D>& load, const uint16_t* rows, long long stride, int t, lds_u8* to) {
+        const int j0 = t * WIDE_BN, n = min(WIDE_BN, sp.n - j0);
+        load(make_rsrc(rows + (size_t)j0 * stride, (uint32_t)(((n - 1) * (size_t)stride + D) * 2)), to);
     };
-
+    if (threadIdx.x == 0) *odd = 0;
     f32x16 o[DB] = {};
-    float m = -__builtin_inff(), l = 0.f;                   // m: in raw scores
-    const int last = min(r0 + PF_BM, sp.n);                 // keys that the work-group needs
-    fetch(kp, a.k_row, kr, 0, kt);
-    for (int j0 = 0, odd = 0; j0 < last; j0 += PF_BN, odd ^= TILE) {
-        barrier_but<0>();                                   // K has arrived; V of the last tile is read
-        const WideAddr<D> ad = ad0.fresh();
-        fetch(vp, a.v_row, vr, j0, vt);
-        const bool more = j0 + PF_BN < last;
-        if (more) fetch(kp, a.k_row, kr, j0 + PF_BN, kt + (odd ^ TILE));
-        __builtin_amdgcn_sched_barrier(0);
-        f32x16 s[PF_BN / 32] = {};
+    float m = -__builtin_inff(), l = 0.f;
+    wide_walk<D, 4>((lds_u8*)lds, ad, q, 0, (min(r0 + PF_BM, sp.n) + WIDE_BN - 1) / WIDE_BN, a.qscale,
+        [&](int t, lds_u8* to) { tile(load_k, kp, a.k_row, t, to); }, [&](int t, lds_u8* to) { tile(load_v, vp, a.v_row, t, to); },
+        [&](int t) { return t * WIDE_BN + WIDE_BN - 1 > r0; },
+        [&](int t, f32x16 (&s)[WIDE_BN / 32]) {
+            if (t * WIDE_BN + WIDE_BN - 1 <= r0 + wave * 32) return;    // no key is behind a row of the wave
+            const int last = row - t * WIDE_BN - 4 * half;
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
-#pragma unroll
-            for (int b = 0; b < PF_BN / 32; ++b) s[b] = mfma_32x32x16(lds_row8(kt + odd + b * 64 * D, ad.k(i)), q[i], s[b]);
-        feed_mfma<PF_BN / 32 * KS, 1, 4>();
-        __builtin_amdgcn_sched_barrier(0);
-        if (j0 + PF_BN - 1 > r0 + wave * 32) {              // keys behind some row of the wave
-#pragma unroll
-            for (int b = 0; b < PF_BN / 32; ++b)
+            for (int b = 0; b < WIDE_BN / 32; ++b)
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
-                    if (j0 + 32 * b + 8 * (v / 4) + 4 * half + v % 4 > row) s[b][v] = -__builtin_inff();
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int b = 0; b < PF_BN / 32; ++b)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) top = fmaxf(top, s[b][v]);
-        top = halves_max(top);
-        if (__any((top - m) * a.qscale > WIDE_SLACK)) {     // also at the first tile: m = -inf
-            const float to = fmaxf(m, top), f = to == m ? 1.f : fast_exp2((m - to) * a.qscale);
-            m = to;
-            l *= f;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) o[db] *= f;
-        }
-        const float base = m == -__builtin_inff() ? 0.f : m * a.qscale - WIDE_OFF;
-        f16x8 p[PF_BN / 32][2];
-#pragma unroll
-        for (int b = 0; b < PF_BN / 32; ++b)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const float e = fast_exp2(__builtin_fmaf(s[b][v], a.qscale, -base));
-                l += e;
-                p[b][v / 8][v % 8] = (_Float16)e;
-            }
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) barrier_but<LPW>();                       // V has arrived, K of the next tile may not have
-        else barrier_but<0>();
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int b = 0; b < PF_BN / 32; ++b) wide_values<D>(vt + b * 64 * D, ad, p[b], o);
-        feed_mfma<PF_BN / 32 * 2 * DB, 2, 4>();
-    }
+                    s[b][v] = 32 * b + 8 * (v / 4) + v % 4 > last ? -__builtin_inff() : s[b][v];
+        }, odd, m, l, o);
     l = halves_sum(l);
     if (!live) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -180,6 +110,15 @@ __global__ __launch_bounds__(256, 3) void prefill_causal(PrefillArgs a) {
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
+            if (*odd) {                                 // of the tiles from the block's first row's on
+                const uint16_t* p = vp + 32 * db + 8 * g + 4 * half;
+#pragma unroll 1
+                for (int j = r0; j <= row; ++j) {
+                    const f16x4 x = *reinterpret_cast<const f16x4*>(p + (size_t)j * a.v_row);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[db][4 * g + i] += wide_odd((float)x[i]);
+                }
+            }
             f16x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = (_Float16)(l == 0.f ? 0.f : o[db][4 * g + i] * inv);

@@ -835,18 +835,15 @@ int va_prefill(const va_prefill_bufs* b, const va_prefill_shape* sh, void* strea
 
 namespace {
 
-// Checks of va_decode_tree's shape; the number of work-groups on success.
-int validate_tree(va_fmt fmt, const va_paged_shape* sh, int T, int* nwg) {
+// Checks of va_decode_tree's shape, and its launch form.
+int validate_tree(va_fmt fmt, const va_paged_shape* sh, int T, va::TreeForm* form) {
     const int rc = validate_shape(fmt, sh, true);
     if (rc) return rc;
     if (T < 1 || T > VA_TREE_MAX) return fail(VA_EINVAL, "T must be in [1, %d] (got %d)", VA_TREE_MAX, T);
     const long long rows = (long long)T * (sh->Hq / sh->Hkv);
     if (rows > 1 << 20 || (long long)sh->B * T * sh->Hq > 0x7FFFFFFFLL / 64) return fail(VA_ERANGE, "B*T*Hq too large");
-    const int bm = va::tree_rows((int)rows), bn = va::tree_tile((int)rows);
-    const long long blocks = (long long)sh->B * sh->Hkv * ((rows + bm - 1) / bm);
-    const long long tiles = blocks * std::max(1LL, ((long long)sh->max_seq_len + bn - 1) / bn);
-    if (tiles > 0x7FFFFFFFLL) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", tiles);
-    *nwg = (int)std::min(tiles, (long long)(getenv("VA_WG") ? atoi(getenv("VA_WG")) : va::tree_groups_per_cu(sh->D, (int)rows)) * cus_or_default());
+    *form = va::tree_form(kind_of(fmt), sh->D, sh->B, sh->Hkv, (int)rows, sh->max_seq_len, cus_or_default());
+    if (form->tiles > 1 << 30) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
     return VA_OK;
 }
 
@@ -855,14 +852,14 @@ int validate_tree(va_fmt fmt, const va_paged_shape* sh, int T, int* nwg) {
 extern "C" {
 
 size_t va_tree_ws_bytes(va_fmt fmt, const va_paged_shape* sh, int T) {
-    int nwg = 0;
-    if (validate_tree(fmt, sh, T, &nwg)) return 0;
-    return (size_t)2 * nwg * va::tree_rows(T * (sh->Hq / sh->Hkv)) * (sh->D + 2) * sizeof(float);
+    va::TreeForm form;
+    if (validate_tree(fmt, sh, T, &form)) return 0;
+    return (size_t)2 * form.groups * (32 * form.qw) * (sh->D + 2) * sizeof(float);
 }
 
 int va_decode_tree(va_fmt fmt, const va_tree_bufs* b, const va_paged_shape* sh, int T, void* stream) {
-    int nwg = 0;
-    const int rc = validate_tree(fmt, sh, T, &nwg);
+    va::TreeForm form;
+    const int rc = validate_tree(fmt, sh, T, &form);
     if (rc) return rc;
     if (!b) return fail(VA_ENULL, "bufs is NULL");
     const bool quant = !is_f16(fmt);
@@ -901,8 +898,8 @@ int va_decode_tree(va_fmt fmt, const va_tree_bufs* b, const va_paged_shape* sh, 
     a.num_pages = sh->num_pages;
     a.cap = sh->max_seq_len;
     a.qscale = (float)(1.4426950408889634074 / std::sqrt((double)sh->D));
-    a.nwg = nwg;
-    a.min_share = getenv("VA_MS") ? atoi(getenv("VA_MS")) : 1;
+    a.nwg = (int)form.groups;
+    a.qw = form.qw;
     const hipError_t e = va::launch_tree(kind_of(fmt), sh->D, is_f16(fmt) ? 64 : sh->G, a, as_stream(stream));
     if (e != hipSuccess) return hip_fail(e, "tree launch");
     return VA_OK;

@@ -1,18 +1,36 @@
 // va_tree.hip — launches of the tree kernels (va_tree.hpp).
 #include "va_tree.hpp"
+#include <algorithm>
 
 namespace va {
 
-// Waves side by side over the query rows of a K/V head.
-static int tree_qw(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
-
-int tree_rows(int rows) { return 32 * tree_qw(rows); }
-int tree_tile(int rows) { return tree_qw(rows) == 1 ? TreeTile<1>::BN : TreeTile<2>::BN; }
-int tree_groups_per_cu(int D, int rows) { return tree_waves(D, tree_qw(rows)); }
+// The row block that holds all rows of a K/V head, up to 128 rows, reads K and V once and
+// fills the card from about 4 tiles to a CU on. Below, one work-group to a CU takes the
+// next narrower block: fewer pieces to join, each with fewer rows, outweigh reading K and V twice.
+// One sequence, 64 rows to a K/V head (8 of them, q8), narrower : wider: 4096 positions (2 tiles)
+// 16.6 : 22.8 us, 32768 (16 tiles) 47.2 : 39.2 us; 128 rows, 4096 positions 19.9 : 28.6 us;
+// 16 sequences of 8192 positions, 128 rows, q4 78.9 : 63.2 us.
+TreeForm tree_form(int kind, int D, int B, int hkv, int rows, int cap, int cus) {
+    TreeForm f;
+    f.qw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+    auto count = [&]() {
+        const long long bm = 32 * f.qw, bn = f.qw == 1 ? TreeTile<1>::BN : TreeTile<2>::BN;
+        return (long long)B * hkv * ((rows + bm - 1) / bm) * std::max(1LL, (cap + bn - 1) / bn);
+    };
+    f.tiles = count();
+    f.groups = (long long)tree_waves(kind, D, f.qw) * cus;
+    if (f.qw > 1 && f.tiles <= 4LL * cus) {
+        f.qw /= 2;
+        f.tiles = count();
+        f.groups = cus;
+    }
+    f.groups = std::min(f.groups, f.tiles);
+    return f;
+}
 
 template <int KIND, int D, int G>
 static hipError_t launch(const TreeArgs& a, hipStream_t stream) {
-    const dim3 grid((unsigned)a.nwg), block(256);
+    const dim3 grid((unsigned)(a.nwg + 7) / 8 * 8), block(256);
     const bool few = (long long)a.B * a.T * a.hkv * a.group <= 8192;   // 32 to a work-group would leave CUs idle
     const int mr = few ? 8 : 32;
     const dim3 mgrid((unsigned)((size_t)a.B * a.hkv * ((a.T * a.group + mr - 1) / mr)));
@@ -27,7 +45,7 @@ static hipError_t launch(const TreeArgs& a, hipStream_t stream) {
             e = hipGetLastError();                                                         \
         }                                                                                  \
     } while (0)
-    switch (tree_qw(a.T * a.group)) {
+    switch (a.qw) {
         case 1: VA_TREE(1); break;
         case 2: VA_TREE(2); break;
         default: VA_TREE(4); break;

@@ -183,18 +183,43 @@ template <int BM, int BN> struct TreePlan {
         b = b0 + l;
         return lane(l);
     }
-    __device__ __forceinline__ int share() const { return max((total + a.nwg - 1) / a.nwg, a.min_share); }
+    __device__ __forceinline__ int share() const { return max((total + a.nwg - 1) / a.nwg, 1); }
+    __device__ __forceinline__ int shares(int share) const { return (total + share - 1) / share; }
 };
 
 // --------------------------------------------------------------- kernel --
-#ifndef KVAUX
-#define KVAUX 0
-#endif
-#ifndef PART_AUX
-#define PART_AUX 16
-#endif
+// The infinite and NaN ones of values c .. c + 3 of position j's V row, as its tile would hold
+// them, 0 for the others.
+template <int KIND, int D, int G, bool EXACT2>
+__device__ __forceinline__ f32x4 tree_odd(const uint8_t* v, const uint16_t* sv, int page_shift, int num_pages, int hkv, int page, int hk, int j, int c) {
+    f32x4 x = {};
+    if (page < 0 || page >= num_pages) return x;
+    const size_t r = (((size_t)page * hkv + hk) << page_shift) + (size_t)(j & ((1 << page_shift) - 1));
+    const uint8_t* row = v + r * RowBytes<KIND, D>::value;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int d = c + e;
+        if constexpr (KIND == KF16) {
+            x[e] = wide_odd((float)reinterpret_cast<const _Float16*>(row)[d]);
+        } else {
+            int n;
+            if constexpr (KIND == KQ8) n = (int8_t)row[d];
+            else if constexpr (KIND == KQ4) n = ((row[d >> 1] >> (4 * (d & 1))) & 15) - 8;
+            else {
+                const uint8_t* p = row + 3 * (d >> 3);      // eight codes in 24 bits
+                n = (int)(((uint32_t)p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16) >> (3 * (d & 7)) & 7u) - 4;
+            }
+            const _Float16 s = __builtin_bit_cast(_Float16, sv[r * (D / G) + d / G]);
+            if constexpr (EXACT2) x[e] = wide_odd((float)((_Float16)(float)n * (s * (_Float16)0.5f)));
+            else x[e] = wide_odd((float)s) == 0.f ? 0.f : (float)n * (float)s;
+        }
+    }
+    return x;
+}
+
+constexpr int PART_AUX = 16;       // written through the L2s (sc1)
 // Work-groups that fit a CU (waves to a SIMD): their registers decide.
-constexpr int tree_waves(int D, int qw) { return qw < 4 ? 2 : D == 128 ? 3 : 4; }
+constexpr int tree_waves(int kind, int D, int qw) { return qw < 4 ? 2 : D == 128 || kind == KF16 ? 3 : 4; }
 template <int QW> struct TreeTile {
     static constexpr int BM = 32 * QW, KW = 4 / QW;
     static constexpr int BN = QW == 1 ? 128 : 64;
@@ -202,7 +227,7 @@ template <int QW> struct TreeTile {
 };
 
 template <int KIND, int D, int G, int QW>
-__global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a) {
+__global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(TreeArgs a) {
     using T = TreeTile<QW>;
     constexpr int BM = T::BM, BN = T::BN, KW = T::KW, KB = T::KB;
     constexpr int KS = D / 16, DB = D / 32;
@@ -217,17 +242,18 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
     // A tile is fetched while its predecessor is computed, or, by the widest row blocks, when it is
     // its turn: three work-groups fit a CU without its registers and cover each other's waits
     constexpr bool AHEAD = QW != 4;
-    constexpr int AUX = QW == 4 ? KVAUX : VA_LOAD_AUX;      // the row blocks of a K/V head read the same rows
+    constexpr int AUX = QW == 4 ? 0 : VA_LOAD_AUX;      // the row blocks of a K/V head read the same rows
     using WR = WeightRange<SCALED ? KIND : KF16>;
     constexpr int GP = QW == 1 ? 1 : NG > 2 ? 2 : NG, VP = GP;   // scale groups that are in registers at once
     constexpr int HALVES = BN / 64;                         // a page holds at least 64 rows
     constexpr int RSRCS = 256 / UPR > 64 ? 1 : HALVES;      // halves that a wave fetches from
     constexpr int SCB = SCALED ? NG * BN * 2 : 0;           // bytes of a tile's scales, [group][row]
-    constexpr int TILES = (EXACT2 ? 3 : 2) * TILE + 2 * SCB;
+    constexpr int TILES = (QW == 4 ? 3 : 2) * TILE + 2 * SCB;   // QW = 4: also K's second terms, or K of the next tile
     constexpr int ES = 68;                                  // epilogue: 64 columns of a row, the next four banks on
     constexpr int EPI = 4 * 32 * ES * 4;
     constexpr int LDS = TILES > EPI + 1024 ? TILES : EPI + 1024;
-    __shared__ __align__(1024) uint8_t lds[LDS];
+    __shared__ __align__(1024) uint8_t lds[LDS + 4];
+    lds_int* odd = (lds_int*)((lds_u8*)lds + LDS);          // infinite or NaN values were left out
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     // the thread's number, made anew: what is computed from it is not held across loops
@@ -245,16 +271,19 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
     WideAddr<D> ad0;
     ad0.init(lane, kw * KB * 32);
 
-    // consecutive shares on one XCD (work-groups are dealt to the eight in turn): the row
-    // blocks of a K/V head lie next to each other and read the same rows
-    const int wg = (a.nwg & 7) == 0 ? (int)(blockIdx.x & 7) * (a.nwg >> 3) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
-    int at = 0, end = 0;
+    if (tid == 0) *odd = 0;
+    int wg = 0, at = 0, end = 0;
     do {                                                    // the pieces of the share; each finds its place anew
         const int lane = fresh_tid() & 63, half = lane >> 5;
         TreePlan<BM, BN> plan(a);                           // (holding the plan would cost the loop's registers)
         if (end == 0) {
-            at = wg * plan.share();
-            end = min(plan.total, at + plan.share());
+            // consecutive shares on one XCD (work-groups are dealt to the eight in turn), as many on
+            // each: the row blocks of a K/V head lie next to each other and read the same rows
+            const int share = plan.share(), per = (plan.shares(share) + 7) >> 3;
+            if ((int)(blockIdx.x >> 3) >= per) return;
+            wg = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+            at = wg * share;
+            end = min(plan.total, at + share);
             if (at >= end) return;
         }
         int b;
@@ -342,8 +371,11 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
                 }
             }
         };
-        auto stage = [&]() {
+        auto hides = [&](int t) { return (t + 1) * BN > sq.ctx; };   // drafts, or rows behind the sequence
+        auto stage = [&](int t) {
             const int tid = fresh_tid();
+            const bool clean = hides(t);
+            bool any = false;
 #pragma unroll
             for (int i = 0; i < UPT; ++i) {
                 const int u = i * 256 + tid, r = u / UPR, c = (u % UPR) * (Unit<KIND>::UE / 8);
@@ -367,7 +399,13 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
 #pragma unroll
                     for (int e = 0; e < Unit<KIND>::UE / 8; ++e) {
                         const int to = r * 2 * D + (((c + e) ^ swz<D>(r)) << 4);
-                        *reinterpret_cast<lds_f16x8*>(vt + to) = EXACT2 ? x[e] * vs : x[e];
+                        if constexpr (EXACT2) x[e] *= vs;
+                        if constexpr (!SCALED) {
+                            u32x4 y = __builtin_bit_cast(u32x4, x[e]);
+                            if (clean) any |= wide_clean(y);
+                            x[e] = __builtin_bit_cast(f16x8, y);
+                        }
+                        *reinterpret_cast<lds_f16x8*>(vt + to) = x[e];
                     }
                     if (!AHEAD) __builtin_amdgcn_sched_barrier(0);
                 }
@@ -376,12 +414,19 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
                 const int r = tid & 127;
                 if (r < BN) {
                     lds_u8* s = tid < 128 ? skt : svt;
+                    if (clean && tid >= 128) {              // odd values of V are those of its scales
+                        u32x4 y = {scr[0], scr[1], 0u, 0u};
+                        any = wide_clean(y);
+                        scr[0] = y.x;
+                        scr[1] = y.y;
+                    }
 #pragma unroll
                     for (int g = 0; g < NG; ++g)
                         *reinterpret_cast<__attribute__((address_space(3))) uint16_t*>(s + (g * BN + r) * 2) =
                             (uint16_t)(scr[g / 2] >> (16 * (g & 1)));
                 }
             }
+            if (any) *odd = 1;
         };
 
         // keeps the operands' loads ahead of the arithmetic that covers their latency; with few
@@ -393,11 +438,64 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
         float m = -__builtin_inff(), l = 0.f;               // m: raw scores; p = exp2((s - m) qscale + OFF)
         if constexpr (AHEAD) fetch(t0);
         const uint64_t mask = sq.n < 64 ? bits & ((1ull << sq.n) - 1) : bits;
-        for (int t = t0; t < t1; ++t) {
+        // takes the positions from j on that a row does not see out of a block of scores
+        auto hide = [&](int j, f32x16& s) {
+            if (j + 32 <= sq.ctx) return;                   // no drafts, nor rows behind the sequence
+            const int d = sq.ctx - j;                       // below 32: where the drafts begin
+            uint32_t seen = d > 0 ? ((1u << d) - 1u) | (uint32_t)(mask << d) : d > -64 ? (uint32_t)(mask >> -d) : 0u;
+            seen >>= 4 * half;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = seen & (1u << (8 * (v / 4) + v % 4)) ? s[v] : -__builtin_inff();
+        };
+        auto hide_tile = [&](int t, f32x16 (&s)[KB]) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) hide(t * BN + 32 * b, s[b]);
+        };
+        if constexpr (KIND == KF16 && QW == 4) {
+            size_t at = 0, next = 0;                        // pool row of the tile fetched, and of its successor
+            int left = 0, ahead = 0;
+            auto tile = [&](const uint8_t* pool, lds_u8* to) {
+                WideFetch<D>(wave, fresh_tid() & 63, ROWB)(make_rsrc(pool + uniform64(at) * ROWB, (uint32_t)(uniform(left) * ROWB)), to);
+            };
+            auto seek = [&](int t) {
+                const int j = t * BN;
+                ahead = min(64, sq.len - j);
+                int page = table[j >> a.page_shift];
+                if (page < 0 || page >= a.num_pages) {
+                    bad = true;
+                    ahead = page = 0;
+                }
+                next = (((size_t)page * a.hkv + hk) << a.page_shift) + (size_t)(j & ((1 << a.page_shift) - 1));
+            };
+            seek(t0);
+            __syncthreads();                                // the last piece's sums are read
+            wide_walk<D, 2>(kt, ad0, q, t0, t1, qs,
+                [&](int t, lds_u8* to) {
+                    at = next;
+                    left = ahead;
+                    if (t + 1 < t1) seek(t + 1);
+                    tile(a.k, to);
+                },
+                [&](int, lds_u8* to) { tile(a.v, to); },    // called before its successor's K is fetched
+                hides, hide_tile, odd, m, l, o);
+        } else if constexpr (QW == 4) {
+            for (int t = t0; t < t1; ++t) {
+                __syncthreads();                            // the last tile, or sums, are read
+                fetch(t);
+                stage(t);
+                __syncthreads();
+                const WideAddr<D> ad = ad0.fresh();
+                f32x16 s[KB];
+                wide_scores<D, KB, 2, true>(kt, skt, ad, q, s);
+                hide_tile(t, s);
+                f16x8 p[KB][2];
+                wide_weights<D, KB>(s, qs, m, l, o, p);
+                wide_values<D, KB>(vt, ad, p, o);
+            }
+        } else for (int t = t0; t < t1; ++t) {
             __syncthreads();                                // the last tile, or sums, are read
-            if constexpr (!AHEAD) fetch(t);
-            stage();
-            if (AHEAD && t + 1 < t1) fetch(t + 1);
+            stage(t);
+            if (t + 1 < t1) fetch(t + 1);
             __syncthreads();
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -406,10 +504,8 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
                 const uint32_t at32 = (uint32_t)(kb * 64 * D);   // the block's rows, in bytes
                 f32x16 s = {};
                 f16x8 kf[KS];
-                if constexpr (QW != 4) {
 #pragma unroll
-                    for (int i = 0; i < KS; ++i) kf[i] = lds_row8(kt, ad.k(i) + at32);
-                }
+                for (int i = 0; i < KS; ++i) kf[i] = lds_row8(kt, ad.k(i) + at32);
                 order();
                 if constexpr (SCALED) {
 #pragma unroll
@@ -431,25 +527,19 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
                             for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(acc[g][v], (float)sc[g][v / 4][v % 4], s[v]);
                     }
                 } else {
-                    if constexpr (EXACT2) {
 #pragma unroll
-                        for (int i = 0; i < KS; ++i) s = mfma_32x32x16(lds_row8(skt, ad.k(i) + at32), q[i], s);
-                    }
-#pragma unroll
-                    for (int i = 0; i < KS; ++i) s = mfma_32x32x16(QW == 4 ? lds_row8(kt, ad.k(i) + at32) : kf[i], q[i], s);
+                    for (int i = 0; i < KS; ++i) s = mfma_32x32x16(kf[i], q[i], s);
                 }
                 // V's operands are on their way while the weights are made
                 order();
                 f16x8 vf[2][DB];
-                if constexpr (QW != 4) {
 #pragma unroll
-                    for (int tt = 0; tt < 2; ++tt)
+                for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-                        for (int db = 0; db < DB; ++db) {
-                            const uint32_t to = at32 + (uint32_t)(tt * 32 * D);
-                            vf[tt][db] = lds_tr8(vt, ad.v(db, 0) + to, ad.v(db, 1) + to);
-                        }
-                }
+                    for (int db = 0; db < DB; ++db) {
+                        const uint32_t to = at32 + (uint32_t)(tt * 32 * D);
+                        vf[tt][db] = lds_tr8(vt, ad.v(db, 0) + to, ad.v(db, 1) + to);
+                    }
                 f16x4 vsc[NG][4];
                 if constexpr (SCALED) {
 #pragma unroll
@@ -458,13 +548,7 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
                         for (int v4 = 0; v4 < 4; ++v4) vsc[g][v4] = lds_scales(svt, sat + (uint32_t)((g * BN + kb * 32 + 8 * v4) * 2));
                 }
                 order();
-                if (j + 32 > sq.ctx) {                      // drafts, or rows behind the sequence
-                    const int d = sq.ctx - j;               // below 32: where the drafts begin
-                    uint32_t seen = d > 0 ? ((1u << d) - 1u) | (uint32_t)(mask << d) : d > -64 ? (uint32_t)(mask >> -d) : 0u;
-                    seen >>= 4 * half;
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) s[v] = seen & (1u << (8 * (v / 4) + v % 4)) ? s[v] : -__builtin_inff();
-                }
+                hide(j, s);
                 float top = s[0];
 #pragma unroll
                 for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
@@ -487,10 +571,6 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
                 if constexpr (!SCALED) {
 #pragma unroll
                     for (int v = 0; v < 16; ++v) p[v / 8][v % 8] = (_Float16)s[v];
-                }
-                if constexpr (QW == 4) {
-                    wide_values<D>(vt + at32, ad, p, o);
-                    continue;
                 }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
@@ -565,6 +645,14 @@ __global__ __launch_bounds__(256, tree_waves(D, QW)) void tree_attend(TreeArgs a
                 const int to = rb * BM + r;
                 if (to >= rows) continue;
                 if (EXACT2) x *= 2.f;
+                if (*odd) {                             // what was left out, to the rows that see it
+                    const int nd = to / a.group;
+                    const uint64_t bits = a.mask[(size_t)b * a.T + nd];
+#pragma unroll 1
+                    for (int j = max(t0, sq.ctx / BN) * BN; j < min(t1 * BN, sq.len); ++j)
+                        if (j < sq.ctx || (bits >> (j - sq.ctx) & 1)) 
+                            x += tree_odd<KIND, D, G, EXACT2>(a.v, a.sv, a.page_shift, a.num_pages, a.hkv, table[j >> a.page_shift], hk, j, c0 + c);
+                }
                 if (whole) {
                     const float inv = ll == 0.f ? 0.f : 1.f / ll;
                     f16x4 y;
