@@ -105,20 +105,20 @@ __global__ __launch_bounds__(256, 3) void prefill_causal(PrefillArgs a) {
         }, odd, m, l, o);
     l = halves_sum(l);
     if (!live) return;
+    if (*odd)                                               // of the tiles from the block's first row's on
+#pragma unroll 1
+        for (int j = r0; j <= row; ++j)
+#pragma unroll
+            for (int d = 0; d < D / 8; ++d) {
+                const f16x4 x = *reinterpret_cast<const f16x4*>(vp + (size_t)j * a.v_row + 8 * d + 4 * half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d / 4][4 * (d % 4) + i] += wide_odd((float)x[i]);
+            }
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            if (*odd) {                                 // of the tiles from the block's first row's on
-                const uint16_t* p = vp + 32 * db + 8 * g + 4 * half;
-#pragma unroll 1
-                for (int j = r0; j <= row; ++j) {
-                    const f16x4 x = *reinterpret_cast<const f16x4*>(p + (size_t)j * a.v_row);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[db][4 * g + i] += wide_odd((float)x[i]);
-                }
-            }
             f16x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = (_Float16)(l == 0.f ? 0.f : o[db][4 * g + i] * inv);
