@@ -353,8 +353,8 @@ typedef struct {
  * its rows 0 .. i, softmax(q.K^T / sqrt(D)) V per query head. Rows of out in no
  * sequence (before cu[0], from cu[B] on) become zero. A bound below its
  * predecessor counts as equal to it, one above total as total. A row whose
- * scores are all -inf is zero; NaN or an infinity in row j of k or v may reach
- * any row of its 128-row block before j, and no row of another sequence.
+ * scores are all -inf is zero. NaN and infinities in row j of k or v reach the
+ * rows from j on of its sequence only.
  * Asynchronous on `stream`; needs no workspace. */
 int va_prefill(const va_prefill_bufs* b, const va_prefill_shape* shape, void* stream);
 
@@ -382,8 +382,11 @@ typedef struct {
  * which nothing is visible, and drafts from tree_sizes[b] on, give zeros. A
  * sequence with ctx + size above max_seq_len, or a length or size out of range,
  * gives NaN for all T drafts; a page id outside the pool on one of its positions
- * NaN for its drafts. V values whose scale exceeds 1023 (q8), 16383 (q4) or 32767
- * (q3), beyond any cache made from fp16 values, may overflow to infinities. The
+ * NaN for its drafts. NaN and infinities in a draft's rows reach the drafts that
+ * attend it only. Quantized formats: caches made from fp16 values are in range;
+ * V values whose scale exceeds 1023 (q8), 16383 (q4) or 32767 (q3) may overflow
+ * to infinities, and where a K/V head has more than 64 query rows (T * Hq / Hkv)
+ * so may K or V values above 131008; there V's values are rounded to fp16. The
  * tiled formats only. The last bits of a sequence's sums depend on the
  * lengths of the whole batch; the same batch gives the same bits. Asynchronous
  * on `stream`; concurrent calls need distinct ws. */

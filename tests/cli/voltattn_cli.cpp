@@ -3,7 +3,8 @@
 //
 //   voltattn [--selftest]   42-case selftest at G=64 (+ the quantized cases at G=32)
 //   voltattn --selftest-ex  grouped-query, paged and append cases through the
-//                           C++ mirror (voltattn.hpp), 42 cases
+//                           C++ mirror (voltattn.hpp), 42 cases, and the serving
+//                           operators together in each tiled format
 //   voltattn --probe        HBM read ceiling
 //   voltattn --bench        selftest gate, probe, then the format x L table
 //   voltattn --selftest-host  the selftest's host side alone, no GPU: every
@@ -343,6 +344,125 @@ bool paged_case(Fmt f, int Hq, int Hkv, int D, int G, int P, const std::vector<i
     return gate(got, ref, maxerr);
 }
 
+// The serving wrappers of the mirror, on one pool: pages for two sequences, their rows appended, a
+// prompt attended, a third sequence forked off, two drafts each verified (a chain: the same as two
+// single steps), the second kept alone, and everything given back; outputs against launch_paged's.
+bool serving_case(Fmt f, int G, double* maxerr) {
+    const int B = 2, C = 3, Hq = 8, Hkv = 2, D = 128, P = 64, pages = 16, wide = 4, T = 2;
+    const int32_t lens[B] = {100, 63};
+    const bool quant = !is_f16(f);
+    const size_t pool = (size_t)pages * page_bytes(f, Hkv, P, D), sc = quant ? (size_t)pages * page_scale_bytes(f, Hkv, P, D, G) : 2;
+    DeviceBuffer K(pool), V(pool), SK(sc), SV(sc);
+    auto ints = [](std::vector<int32_t> x) {
+        DeviceBuffer d(x.size() * 4);
+        d.upload(x.data(), x.size() * 4);
+        return d;
+    };
+    auto read = [](const DeviceBuffer& d, size_t n) {
+        std::vector<int32_t> x(n);
+        check(va_sync());
+        d.download(x.data(), n * 4);
+        return x;
+    };
+    auto rows = [](size_t n, uint64_t seed) {               // fp16 normal values
+        DeviceBuffer x(n * 4), h(n * 2);
+        check(va_fill_normal(x.as<float>(), n, seed, nullptr));
+        check(va_f32_to_f16(x.as<float>(), n, h.as<uint16_t>(), nullptr));
+        check(va_sync());
+        return h;
+    };
+    DeviceBuffer table = ints(std::vector<int32_t>(B * wide, -1)), refs = ints(std::vector<int32_t>(pages, 0));
+    DeviceBuffer none = ints({0, 0, 0}), held = ints({lens[0], lens[1]}), missing = ints({-1});
+    resize_pages(B, P, wide, pages, table.as<int32_t>(), refs.as<int32_t>(), none.as<int32_t>(), held.as<int32_t>(), missing.as<int32_t>());
+    bool ok = read(missing, 1)[0] == 0;
+    PagedShape sh{B, Hq, Hkv, D, G, P, wide, pages, wide * P};
+    DeviceBuffer kx = rows((size_t)B * Hkv * 100 * D, 1), vx = rows((size_t)B * Hkv * 100 * D, 2);
+    auto append = [&](const DeviceBuffer& k, const DeviceBuffer& v, int n, const DeviceBuffer& start, const DeviceBuffer& tab, const PagedShape& s) {
+        append_kv(f, k.as<uint16_t>(), n, start.as<int32_t>(), tab.as<int32_t>(), s, K.get(), quant ? SK.as<uint16_t>() : nullptr);
+        append_kv(f, v.as<uint16_t>(), n, start.as<int32_t>(), tab.as<int32_t>(), s, V.get(), quant ? SV.as<uint16_t>() : nullptr);
+    };
+    append(kx, vx, 100, none, table, sh);                   // rows past a sequence's pages are dropped
+
+    // the forked sequences: 0, 0 again, 1; then two drafts each
+    DeviceBuffer parents = ints({0, 0, 1}), table2 = ints(std::vector<int32_t>(C * wide, -7)), ctx = ints({0, 0, 0});
+    const Pools pools{K.get(), V.get(), quant ? SK.as<uint16_t>() : nullptr, quant ? SV.as<uint16_t>() : nullptr};
+    fork_pages(f, pools, sh, table.as<int32_t>(), held.as<int32_t>(), parents.as<int32_t>(), C, refs.as<int32_t>(), table2.as<int32_t>(),
+               ctx.as<int32_t>(), missing.as<int32_t>());
+    ok = ok && read(missing, 1)[0] == 0 && read(ctx, C) == std::vector<int32_t>{100, 100, 63};
+    PagedShape sh2 = sh;
+    sh2.B = C;
+    DeviceBuffer grown = ints({102, 102, 65}), one = ints({101, 101, 64});
+    resize_pages(C, P, wide, pages, table2.as<int32_t>(), refs.as<int32_t>(), ctx.as<int32_t>(), grown.as<int32_t>());
+    DeviceBuffer kd = rows((size_t)C * Hkv * T * D, 3), vd = rows((size_t)C * Hkv * T * D, 4), q = rows((size_t)C * T * Hq * D, 5);
+    append(kd, vd, T, ctx, table2, sh2);
+    const size_t nq = (size_t)C * Hq * D;
+    DeviceBuffer masks(C * T * 8), out(nq * T * 2), step(nq * 2), qs(nq * 2), ws(tree_ws_bytes(f, sh2, T));
+    const std::vector<uint64_t> chain = {1, 3, 1, 3, 1, 3};
+    masks.upload(chain.data(), chain.size() * 8);
+    TreeBufs tb;
+    tb.K = K.get(); tb.V = V.get(); tb.scK = SK.get(); tb.scV = SV.get();
+    tb.block_table = table2.as<int32_t>(); tb.ctx_lens = ctx.as<int32_t>(); tb.tree_mask = masks.as<uint64_t>();
+    tb.q = q.as<uint16_t>(); tb.out = out.as<uint16_t>(); tb.ws = ws.as<float>();
+    decode_tree(f, tb, sh2, T);
+    const int S = pick_splits_paged(f, sh2);
+    DeviceBuffer ws1(ws_bytes(C * Hq, D, S));
+    std::vector<uint16_t> hq(nq * T), got(nq * T), want(nq), part(nq);
+    check(va_sync());
+    q.download(hq.data(), hq.size() * 2);
+    out.download(got.data(), got.size() * 2);
+    PagedBufs pb;
+    pb.K = K.get(); pb.V = V.get(); pb.scK = SK.get(); pb.scV = SV.get(); pb.block_table = table2.as<int32_t>();
+    pb.q = qs.as<uint16_t>(); pb.out = step.as<uint16_t>(); pb.ws = ws1.as<float>();
+    const size_t row = (size_t)Hq * D;
+    for (int t = 0; t < T; ++t) {
+        for (int c = 0; c < C; ++c) std::copy_n(hq.begin() + (c * T + t) * row, row, part.begin() + c * row);
+        qs.upload(part.data(), nq * 2);
+        pb.seq_lens = (t ? grown : one).as<int32_t>();
+        launch_paged(f, pb, sh2, S);
+        check(va_sync());
+        step.download(want.data(), nq * 2);
+        for (int c = 0; c < C; ++c)
+            for (size_t i = 0; i < row; ++i) {
+                const double a = half_to_double(got[(c * T + t) * row + i]), b = half_to_double(want[c * row + i]);
+                const double e = std::fabs(a - b);
+                *maxerr = std::max(*maxerr, e);
+                ok = ok && e <= (std::fabs(b) + 1.0) / 1024;   // two roundings to fp16, and the weights'
+            }
+    }
+    // the second draft moves to the first one's place: a step over it sees the same rows as a tree without draft 0
+    DeviceBuffer keep = ints({1, 0, 1, 0, 1, 0}), counts = ints({1, 1, 1});
+    const std::vector<uint64_t> alone = {1, 2, 1, 2, 1, 2};
+    masks.upload(alone.data(), alone.size() * 8);
+    decode_tree(f, tb, sh2, T);
+    check(va_sync());
+    out.download(got.data(), got.size() * 2);
+    compact_kv(f, pools, sh2, table2.as<int32_t>(), ctx.as<int32_t>(), keep.as<int32_t>(), counts.as<int32_t>(), T);
+    pb.seq_lens = one.as<int32_t>();
+    launch_paged(f, pb, sh2, S);                            // qs: the second drafts' queries
+    check(va_sync());
+    step.download(want.data(), nq * 2);
+    for (int c = 0; c < C; ++c)
+        for (size_t i = 0; i < row; ++i) {
+            const double a = half_to_double(got[(c * T + 1) * row + i]), b = half_to_double(want[c * row + i]);
+            *maxerr = std::max(*maxerr, std::fabs(a - b));
+            ok = ok && std::fabs(a - b) <= (std::fabs(b) + 1.0) / 1024;
+        }
+    resize_pages(C, P, wide, pages, table2.as<int32_t>(), refs.as<int32_t>(), grown.as<int32_t>(), none.as<int32_t>());
+    ok = ok && read(refs, pages) == std::vector<int32_t>(pages, 0);
+
+    // a prompt of one row attends itself: its value
+    DeviceBuffer cu = ints({0, 1}), pq = rows((size_t)Hq * D, 6), pk = rows((size_t)Hkv * D, 7), pv = rows((size_t)Hkv * D, 8), po((size_t)Hq * D * 2);
+    PrefillShape ps{1, 1, Hq, Hkv, D, Hq * D, D, Hkv * D, D, Hkv * D, D};
+    prefill(PrefillBufs{pq.as<uint16_t>(), pk.as<uint16_t>(), pv.as<uint16_t>(), cu.as<int32_t>(), po.as<uint16_t>()}, ps);
+    std::vector<uint16_t> o((size_t)Hq * D), v((size_t)Hkv * D);
+    check(va_sync());
+    po.download(o.data(), o.size() * 2);
+    pv.download(v.data(), v.size() * 2);
+    for (int h = 0; h < Hq; ++h)
+        for (int d = 0; d < D; ++d) ok = ok && o[h * D + d] == v[(h * Hkv / Hq) * D + d];
+    return ok;
+}
+
 int selftest_ex() {
     const Fmt tiled[] = {Fmt::F16M, Fmt::Q8M, Fmt::Q4M, Fmt::Q3M};
     struct GqaCase { int Hq, Hkv, L, D, S; };
@@ -373,6 +493,14 @@ int selftest_ex() {
         }
     if (fails) { std::printf("%d of %d grouped/paged case(s) FAILED\n", fails, n); return 1; }
     std::printf("all %d grouped/paged cases passed\n", n);
+    for (Fmt f : tiled) {
+        double maxerr = 0.0;
+        const bool ok = serving_case(f, 64, &maxerr);
+        std::printf("serve  %-4s Hq=8  Hkv=2  lens=100,63 G=64  maxerr=%.2e  %s\n", fmt_name(f), maxerr, ok ? "PASS" : "FAIL");
+        fails += !ok;
+    }
+    if (fails) { std::printf("%d serving case(s) FAILED\n", fails); return 1; }
+    std::printf("all serving cases passed\n");
     return 0;
 }
 

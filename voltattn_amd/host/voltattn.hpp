@@ -11,8 +11,9 @@
 //   voltattn::dequantize  device dq() over whole rows (src/voltattn.cu:747-767)
 //
 // Beyond the reference (its README.md:205-206 lists GQA and paged KV as
-// missing): launch_gqa, launch_paged, append_kv, and the Stream / Graph
-// helpers for replaying captured decode steps.
+// missing): launch_gqa, launch_paged, append_kv, prefill, decode_tree,
+// compact_kv, fork_pages, resize_pages, and the Stream / Graph helpers for
+// replaying captured decode steps.
 //
 // Errors throw voltattn::Error (status code + message), where the reference
 // exits through CUDA_CHECK (src/voltattn.cu:49-58).
@@ -211,6 +212,61 @@ inline size_t page_scale_bytes(Fmt f, int Hkv, int page_rows, int D, int G = 64)
 inline void append_kv(Fmt f, const uint16_t* x, int n, const int32_t* start, const int32_t* block_table,
                       const PagedShape& shape, void* pages, uint16_t* scales, void* stream = nullptr) {
     check(va_append_kv(static_cast<va_fmt>(f), x, n, start, block_table, &shape, pages, scales, stream));
+}
+
+// Causal attention of packed prompts (va_prefill_shape documents the layout).
+using PrefillShape = va_prefill_shape;
+using PrefillBufs = va_prefill_bufs;
+
+inline void prefill(const PrefillBufs& b, const PrefillShape& shape, void* stream = nullptr) {
+    check(va_prefill(&b, &shape, stream));
+}
+
+// Attention of drafted tokens over a paged cache.
+struct TreeBufs {
+    void*           K           = nullptr;  // K page pool
+    void*           V           = nullptr;  // V page pool
+    void*           scK         = nullptr;  // K scale pool (quantized formats)
+    void*           scV         = nullptr;  // V scale pool
+    const int32_t*  block_table = nullptr;  // [B][max_pages]
+    const int32_t*  ctx_lens    = nullptr;  // [B]
+    const int32_t*  tree_sizes  = nullptr;  // [B], null: T each
+    const uint64_t* tree_mask   = nullptr;  // [B][T]
+    uint16_t*       q           = nullptr;  // [B][T][Hq][D]
+    uint16_t*       out         = nullptr;  // [B][T][Hq][D]
+    float*          ws          = nullptr;  // tree_ws_bytes
+};
+
+inline va_tree_bufs to_c(const TreeBufs& b) {
+    return va_tree_bufs{b.K, b.V, static_cast<const uint16_t*>(b.scK), static_cast<const uint16_t*>(b.scV),
+                        b.block_table, b.ctx_lens, b.tree_sizes, b.tree_mask, b.q, b.out, b.ws};
+}
+
+inline void decode_tree(Fmt f, const TreeBufs& b, const PagedShape& shape, int T, void* stream = nullptr) {
+    const va_tree_bufs cb = to_c(b);
+    check(va_decode_tree(static_cast<va_fmt>(f), &cb, &shape, T, stream));
+}
+inline size_t tree_ws_bytes(Fmt f, const PagedShape& shape, int T) {
+    return va_tree_ws_bytes(static_cast<va_fmt>(f), &shape, T);
+}
+
+// The page pools of a cache, and what moves their rows and pages (voltattn.h).
+using Pools = va_pools;
+
+inline void compact_kv(Fmt f, const Pools& pools, const PagedShape& shape, const int32_t* block_table,
+                       const int32_t* base, const int32_t* keep, const int32_t* counts, int n, void* stream = nullptr) {
+    check(va_compact_kv(static_cast<va_fmt>(f), &pools, &shape, block_table, base, keep, counts, n, stream));
+}
+inline void fork_pages(Fmt f, const Pools& pools, const PagedShape& shape, const int32_t* block_table,
+                       const int32_t* seq_lens, const int32_t* parents, int children, int32_t* refs, int32_t* new_table,
+                       int32_t* new_lens, int32_t* missing = nullptr, void* stream = nullptr) {
+    check(va_fork_pages(static_cast<va_fmt>(f), &pools, &shape, block_table, seq_lens, parents, children, refs,
+                        new_table, new_lens, missing, stream));
+}
+inline void resize_pages(int B, int page_rows, int max_pages, int num_pages, int32_t* block_table, int32_t* refs,
+                         const int32_t* old_lens, const int32_t* new_lens, int32_t* missing = nullptr,
+                         void* stream = nullptr) {
+    check(va_resize_pages(B, page_rows, max_pages, num_pages, block_table, refs, old_lens, new_lens, missing, stream));
 }
 
 // Device quantize() of fp32 rows [rows][D] into packed codes and fp16 scales.
