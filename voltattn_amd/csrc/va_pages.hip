@@ -306,7 +306,9 @@ hipError_t launch_compact(const PageArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// One launch plans a small batch; a large one's rows are dealt over the device first.
+// One launch plans a small batch; a large one's rows are dealt over the device first. Sixteen
+// sequences forked into sixteen: 7.6 us with one planning launch, 7.7 with two; a single group's
+// time grows with the table, and its LDS holds up to PLAN_ONE.
 static bool plan_in_one(const PageArgs& a, int rows) { return rows <= PLAN_ONE && (long long)rows * a.max_pages <= 1 << 15; }
 
 hipError_t launch_resize(const PageArgs& a, hipStream_t stream) {

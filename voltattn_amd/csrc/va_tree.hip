@@ -31,7 +31,10 @@ TreeForm tree_form(int kind, int D, int B, int hkv, int rows, int cap, int cus) 
 template <int KIND, int D, int G>
 static hipError_t launch(const TreeArgs& a, hipStream_t stream) {
     const dim3 grid((unsigned)(a.nwg + 7) / 8 * 8), block(256);
-    const bool few = (long long)a.B * a.T * a.hkv * a.group <= 8192;   // 32 to a work-group would leave CUs idle
+    // rows to a merging work-group, and waves to a row's pieces: 32 and 1, or 8 and 4 where the former
+    // would leave CUs idle (512 rows: 19.5 us the whole call with the former, 17.5 with the latter;
+    // 16384 rows 65.0 : 66.2 us)
+    const bool few = (long long)a.B * a.T * a.hkv * a.group <= 8192;
     const int mr = few ? 8 : 32;
     const dim3 mgrid((unsigned)((size_t)a.B * a.hkv * ((a.T * a.group + mr - 1) / mr)));
     hipError_t e;

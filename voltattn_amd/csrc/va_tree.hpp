@@ -9,20 +9,32 @@
 // the columns of va_wide.hpp's tiles.
 //
 // Work-group: 4 waves, QW of them side by side over the query rows (BM = 32 QW) and
-// KW = 4/QW over the K/V rows of a tile of BN. A tile is fetched into registers while
-// its predecessor is computed, unpacked into LDS as exact fp16 codes (one unpack for all
-// query rows) and its group scales beside it; K's scales are applied to each group's part
-// of the dot product in fp32, V's to the weights: p * s is rounded once, to fp16 (RNE),
-// an independent error of 2^-12 of each weight, and the output's own rounding to fp16 is
-// as large. fp16 holds p * s from 2^-24 to 65504: the lazy maximum lets p grow to 2^SLACK
-// and starts it at 2^OFF, so that no scale of a cache made from fp16 values (|v| <= 65504)
-// overflows and weights far below the largest one keep their digits.
+// KW = 4/QW over the K/V rows of a tile of BN. The sums are fp32, the weights are rounded
+// to fp16 (RNE) for the second product, an independent error of 2^-12 of each weight, so
+// that of the output stays below its own rounding to fp16. Scales, by the row block:
+//   QW <= 2: a tile is fetched into registers while its predecessor is computed, unpacked
+//     into LDS as exact fp16 codes and its group scales beside it; K's scales are applied to
+//     each group's part of the dot product in fp32, V's to the weights (p * s is what is
+//     rounded). The range of fp16 holds p * s: see WeightRange.
+//   QW = 4: 128 rows share one unpacking, so the scales are applied there, which leaves the
+//     waves' loop as it is for fp16 rows: K becomes two fp16 terms whose sum is code * scale
+//     exactly (twice the products of S, but no scaling of 128 x 64 scores per group), V is
+//     rounded to fp16, an error of 2^-12 of each value. Both are halved, so that code * scale
+//     up to 131008 fits. fp16 rows go straight to LDS (wide_walk).
+// Measured (MI355X, D = 128): 24 x 32 drafts over up to 16384 positions q4 137 us (388 TFLOP/s
+// of the two products; unpacking and K's second term bound it, the pieces' 11 us of joining
+// next), 4 x 64 drafts over up to 8003 positions f16, 8 query heads to a K/V head, 65 us
+// (467 TFLOP/s), one sequence's 16 drafts over 4096 positions q8 17.6 us (latency: a launch
+// of two kernels, 2 tiles of work to a CU).
 //
 // Work split: the tiles of all (sequence, K/V head, row block), numbered one behind the
 // other, are cut into equal shares, one to a work-group. A row block inside one share is
 // finished there; the pieces of one that several shares cut go to ws (slot 2w: the
 // piece that work-group w begins with, 2w + 1: the one it ends with) and tree_merge
 // joins them.
+//
+// Tiles with drafts, or rows behind the sequence, are masked: see wide_clean for V's infinite
+// and NaN values there.
 #pragma once
 #include "va_kernels.hpp"
 #include "va_wide.hpp"
@@ -671,7 +683,8 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
     } while (at < end);
 }
 
-// Joins the pieces of the row blocks that several shares cut, and fills the rows that no
+// Joins the pieces of the row blocks that several shares cut (bound by reading them: 66 KB for each
+// 128 rows; 11 us for the 24 x 32 drafts above), and fills the rows that no
 // work-group has: zeros for drafts behind a sequence's last one and for sequences of
 // length 0, NaN for sequences whose lengths are out of range. A work-group has 32/PW rows of
 // one (sequence, K/V head), eight lanes to a row with D/8 columns each; PW of its waves

@@ -209,8 +209,9 @@ template <int N> __device__ __forceinline__ void wait_loads() {
 }
 
 // A tile of WIDE_BN fp16 rows (row_bytes apart; uniform) on its way to LDS, a quarter by each wave
-// of a 4-wave group, 16 bytes per lane and load, zeros from out of range. Load i of a wave covers rows (wave N + i) ROWS + lane / (D/8); its lanes fetch the chunks that swz()
-// puts in their places, which are those of load 0 with another XOR.
+// of a 4-wave group, 16 bytes per lane and load, zeros from out of range. Load i of a wave covers
+// rows (wave N + i) ROWS + lane / (D/8); its lanes fetch the chunks that swz() puts in their
+// places, which are those of load 0 with another XOR.
 constexpr int WIDE_BN = 64;
 template <int D> struct WideFetch {
     static constexpr int TILE = WIDE_BN * 2 * D, N = TILE / 1024 / 4, ROWS = 1024 / (2 * D);
