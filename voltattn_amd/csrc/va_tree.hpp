@@ -23,8 +23,8 @@
 //     up to 131008 fits. fp16 rows go straight to LDS (wide_walk).
 // Measured (MI355X, D = 128): 24 x 32 drafts over up to 16384 positions q4 137 us (388 TFLOP/s
 // of the two products; unpacking and K's second term bound it, the pieces' 11 us of joining
-// next), 4 x 64 drafts over up to 8003 positions f16, 8 query heads to a K/V head, 65 us
-// (467 TFLOP/s), one sequence's 16 drafts over 4096 positions q8 17.6 us (latency: a launch
+// next), 4 x 64 drafts over up to 8003 positions f16, 8 query heads to a K/V head, 62.5 us
+// (485 TFLOP/s), one sequence's 16 drafts over 4096 positions q8 17.6 us (latency: a launch
 // of two kernels, 2 tiles of work to a CU).
 //
 // Work split: the tiles of all (sequence, K/V head, row block), numbered one behind the
@@ -229,7 +229,6 @@ __device__ __forceinline__ f32x4 tree_odd(const uint8_t* v, const uint16_t* sv, 
     return x;
 }
 
-constexpr int PART_AUX = 16;       // written through the L2s (sc1)
 // Work-groups that fit a CU (waves to a SIMD): their registers decide.
 constexpr int tree_waves(int kind, int D, int qw) { return qw < 4 ? 2 : D == 128 || kind == KF16 ? 3 : 4; }
 template <int QW> struct TreeTile {
@@ -609,8 +608,11 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
         // sequence, 16 drafts over 4096 positions q8, 26.4 us with it).
         const bool whole = t0 == 0 && t1 == sq.tiles;
         const int slot = 2 * wg + (t0 == 0 ? 1 : 0);
-        // [BM][D] sums, then [BM][2] (m, l); written through to memory: what is dirty in the L2s is
-        // written back when the kernel ends, at a fraction of the rate
+        // [BM][D] sums, then [BM][2] (m, l). Of few rows they are written through to memory (sc1): what is
+        // dirty in the L2s is written back when the kernel ends, which nothing covers there (one
+        // sequence's 64 rows 17.5 us, 18.0 through the L2s). The widest blocks' pieces, begun and ended
+        // at different times, go through the L2s (4 x 512 rows f16 62.5 us, 65.0 written through).
+        constexpr int PART_AUX = QW == 4 ? 0 : 16;
         const __amdgpu_buffer_rsrc_t part = make_rsrc(a.ws + (size_t)uniform(slot) * BM * (D + 2), BM * (D + 2) * 4);
         __attribute__((address_space(3))) float* es = (__attribute__((address_space(3))) float*)lds;
         __attribute__((address_space(3))) float* ml = es + EPI / 4;     // [wave][32][2]
