@@ -209,7 +209,10 @@ template <int N> __device__ __forceinline__ void wait_loads() {
 }
 
 // A tile of WIDE_BN fp16 rows (row_bytes apart; uniform) on its way to LDS, a quarter by each wave
-// of a 4-wave group, 16 bytes per lane and load, zeros from out of range. Load i of a wave covers
+// of a 4-wave group, 16 bytes per lane and load, zeros from out of range: the whole offset is in the
+// vector operand, which the descriptor's range check covers by its documentation. (With the rows in
+// the scalar operand a short tile relies on a check of the sum, which MI355X makes; no slower so:
+// one prompt of 16384 tokens 2.06 ms with either.) Load i of a wave covers
 // rows (wave N + i) ROWS + lane / (D/8); its lanes fetch the chunks that swz() puts in their
 // places, which are those of load 0 with another XOR.
 constexpr int WIDE_BN = 64;
@@ -225,8 +228,8 @@ template <int D> struct WideFetch {
     __device__ __forceinline__ void operator()(__amdgpu_buffer_rsrc_t r, lds_u8* to) const {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + (wave * N + i) * 1024, 16, at + (chunk ^ (uint32_t)((D == 128 ? i : 2 * i) << 4)),
-                                                     (uint32_t)(i * ROWS) * row_bytes, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + (wave * N + i) * 1024, 16,
+                                                     at + (uint32_t)(i * ROWS) * row_bytes + (chunk ^ (uint32_t)((D == 128 ? i : 2 * i) << 4)), 0, 0, 0);
     }
 };
 
