@@ -383,11 +383,12 @@ typedef struct {
  * sequence with ctx + size above max_seq_len, or a length or size out of range,
  * gives NaN for all T drafts; a page id outside the pool on one of its positions
  * NaN for its drafts. NaN and infinities in a draft's rows reach the drafts that
- * attend it only. Quantized formats: caches made from fp16 values are in range;
- * V values whose scale exceeds 1023 (q8), 16383 (q4) or 32767 (q3) may overflow
- * to infinities, and where a K/V head has more than 64 query rows (T * Hq / Hkv)
- * so may K or V values above 131008; there V's values are rounded to fp16. The
- * tiled formats only. The last bits of a sequence's sums depend on the
+ * attend it only. Quantized formats: caches made from fp16 values are in range.
+ * Where a K/V head has more than 64 query rows (T * Hq / Hkv) and the batch over
+ * four K/V tiles of 64 positions (max_seq_len, per K/V head and 128 query rows)
+ * for each CU, V's values are rounded to fp16 (2^-11 of each), and K or V values
+ * above 131008 may overflow to infinities; elsewhere code times scale is not
+ * rounded by itself. The tiled formats only. The last bits of a sequence's sums depend on the
  * lengths of the whole batch; the same batch gives the same bits. Asynchronous
  * on `stream`; concurrent calls need distinct ws. */
 #define VA_TREE_MAX 64

@@ -10,12 +10,13 @@
 //
 // Work-group: 4 waves, QW of them side by side over the query rows (BM = 32 QW) and
 // KW = 4/QW over the K/V rows of a tile of BN. The sums are fp32, the weights are rounded
-// to fp16 (RNE) for the second product, an independent error of 2^-12 of each weight, so
-// that of the output stays below its own rounding to fp16. Scales, by the row block:
+// to fp16 (RNE) for the second product, each off by at most 2^-11 of itself (see WeightRange for
+// small ones), independently of each other, so that the output's error is mostly its own rounding
+// to fp16. Scales, by the row block:
 //   QW <= 2: a tile is fetched into registers while its predecessor is computed, unpacked
 //     into LDS as exact fp16 codes and its group scales beside it; K's scales are applied to
 //     each group's part of the dot product in fp32, V's to the weights (p * s is what is
-//     rounded). The range of fp16 holds p * s: see WeightRange.
+//     rounded, relative to the largest scale so far: see WeightRange).
 //   QW = 4: 128 rows share one unpacking, so the scales are applied there, which leaves the
 //     waves' loop as it is for fp16 rows: K becomes two fp16 terms whose sum is code * scale
 //     exactly (twice the products of S, but no scaling of 128 x 64 scores per group), V is
@@ -114,14 +115,13 @@ template <int AUX> __device__ __forceinline__ u32x3 load96(__amdgpu_buffer_rsrc_
     return __builtin_amdgcn_raw_buffer_load_b96(r, off, 0, AUX);
 }
 
-// p and p * scale stay within fp16: the weights start at 2^OFF and may grow by 2^SLACK
-// before the maximum follows. A scale of a cache of fp16 values is at most 65504/127 (q8),
-// 65504/7 (q4), 65504/3 (q3).
-template <int KIND> struct WeightRange;
-template <> struct WeightRange<KF16> { static constexpr float off = WIDE_OFF, slack = WIDE_SLACK; };
-template <> struct WeightRange<KQ8>  { static constexpr float off = 3.f, slack = 3.f; };
-template <> struct WeightRange<KQ4>  { static constexpr float off = 0.f, slack = 2.f; };
-template <> struct WeightRange<KQ3>  { static constexpr float off = 0.f, slack = 1.f; };
+// The range of the weights' operand: the largest weight is held as 2^off at least and may grow
+// by 2^slack before the maximum follows. SCALED: times V's group scale over a power of two
+// 2^ve above every scale so far (see scale_top), so that the operand stays below 2^15 for any
+// finite scale, and a product of weight and scale keeps fp16's 11 bits down to 2^-26 of the
+// largest weight times the largest scale.
+template <bool SCALED> struct WeightRange { static constexpr float off = WIDE_OFF, slack = WIDE_SLACK; };
+template <> struct WeightRange<true> { static constexpr float off = 12.f, slack = 3.f; };
 
 __device__ __forceinline__ f16x4 lds_scales(const lds_u8* p, uint32_t at) {
     return *reinterpret_cast<const __attribute__((address_space(3))) f16x4*>(p + at);
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
     // its turn: three work-groups fit a CU without its registers and cover each other's waits
     constexpr bool AHEAD = QW != 4;
     constexpr int AUX = QW == 4 ? 0 : VA_LOAD_AUX;      // the row blocks of a K/V head read the same rows
-    using WR = WeightRange<SCALED ? KIND : KF16>;
+    using WR = WeightRange<SCALED>;
     constexpr int GP = QW == 1 ? 1 : NG > 2 ? 2 : NG, VP = GP;   // scale groups that are in registers at once
     constexpr int HALVES = BN / 64;                         // a page holds at least 64 rows
     constexpr int RSRCS = 256 / UPR > 64 ? 1 : HALVES;      // halves that a wave fetches from
@@ -263,8 +263,9 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
     constexpr int ES = 68;                                  // epilogue: 64 columns of a row, the next four banks on
     constexpr int EPI = 4 * 32 * ES * 4;
     constexpr int LDS = TILES > EPI + 1024 ? TILES : EPI + 1024;
-    __shared__ __align__(1024) uint8_t lds[LDS + 4];
+    __shared__ __align__(1024) uint8_t lds[LDS + 16];
     lds_int* odd = (lds_int*)((lds_u8*)lds + LDS);          // infinite or NaN values were left out
+    lds_int* scale_top = odd + 1;                           // SCALED: the largest of V's scales in each half of the tile
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     // the thread's number, made anew: what is computed from it is not held across loops
@@ -425,11 +426,19 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                 const int r = tid & 127;
                 if (r < BN) {
                     lds_u8* s = tid < 128 ? skt : svt;
-                    if (clean && tid >= 128) {              // odd values of V are those of its scales
+                    if (tid >= 128) {
                         u32x4 y = {scr[0], scr[1], 0u, 0u};
-                        any = wide_clean(y);
-                        scr[0] = y.x;
-                        scr[1] = y.y;
+                        const bool odds = wide_clean(y);
+                        if (clean) {                        // odd values of V are those of its scales
+                            any = odds;
+                            scr[0] = y.x;
+                            scr[1] = y.y;
+                        }
+                        int top = 0;                        // as bits, which order like the values
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) top = max(top, (int)(y[g / 2] >> (16 * (g & 1)) & 0x7FFFu));
+                        top = wave_scan_max(top);
+                        if ((tid & 63) == 63) scale_top[(tid >> 6) & 1] = top;
                     }
 #pragma unroll
                     for (int g = 0; g < NG; ++g)
@@ -446,7 +455,8 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
             if constexpr (QW == 2) __builtin_amdgcn_sched_barrier(0);
         };
         f32x16 o[DB] = {};
-        float m = -__builtin_inff(), l = 0.f;               // m: raw scores; p = exp2((s - m) qscale + OFF)
+        float m = -__builtin_inff(), l = 0.f;               // m: raw scores; p = exp2((s - m) qscale + OFF - ve)
+        int ve = -24;                                       // SCALED: V's scales so far are below 2^ve; else unused
         if constexpr (AHEAD) fetch(t0);
         const uint64_t mask = sq.n < 64 ? bits & ((1ull << sq.n) - 1) : bits;
         // takes the positions from j on that a row does not see out of a block of scores
@@ -508,6 +518,16 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
             stage(t);
             if (t + 1 < t1) fetch(t + 1);
             __syncthreads();
+            float grown = 1.f;                              // 2^-(what ve grows by)
+            if constexpr (SCALED) {
+                static_assert(KB == 1, "one rescale per tile");
+                const float top = h2f((uint32_t)uniform(HALVES == 2 ? max(scale_top[0], scale_top[1]) : scale_top[0]));
+                const int to = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 126;   // top < 2^to
+                if (to > ve) {
+                    grown = __builtin_bit_cast(float, (uint32_t)(127 + ve - to) << 23);
+                    ve = to;
+                }
+            }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 const int j = t * BN + (kw * KB + kb) * 32;
@@ -564,15 +584,15 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
 #pragma unroll
                 for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
                 top = halves_max(top);
-                if (__any((top - m) * qs > WR::slack)) {   // also the first one: m = -inf
+                if (grown < 1.f || __any((top - m) * qs > WR::slack)) {   // also the first one: m = -inf
                     const float to = fmaxf(m, top);
-                    const float f = to == m ? 1.f : fast_exp2((m - to) * qs);
+                    const float f = (to == m ? 1.f : fast_exp2((m - to) * qs)) * grown;
                     m = to;
                     l *= f;
 #pragma unroll
                     for (int db = 0; db < DB; ++db) o[db] *= f;
                 }
-                const float base = m == -__builtin_inff() ? 0.f : m * qs - WR::off;
+                const float base = m == -__builtin_inff() ? 0.f : m * qs - WR::off + (SCALED ? (float)ve : 0.f);
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     s[v] = fast_exp2(__builtin_fmaf(s[v], qs, -base));
@@ -659,6 +679,11 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                 const int to = rb * BM + r;
                 if (to >= rows) continue;
                 if (EXACT2) x *= 2.f;
+                if (SCALED) {                           // out of the units of 2^ve
+                    const float f = __builtin_bit_cast(float, (uint32_t)(127 + ve) << 23);
+                    ll *= f;
+                    x *= f;
+                }
                 if (*odd) {                             // what was left out, to the rows that see it
                     const int nd = to / a.group;
                     const uint64_t bits = a.mask[(size_t)b * a.T + nd];
