@@ -1,7 +1,7 @@
 """GPU: attention whose output comes from weights far below the largest one and from small
 values (a sink: one position that takes most of the weight and has next to no value), by
-the tree kernel in every tiled format. The bound is the
-operator's (attn_bound.py), and none that an output of zeros would meet."""
+the tree kernel in every tiled format and row block. The bound is
+the operator's (attn_bound.py), and none that an output of zeros would meet."""
 import pytest
 import torch
 
@@ -74,15 +74,15 @@ def _tree(fmt, form, n, nats, spread, vmag, D=128, G=32, seed=0, sink=0.01):
         attn_bound.check(got[:, h], *attn_bound.attend(q[0, :, h], kx[:, h // group], vx[:, h // group], seen, rounded), h)
 
 
-@pytest.mark.parametrize("vmag", [1.0, 0.02, 0.005])
-@pytest.mark.parametrize("form", [32, 64])
+@pytest.mark.parametrize("vmag", [1.0, 0.02, 0.005, 0.0005])
+@pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("fmt", list(BITS))
 def test_tree_with_a_sink(fmt, form, vmag):
     _tree(fmt, form, 16384, 12.0, 1.0, vmag)
 
 
 @pytest.mark.parametrize("nats", [6.0, 16.0])
-@pytest.mark.parametrize("form", [32, 64])
+@pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("fmt", list(BITS))
 def test_tree_with_a_sink_over_equal_scores(fmt, form, nats):
     """Equal weights round alike: nothing averages out."""

@@ -19,9 +19,10 @@
 //     rounded, relative to the largest scale so far: see WeightRange).
 //   QW = 4: 128 rows share one unpacking, so the scales are applied there, which leaves the
 //     waves' loop as it is for fp16 rows: K becomes two fp16 terms whose sum is code * scale
-//     exactly (twice the products of S, but no scaling of 128 x 64 scores per group), V is
-//     rounded to fp16, an error of 2^-12 of each value. Both are halved, so that code * scale
-//     up to 131008 fits. fp16 rows go straight to LDS (wide_walk).
+//     to 22 bits (twice the products of S, but no scaling of 128 x 64 scores per group), V is
+//     rounded to fp16, each value off by at most 2^-11 of itself. Both are halved, in the codes,
+//     where it is exact, so that code * scale up to 131008 fits; what is below fp16's normal numbers
+//     there is off by 2^-24 at most. fp16 rows go straight to LDS (wide_walk).
 // Measured (MI355X, D = 128): 24 x 32 drafts over up to 16384 positions q4 137 us (388 TFLOP/s
 // of the two products; unpacking and K's second term bound it, the pieces' 11 us of joining
 // next), 4 x 64 drafts over up to 8003 positions f16, 8 query heads to a K/V head, 62.5 us
@@ -55,14 +56,17 @@ __device__ __forceinline__ f16x2 as_f16x2(uint32_t x) { return __builtin_bit_cas
 __device__ __forceinline__ f16x8 join4(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
     return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
-// Four codes, one to a byte of w, as fp16 pairs 1024 + n, less `bias`: exact.
-__device__ __forceinline__ void bytes_to_f16(uint32_t w, _Float16 bias, f16x2& a, f16x2& b) {
-    const f16x2 z = {bias, bias};
-    a = as_f16x2(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - z;
-    b = as_f16x2(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - z;
+// Four codes, one to a byte of w, as fp16 pairs 1024 + n, less 1024 + bias (HALF: half of that, 512 +
+// n/2, less 512 + bias/2): exact.
+template <bool HALF> __device__ __forceinline__ void bytes_to_f16(uint32_t w, float bias, f16x2& a, f16x2& b) {
+    const _Float16 x = (_Float16)((1024.f + bias) * (HALF ? 0.5f : 1.f));
+    const f16x2 z = {x, x};
+    constexpr uint32_t HIGH = HALF ? 0x60606060u : 0x64646464u;
+    a = as_f16x2(__builtin_amdgcn_perm(HIGH, w, 0x04010400u)) - z;
+    b = as_f16x2(__builtin_amdgcn_perm(HIGH, w, 0x04030402u)) - z;
 }
-// A unit's values in order, as exact fp16 codes (f16: the values).
-template <int KIND>
+// A unit's values in order, as exact fp16 codes, or halves of codes (f16: the values).
+template <int KIND, bool HALF>
 __device__ __forceinline__ void unpack_unit(const Words<Unit<KIND>::W>& u, f16x8 (&out)[Unit<KIND>::UE / 8]) {
     if constexpr (KIND == KF16) {
         out[0] = __builtin_bit_cast(f16x8, u32x4{u.w[0], u.w[1], u.w[2], u.w[3]});
@@ -70,20 +74,21 @@ __device__ __forceinline__ void unpack_unit(const Words<Unit<KIND>::W>& u, f16x8
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             f16x2 a, b, c, d;
-            bytes_to_f16(u.w[2 * i] ^ 0x80808080u, (_Float16)1152.f, a, b);
-            bytes_to_f16(u.w[2 * i + 1] ^ 0x80808080u, (_Float16)1152.f, c, d);
+            bytes_to_f16<HALF>(u.w[2 * i] ^ 0x80808080u, 128.f, a, b);
+            bytes_to_f16<HALF>(u.w[2 * i + 1] ^ 0x80808080u, 128.f, c, d);
             out[i] = join4(a, b, c, d);
         }
     } else if constexpr (KIND == KQ4) {
-        const f16x2 lo = {(_Float16)1032.f, (_Float16)1032.f}, hi = {(_Float16)72.f, (_Float16)72.f};
-        const f16x2 r16 = {(_Float16)0.0625f, (_Float16)0.0625f};
+        constexpr float H = HALF ? 0.5f : 1.f;
+        constexpr uint32_t LOW = HALF ? 0x60006000u : 0x64006400u;   // 512 + n/2, or 1024 + n
+        const f16x2 lo = f16x2((_Float16)(1032.f * H)), hi = f16x2((_Float16)(72.f * H)), r16 = f16x2((_Float16)(0.0625f * H));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t w = u.w[i], x = w >> 8;
             // nibbles (0,4), (1,5), (2,6), (3,7): n - 8, the upper ones from 1024 + 16n
-            const uint32_t p04 = __builtin_bit_cast(uint32_t, as_f16x2((w & 0x000F000Fu) | 0x64006400u) - lo);
+            const uint32_t p04 = __builtin_bit_cast(uint32_t, as_f16x2((w & 0x000F000Fu) | LOW) - lo);
             const uint32_t p15 = __builtin_bit_cast(uint32_t, as_f16x2((w & 0x00F000F0u) | 0x64006400u) * r16 - hi);
-            const uint32_t p26 = __builtin_bit_cast(uint32_t, as_f16x2((x & 0x000F000Fu) | 0x64006400u) - lo);
+            const uint32_t p26 = __builtin_bit_cast(uint32_t, as_f16x2((x & 0x000F000Fu) | LOW) - lo);
             const uint32_t p37 = __builtin_bit_cast(uint32_t, as_f16x2((x & 0x00F000F0u) | 0x64006400u) * r16 - hi);
             out[i] = __builtin_bit_cast(f16x8, u32x4{__builtin_amdgcn_perm(p15, p04, 0x05040100u), __builtin_amdgcn_perm(p37, p26, 0x05040100u),
                                                      __builtin_amdgcn_perm(p15, p04, 0x07060302u), __builtin_amdgcn_perm(p37, p26, 0x07060302u)});
@@ -101,8 +106,8 @@ __device__ __forceinline__ void unpack_unit(const Words<Unit<KIND>::W>& u, f16x8
                 c[j] = (t | (t << 5)) & 0x07070707u;        // one code to a byte
             }
             f16x2 a, b, d, e;
-            bytes_to_f16(c[0], (_Float16)1028.f, a, b);
-            bytes_to_f16(c[1], (_Float16)1028.f, d, e);
+            bytes_to_f16<HALF>(c[0], 4.f, a, b);
+            bytes_to_f16<HALF>(c[1], 4.f, d, e);
             out[i] = join4(a, b, d, e);
         }
     }
@@ -222,7 +227,7 @@ __device__ __forceinline__ f32x4 tree_odd(const uint8_t* v, const uint16_t* sv, 
                 n = (int)(((uint32_t)p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16) >> (3 * (d & 7)) & 7u) - 4;
             }
             const _Float16 s = __builtin_bit_cast(_Float16, sv[r * (D / G) + d / G]);
-            if constexpr (EXACT2) x[e] = wide_odd((float)((_Float16)(float)n * (s * (_Float16)0.5f)));
+            if constexpr (EXACT2) x[e] = wide_odd((float)((_Float16)(0.5f * (float)n) * s));
             else x[e] = wide_odd((float)s) == 0.f ? 0.f : (float)n * (float)s;
         }
     }
@@ -393,8 +398,8 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                 const int u = i * 256 + tid, r = u / UPR, c = (u % UPR) * (Unit<KIND>::UE / 8);
                 if (UNITS % 256 == 0 || u < UNITS) {
                     f16x8 x[Unit<KIND>::UE / 8];
-                    unpack_unit<KIND>(kr[i], x);
-                    const f16x8 ks = EXACT2 ? f16x8(__builtin_bit_cast(_Float16, (uint16_t)ksu[i])) * (_Float16)0.5f : f16x8{};
+                    unpack_unit<KIND, EXACT2>(kr[i], x);
+                    const f16x8 ks = EXACT2 ? f16x8(__builtin_bit_cast(_Float16, (uint16_t)ksu[i])) : f16x8{};
 #pragma unroll
                     for (int e = 0; e < Unit<KIND>::UE / 8; ++e) {
                         const int to = r * 2 * D + (((c + e) ^ swz<D>(r)) << 4);
@@ -406,8 +411,8 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                         *reinterpret_cast<lds_f16x8*>(kt + to) = x[e];
                     }
                     if (!AHEAD) __builtin_amdgcn_sched_barrier(0);   // one operand's values in registers at a time
-                    unpack_unit<KIND>(vr[i], x);
-                    const f16x8 vs = EXACT2 ? f16x8(__builtin_bit_cast(_Float16, (uint16_t)vsu[i])) * (_Float16)0.5f : f16x8{};
+                    unpack_unit<KIND, EXACT2>(vr[i], x);
+                    const f16x8 vs = EXACT2 ? f16x8(__builtin_bit_cast(_Float16, (uint16_t)vsu[i])) : f16x8{};
 #pragma unroll
                     for (int e = 0; e < Unit<KIND>::UE / 8; ++e) {
                         const int to = r * 2 * D + (((c + e) ^ swz<D>(r)) << 4);
