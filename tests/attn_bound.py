@@ -8,9 +8,10 @@ fp16 result may be off, each rounding by at most half a step of its type:
   most sum|q k|/sqrt(D); a weight by that share twice (its own score's and the maximum's),
   and by 2^-22 for exp2;
 * a weight (times its value's group scale, relative to the largest scale): 2^-11 of itself as a
-  normal fp16 number. The largest weight is held as at least 2^12 and the largest scale as at
-  least 1/2, so that fp16's last step, 2^-24, half of it rounded away, is at most 2^-36 of
-  the largest weight (1) times the largest value, for each of n positions;
+  normal fp16 number. Below that, half of fp16's last step, 2^-25, is rounded away at most, for each of n
+  positions: of weights whose largest one is held as at least 2^10, 2^-35 of it (1) times the
+  value; of weights times scales, the largest of which are held as at least 2^12 and 1/2, 2^-36 of
+  the largest weight times the largest value;
 * values of quantized rows rounded to fp16 at half their size (v_rounded): 2^-11 of each, or
   2 * 2^-25 where fp16 has no finer step;
 * the sums over n positions in fp32: 2^-24 of sum p|v| for each addition;
@@ -37,7 +38,7 @@ def attend(q, k, v, seen=None, v_rounded=False):
     out, size = w @ v / total, w @ v.abs() / total
     e_score = 2 * (D + 4) * 2.0 ** -24 * raw.amax(-1, keepdim=True) + 2.0 ** -22
     rel = 2.0 ** -11 * (2 if v_rounded else 1) + 2.0 ** -24 * (n + 64) + e_score
-    low = n * 2.0 ** -36 * v.abs().max() / total
+    low = n * 2.0 ** -35 * v.abs().max() / total
     return out, rel * size + low + 2.0 ** -11 * out.abs() + 2.0 ** -25 + (2.0 ** -24 if v_rounded else 0.0)
 
 

@@ -1,7 +1,7 @@
 """GPU: attention whose output comes from weights far below the largest one and from small
 values (a sink: one position that takes most of the weight and has next to no value), by
-the tree kernel in every tiled format and row block. The bound is
-the operator's (attn_bound.py), and none that an output of zeros would meet."""
+the prompt kernel and by the tree kernel in every tiled format and row block. The bound is the
+operator's (attn_bound.py), and none that an output of zeros would meet."""
 import pytest
 import torch
 
@@ -113,3 +113,15 @@ def test_tree_over_values_of_very_different_size(fmt, form):
         seen = torch.cat([torch.ones((T, n), dtype=torch.bool, device="cuda"), torch.eye(T, dtype=torch.bool, device="cuda")], 1)
         for h in range(heads * group):
             attn_bound.check(got[:, h], *attn_bound.attend(q[0, :, h], kx[:, h // group], vx[:, h // group], seen), (sign, h))
+
+
+@pytest.mark.parametrize("nats,spread", [(6.0, 0.0), (16.0, 0.0), (12.0, 1.0)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_with_a_sink(D, nats, spread):
+    n, heads = 4097, 2
+    q, k, v = _draws(n, heads, D, nats, spread, 1.0, 4, (n, heads), 0.0)
+    got = ops.prefill(q, k, v, _int([0, n]))
+    rows = torch.arange(1024, n, 96, device="cuda")         # rows with a tail in their outputs
+    seen = torch.arange(n, device="cuda")[None] <= rows[:, None]
+    for h in range(heads):
+        attn_bound.check(got[rows, h], *attn_bound.attend(q[rows, h], k[:, h], v[:, h], seen), h)

@@ -6,8 +6,9 @@
 // (32 per wave, as the columns of va_wide.hpp's tiles) and walks the K/V rows up to
 // its own last one in tiles of 64, one pass with a running maximum and sum. Scores,
 // statistics and the output are held in fp32; the weights p are rounded to fp16 (RNE)
-// for the second product, an error of 2^-12 of each weight, independent between
-// weights, so that of the output stays below its own rounding to fp16.
+// for the second product, each off by at most 2^-11 of itself (down to 2^-24 of the row's
+// largest, see WIDE_OFF), independently of each other, so that the output's error is mostly its
+// own rounding to fp16.
 //
 // The matrix cores bound it: one prompt of 16384 tokens (Hq 32, Hkv 8, D 128) 2.01 ms, 1092
 // TFLOP/s of the products that the mask leaves, where a plain 8192^3 fp16 product reaches 1465;
