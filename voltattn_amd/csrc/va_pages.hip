@@ -47,7 +47,10 @@ __device__ __forceinline__ int count_parents(const int32_t* parents, int n, int 
 }
 
 // A child's block-table row and length, by one wave; true, and the entry, if it needs a page
-// of its own there (a later child's copy of the partly filled last page): the entry is -2.
+// of its own there (a later child's copy of the partly filled last page): the entry is -1. NOTE:
+// its length is then left as its complement for the next launch, which looks for no id, since any id
+// outside the pool may be a parent's.
+template <bool NOTE>
 __device__ __forceinline__ bool fork_child(const PageArgs& a, const int32_t* parents, const int32_t* lens, int c, int& full) {
     const int p = parents[c], lane = (int)__lane_id();
     const bool has = p >= 0 && p < a.B;
@@ -61,13 +64,14 @@ __device__ __forceinline__ bool fork_child(const PageArgs& a, const int32_t* par
     for (int i = lane; i < a.max_pages; i += 64) {
         int id = i < own ? from[i] : -1;
         if (later && i == full && in_pool(a, id)) {         // i < own here: the page in part
-            id = -2;
+            id = -1;
             asks = true;
         }
         to[i] = id;
     }
-    if (lane == 0) a.new_lens[c] = len;
-    return __any(asks);
+    asks = __any(asks);
+    if (lane == 0) a.new_lens[c] = NOTE && asks ? ~len : len;
+    return asks;
 }
 // The counts of a parent's pages: every child more holds the full ones, the first child
 // keeps the last one, and without children all are given up.
@@ -106,7 +110,7 @@ __global__ __launch_bounds__(256) void pages_rows(PageArgs a) {
     const int i = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
     int first;
     if (FORK) {
-        if (i < a.children) (void)fork_child(a, a.parents, a.lens, i, first);
+        if (i < a.children) (void)fork_child<true>(a, a.parents, a.lens, i, first);
         else if (i < a.children + a.B) fork_parent<__HIP_MEMORY_SCOPE_AGENT>(a, a.parents, a.lens, i - a.children);
     } else if (i < a.B) {
         (void)resize_row<__HIP_MEMORY_SCOPE_AGENT>(a, i, a.lens[i], a.after[i], first);
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(PLAN_T) void pages_take(PageArgs a) {
                 fork_parent<__HIP_MEMORY_SCOPE_WORKGROUP>(a, in0, in1, i - rows);
                 continue;
             }
-            if (FORK) need = fork_child(a, in0, in1, i, first);
+            if (FORK) need = fork_child<false>(a, in0, in1, i, first);
             else need = resize_row<__HIP_MEMORY_SCOPE_WORKGROUP>(a, i, in0[i], in1[i], first);
             if (lane == 0) {
                 s_first[i] = first;
@@ -158,8 +162,10 @@ __global__ __launch_bounds__(PLAN_T) void pages_take(PageArgs a) {
                 const int cap = a.max_pages * a.page_rows;
                 int first;
                 if (FORK) {
-                    first = a.new_lens[b] / a.page_rows;
-                    need = first < a.max_pages && a.new_table[(size_t)b * a.max_pages + first] == -2;
+                    int len = a.new_lens[b];
+                    need = len < 0;
+                    if (need) a.new_lens[b] = len = ~len;
+                    first = len / a.page_rows;
                 } else {
                     first = pages_of(min(a.lens[b], cap), a.page_rows);
                     need = max(0, pages_of(min(a.after[b], cap), a.page_rows) - first);
@@ -203,7 +209,6 @@ __global__ __launch_bounds__(PLAN_T) void pages_take(PageArgs a) {
             __syncthreads();                                // s_free is read
         }
         missing += total - got;
-        if (FORK && need && upto > got) a.new_table[(size_t)b * a.max_pages + s_first[tid]] = -1;
         __syncthreads();                                    // s_upto and s_first are read
     }
     if (tid == 0 && a.missing) *a.missing = missing;
