@@ -1,0 +1,60 @@
+"""The serving operators have no gradients and say so: an output of prefill or decode_tree for
+inputs that require grad raises in backward(), as that of decode_paged does, instead of leaving
+gradients of None behind a warning. Inputs that require none, or calls under no_grad, are as they were."""
+import warnings
+
+import pytest
+import torch
+
+import voltattn_amd.torch_ops  # noqa: F401
+
+ops = torch.ops.voltattn
+
+
+def _int(x, dtype=torch.int32):
+    return torch.tensor(x, dtype=dtype, device="cuda")
+
+
+def _calls(q_grad):
+    g = torch.Generator("cuda").manual_seed(0)
+    q = torch.randn((40, 4, 64), generator=g, device="cuda").half().requires_grad_(q_grad)
+    k, v = (torch.randn((40, 2, 64), generator=g, device="cuda").half() for _ in "kv")
+    yield q, lambda: ops.prefill(q, k, v, _int([0, 40]))
+    qt = torch.randn((1, 3, 4, 64), generator=g, device="cuda").half().requires_grad_(q_grad)
+    kp, vp = (torch.randn((2, 2, 64, 64), generator=g, device="cuda").half() for _ in "kv")
+    yield qt, lambda: ops.decode_tree(qt, kp, vp, None, None, _int([[0, 1]]), _int([90]), None, _int([[1, 2, 4]], torch.int64), "f16+", 128)
+
+
+@pytest.mark.gpu
+def test_backward_raises():
+    for leaf, call in _calls(True):
+        out = call()
+        assert out.requires_grad
+        with pytest.raises(RuntimeError, match="no gradient|no autograd|autograd"):
+            out.float().sum().backward()
+        assert leaf.grad is None
+
+
+@pytest.mark.gpu
+def test_without_gradients_nothing_changes():
+    plain = [call() for _, call in _calls(False)]
+    assert not any(o.requires_grad for o in plain)
+    with torch.no_grad():
+        quiet = [call() for _, call in _calls(True)]
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        grads = [call() for _, call in _calls(True)]
+    for a, b, c in zip(plain, quiet, grads):
+        assert not b.requires_grad and torch.equal(a, b) and torch.equal(a, c.detach())
+
+
+def test_traced_calls_raise_too():
+    """The same through the shapes-only implementation (meta tensors)."""
+    q = torch.empty((5, 4, 64), dtype=torch.float16, device="meta", requires_grad=True)
+    k = torch.empty((5, 2, 64), dtype=torch.float16, device="meta")
+    out = ops.prefill(q, k, k, torch.empty(2, dtype=torch.int32, device="meta"))
+    assert out.shape == q.shape and out.requires_grad
+    with pytest.raises(RuntimeError, match="no gradient|no autograd|autograd"):
+        out.float().sum().backward()
+    with torch.no_grad():
+        assert not ops.prefill(q, k, k, torch.empty(2, dtype=torch.int32, device="meta")).requires_grad

@@ -381,6 +381,23 @@ def _(packed, scales, bits, group=32):
 _LIBRARY = torch.library.Library("voltattn", "FRAGMENT")
 
 
+_KEY = torch._C.DispatchKey
+_PLAIN = (torch._C.DispatchKeySet(_KEY.CUDA) | torch._C.DispatchKeySet(_KEY.AutogradCUDA)).raw_repr()
+
+
+class _NoGradient(torch.autograd.Function):
+    """An op's output for inputs that require grad: backward() raises, as that of custom_op's ops does."""
+
+    @staticmethod
+    def forward(ctx, name, call, *args):
+        ctx.name = name
+        return call(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        _fail(f"backward through voltattn::{ctx.name}, which has no gradient formula")
+
+
 def _op(schema: str, fake):
     """Registers the decorated function and its fake implementation; what it returns is the op."""
     name = schema.split("(")[0]
@@ -391,6 +408,18 @@ def _op(schema: str, fake):
         torch.library.register_fake(f"voltattn::{name}", fake, lib=_LIBRARY)
         op = getattr(torch.ops.voltattn, name)
         op.__doc__ = fn.__doc__
+        if "!" not in schema:                           # its outputs are computed from its inputs
+
+            def autograd(keys, *args):
+                below = keys & torch._C._after_autograd_keyset
+                if torch._C.is_grad_enabled() and torch._C._any_requires_grad(*args):
+                    return _NoGradient.apply(name, lambda *a: op.default.redispatch(below, *a), *args)
+                if keys.raw_repr() == _PLAIN:           # plain tensors on a GPU: the dispatcher's second turn takes 3 us
+                    return fn(*args)
+                with torch._C._AutoDispatchBelowAutograd():
+                    return op.default.redispatch(below, *args)
+
+            _LIBRARY.impl(name, autograd, "Autograd", with_keyset=True)
         return op
 
     return register
