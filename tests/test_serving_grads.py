@@ -58,3 +58,34 @@ def test_traced_calls_raise_too():
         out.float().sum().backward()
     with torch.no_grad():
         assert not ops.prefill(q, k, k, torch.empty(2, dtype=torch.int32, device="meta")).requires_grad
+
+
+@pytest.mark.gpu
+def test_changed_pools_are_noticed():
+    """A pool that backward() needs and that an operator then changes in place: torch's own error, no wrong gradient."""
+    for change in ("compact", "fork", "resize"):
+        pool = torch.ones((3, 1, 64, 64), device="cuda").half()
+        x = torch.ones_like(pool).requires_grad_()
+        table, refs = _int([[0, 1]]), _int([1, 1, 0])
+        y = (x * pool).sum() + (torch.ones(3, device="cuda", requires_grad=True) * refs).sum()
+        if change == "compact":
+            ops.compact_kv(pool, pool.clone(), None, None, table, _int([0]), _int([[1]]), _int([1]), "f16+")
+        elif change == "fork":
+            ops.fork_pages(table, _int([100]), _int([0, 0]), refs, pool, pool.clone(), None, None, "f16+")
+        else:
+            ops.resize_pages(table, refs, _int([100]), _int([60]), 64)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+@pytest.mark.gpu
+def test_pools_made_in_inference_mode():
+    """They keep no count of changes: the operators take them as they are."""
+    with torch.inference_mode():
+        pool = torch.ones((3, 1, 64, 64), device="cuda").half()
+        table, refs = _int([[0, 1]]), _int([1, 1, 0])
+    for again in (False, True):
+        with torch.inference_mode(again):
+            ops.compact_kv(pool, pool.clone(), None, None, table, _int([0]), _int([[1]]), _int([1]), "f16+")
+            ops.fork_pages(table, _int([100]), _int([0]), refs, pool, pool.clone(), None, None, "f16+")
+            assert int(ops.resize_pages(table, refs, _int([100]), _int([100]), 64)) == 0

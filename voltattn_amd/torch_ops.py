@@ -444,6 +444,11 @@ def _contiguous(*ts) -> None:
             _fail(f"a tensor of shape {tuple(t.shape)} must be contiguous")
 
 
+def _changed(*ts) -> None:
+    """Notes that the tensors have changed in place, so that backward() does not take them for what was saved."""
+    torch.autograd.graph.increment_version([t for t in ts if t is not None and not t.is_inference()])
+
+
 def _validate_prefill(q, k, v, cu) -> None:
     if q.dim() != 3:
         _fail(f"q must be [T, Hq, D] (got {tuple(q.shape)})")
@@ -607,6 +612,7 @@ def compact_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: Opti
     p, shape = _pools(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, f, group)
     check(lib.va_compact_kv(int(f), C.byref(p), C.byref(shape), _ptr(block_table), _ptr(base), _ptr(keep),
                             _ptr(counts), keep.shape[1], stream))
+    _changed(k_pages, v_pages, k_scale_pages, v_scale_pages)
 
 
 def _validate_fork(block_table, seq_lens, parents, refs, kp, vp, ksp, vsp, f: Fmt, group: int) -> None:
@@ -644,6 +650,7 @@ def fork_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch
     lens, missing = block_table.new_empty((n,)), block_table.new_empty((1,))
     check(lib.va_fork_pages(int(f), C.byref(p), C.byref(shape), _ptr(block_table), _ptr(seq_lens), _ptr(parents), n,
                             _ptr(refs), _ptr(table), _ptr(lens), _ptr(missing), stream))
+    _changed(refs, k_pages, v_pages, k_scale_pages, v_scale_pages)
     return table, lens, missing
 
 
@@ -675,6 +682,7 @@ def resize_pages(block_table: torch.Tensor, refs: torch.Tensor, old_lens: torch.
     missing = block_table.new_empty((1,))
     check(lib.va_resize_pages(block_table.shape[0], page_rows, block_table.shape[1], refs.shape[0], _ptr(block_table),
                               _ptr(refs), _ptr(old_lens), _ptr(new_lens), _ptr(missing), stream))
+    _changed(block_table, refs)
     return missing
 
 
