@@ -470,7 +470,8 @@ def _validate_prefill(q, k, v, cu) -> None:
 
 
 def _strides(name: str, t: torch.Tensor):
-    """(row, head) strides; the last dimension must be dense. The stride of a dimension of one is free."""
+    """(row, head) strides; the last dimension must be dense. The stride of a dimension of one is never
+    stepped: any that the library takes."""
     T, H, D = t.shape
     row, head, last = t.stride()
     if last != 1:
@@ -478,7 +479,7 @@ def _strides(name: str, t: torch.Tensor):
     if H == 1:
         head = 0
     if T <= 1:
-        row = max(head * H, D)
+        row = D
     return row, head
 
 
