@@ -149,7 +149,7 @@ template <int BM, int BN> struct TreePlan {
     __device__ __forceinline__ void make(TreeSeq& s) const {
         s.bad = s.ctx < 0 || s.n < 0 || s.n > a.T || s.ctx > a.cap - s.n;
         s.len = s.bad ? 0 : s.ctx + s.n;
-        s.tiles = (s.len + BN - 1) / BN;
+        s.tiles = s.len / BN + (s.len % BN != 0);           // len + BN may pass 2^31, as (t + 1) * BN below
         s.blocks = s.bad ? 0 : (s.n * a.group + BM - 1) / BM;
     }
     __device__ __forceinline__ void load(int from, int before) {
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
 #pragma unroll
             for (int x = 0; x < HALVES; ++x) {
                 const int j = t * BN + x * 64;
-                left[x] = max(min(64, sq.len - j), 0);
+                left[x] = max(min(64, sq.len - t * BN - x * 64), 0);
                 int page = left[x] > 0 ? table[j >> a.page_shift] : 0;
                 if (page < 0 || page >= a.num_pages) {
                     bad = true;
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                 }
             }
         };
-        auto hides = [&](int t) { return (t + 1) * BN > sq.ctx; };   // drafts, or rows behind the sequence
+        auto hides = [&](int t) { return t * BN > sq.ctx - BN; };   // drafts, or rows behind the sequence
         auto stage = [&](int t) {
             const int tid = fresh_tid();
             const bool clean = hides(t);
@@ -464,10 +464,10 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
         int ve = -24;                                       // SCALED: V's scales so far are below 2^ve; else unused
         if constexpr (AHEAD) fetch(t0);
         const uint64_t mask = sq.n < 64 ? bits & ((1ull << sq.n) - 1) : bits;
-        // takes the positions from j on that a row does not see out of a block of scores
-        auto hide = [&](int j, f32x16& s) {
-            if (j + 32 <= sq.ctx) return;                   // no drafts, nor rows behind the sequence
-            const int d = sq.ctx - j;                       // below 32: where the drafts begin
+        // takes the positions that a row does not see out of a block of scores; d: where the drafts begin,
+        // from the block's first position
+        auto hide = [&](int d, f32x16& s) {
+            if (d >= 32) return;                            // no drafts, nor rows behind the sequence
             uint32_t seen = d > 0 ? ((1u << d) - 1u) | (uint32_t)(mask << d) : d > -64 ? (uint32_t)(mask >> -d) : 0u;
             seen >>= 4 * half;
 #pragma unroll
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
         };
         auto hide_tile = [&](int t, f32x16 (&s)[KB]) {
 #pragma unroll
-            for (int b = 0; b < KB; ++b) hide(t * BN + 32 * b, s[b]);
+            for (int b = 0; b < KB; ++b) hide(sq.ctx - t * BN - 32 * b, s[b]);
         };
         if constexpr (KIND == KF16 && QW == 4) {
             size_t at = 0, next = 0;                        // pool row of the tile fetched, and of its successor
@@ -535,7 +535,6 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
             }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                const int j = t * BN + (kw * KB + kb) * 32;
                 const WideAddr<D> ad = ad0.fresh();
                 const uint32_t at32 = (uint32_t)(kb * 64 * D);   // the block's rows, in bytes
                 f32x16 s = {};
@@ -584,7 +583,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                         for (int v4 = 0; v4 < 4; ++v4) vsc[g][v4] = lds_scales(svt, sat + (uint32_t)((g * BN + kb * 32 + 8 * v4) * 2));
                 }
                 order();
-                hide(j, s);
+                hide(sq.ctx - t * BN - (kw * KB + kb) * 32, s);
                 float top = s[0];
 #pragma unroll
                 for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
@@ -693,7 +692,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                     const int nd = to / a.group;
                     const uint64_t bits = a.mask[(size_t)b * a.T + nd];
 #pragma unroll 1
-                    for (int j = max(t0, sq.ctx / BN) * BN; j < min(t1 * BN, sq.len); ++j)
+                    for (int j = max(t0, sq.ctx / BN) * BN; j < (t1 < sq.tiles ? t1 * BN : sq.len); ++j)
                         if (j < sq.ctx || (bits >> (j - sq.ctx) & 1)) 
                             x += tree_odd<KIND, D, G, EXACT2>(a.v, a.sv, a.page_shift, a.num_pages, a.hkv, table[j >> a.page_shift], hk, j, c0 + c);
                 }
