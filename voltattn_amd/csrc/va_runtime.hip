@@ -791,6 +791,18 @@ int va_append_kv(va_fmt fmt, const uint16_t* x, int n, const int32_t* start,
     return VA_OK;
 }
 
+} // extern "C"
+
+namespace {
+
+// Work-groups of 256 threads in a launch at most: the runtime counts 2^32 - 1 threads, and a larger
+// grid may run as its remainder without an error.
+constexpr long long MAX_GROUPS = (1 << 24) - 1;
+
+} // namespace
+
+extern "C" {
+
 int va_prefill(const va_prefill_bufs* b, const va_prefill_shape* sh, void* stream) {
     if (!sh) return fail(VA_ENULL, "shape is NULL");
     if (!b) return fail(VA_ENULL, "bufs is NULL");
@@ -803,7 +815,7 @@ int va_prefill(const va_prefill_bufs* b, const va_prefill_shape* sh, void* strea
         if (s < 0 || s % 8) return fail(VA_EINVAL, "strides must be multiples of 8 and >= 0 (got %lld)", (long long)s);
     for (const int64_t s : {sh->k_row, sh->v_row})
         if (s < sh->D || s >= 1 << 24) return fail(VA_EINVAL, "k_row and v_row must be in [D, 2^24) (got %lld)", (long long)s);
-    if (va::prefill_items(sh->total, sh->B) * sh->Hq > 0x7FFFFFFFLL) return fail(VA_ERANGE, "B or total too large");
+    if (va::prefill_items(sh->total, sh->B) * sh->Hq > MAX_GROUPS) return fail(VA_ERANGE, "B or total too large");
     if (sh->total == 0) return VA_OK;
     if (!b->q || !b->k || !b->v || !b->cu || !b->out) return fail(VA_ENULL, "q, k, v, cu and out must be non-NULL");
     if (!aligned(b->q, 16) || !aligned(b->k, 16) || !aligned(b->v, 16) || !aligned(b->out, 16))
@@ -842,6 +854,7 @@ int validate_tree(va_fmt fmt, const va_paged_shape* sh, int T, va::TreeForm* for
     if (T < 1 || T > VA_TREE_MAX) return fail(VA_EINVAL, "T must be in [1, %d] (got %d)", VA_TREE_MAX, T);
     const long long rows = (long long)T * (sh->Hq / sh->Hkv);
     if (rows > 1 << 20 || (long long)sh->B * T * sh->Hq > 0x7FFFFFFFLL / 64) return fail(VA_ERANGE, "B*T*Hq too large");
+    if ((long long)sh->B * sh->Hkv * ((rows + 31) / 32) > MAX_GROUPS) return fail(VA_ERANGE, "B*Hkv too large");
     *form = va::tree_form(kind_of(fmt), sh->D, sh->B, sh->Hkv, (int)rows, sh->max_seq_len, cus_or_default());
     if (form->tiles > 1 << 30) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
     return VA_OK;
@@ -955,7 +968,7 @@ int va_compact_kv(va_fmt fmt, const va_pools* pools, const va_paged_shape* sh, c
     const int rc = page_args(fmt, pools, sh, &a);
     if (rc) return rc;
     if (n < 0 || n > VA_TREE_MAX) return fail(VA_EINVAL, "n must be in [0, %d] (got %d)", VA_TREE_MAX, n);
-    if ((long long)sh->B * sh->Hkv > 0x7FFFFFFFLL) return fail(VA_ERANGE, "B*Hkv too large");
+    if ((long long)sh->B * sh->Hkv > MAX_GROUPS) return fail(VA_ERANGE, "B*Hkv too large");
     if (n == 0) return VA_OK;
     if (!block_table || !base || !keep || !counts) return fail(VA_ENULL, "block_table, base, keep and counts must be non-NULL");
     if (!aligned4({block_table, base, keep, counts})) return fail(VA_EALIGN, "block_table, base, keep or counts misaligned");
@@ -976,7 +989,7 @@ int va_fork_pages(va_fmt fmt, const va_pools* pools, const va_paged_shape* sh, c
     const int rc = page_args(fmt, pools, sh, &a);
     if (rc) return rc;
     if (children < 1) return fail(VA_EINVAL, "children must be >= 1 (got %d)", children);
-    if ((long long)children * sh->Hkv > 0x7FFFFFFFLL || (long long)children + sh->B > 0x7FFFFFF0LL)
+    if ((long long)children * sh->Hkv > MAX_GROUPS || (long long)children + sh->B > 4 * MAX_GROUPS)   // a wave each
         return fail(VA_ERANGE, "too many sequences");
     if (!block_table || !seq_lens || !parents || !refs || !new_table || !new_lens)
         return fail(VA_ENULL, "block_table, seq_lens, parents, refs, new_table and new_lens must be non-NULL");
@@ -1001,7 +1014,7 @@ int va_resize_pages(int B, int page_rows, int max_pages, int num_pages, int32_t*
                     const int32_t* old_lens, const int32_t* new_lens, int32_t* missing, void* stream) {
     if (B < 1 || page_rows < 1 || max_pages < 1 || num_pages < 1)
         return fail(VA_EINVAL, "B, page_rows, max_pages and num_pages must be >= 1");
-    if (B > 0x7FFFFFF0) return fail(VA_ERANGE, "too many sequences");
+    if (B > 4 * MAX_GROUPS) return fail(VA_ERANGE, "too many sequences");
     const int rc = validate_pages(page_rows, max_pages, num_pages);
     if (rc) return rc;
     if (!block_table || !refs || !old_lens || !new_lens)

@@ -556,8 +556,8 @@ def decode_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k
     nbytes = lib.va_tree_ws_bytes(int(f), C.byref(shape), T)
     out = torch.empty_like(q)
     ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
-    b = _TreeBufs(_ptr(k_pages), _ptr(v_pages), _ptr(k_scale_pages), _ptr(v_scale_pages), _ptr(block_table),
-                  _ptr(ctx_lens), _ptr(tree_sizes), _ptr(tree_mask), _ptr(q), _ptr(out), _ptr(ws))
+    b = _TreeBufs(k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale_pages), _ptr(v_scale_pages), block_table.data_ptr(),
+                  ctx_lens.data_ptr(), _ptr(tree_sizes), tree_mask.data_ptr(), q.data_ptr(), out.data_ptr(), ws.data_ptr())
     check(lib.va_decode_tree(int(f), C.byref(b), C.byref(shape), T, stream))
     return out
 
