@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("odd", [-2, -1, -3, -(2 ** 31), 2 ** 31 - 1])
-@pytest.mark.parametrize("B,wide", [(6, 5), (80, 5), (3, 9000)])
+@pytest.mark.parametrize("B,wide", [(6, 5), (14, 5), (15, 5), (80, 5), (3, 9000)])
 def test_ids_outside_the_pool_are_carried_along(B, wide, odd):
     rng = random.Random(B + wide)
     page, fmt, spare = 8, "q8+", 4 * B

@@ -13,7 +13,7 @@ namespace va {
 
 constexpr int PLAN_T = 1024;          // threads of the planning work-group
 constexpr int PLAN_IDS = 8;           // page counts that one of its threads looks at at once
-constexpr int PLAN_ONE = 128;         // sequences (parents and children) that it plans by itself
+constexpr int PLAN_ONE = 32;          // sequences (parents and children) that it plans by itself at most
 
 __device__ __forceinline__ int pages_of(int n, int page_rows) { return n <= 0 ? 0 : (n - 1) / page_rows + 1; }
 __device__ __forceinline__ bool in_pool(const PageArgs& a, int id) { return id >= 0 && id < a.num_pages; }
@@ -311,13 +311,17 @@ hipError_t launch_compact(const PageArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// One launch plans a small batch; a large one's rows are dealt over the device first. Sixteen
-// sequences forked into sixteen: 7.6 us with one planning launch, 7.7 with two; a single group's
-// time grows with the table, and its LDS holds up to PLAN_ONE.
-static bool plan_in_one(const PageArgs& a, int rows) { return rows <= PLAN_ONE && (long long)rows * a.max_pages <= 1 << 15; }
+// One launch plans a small batch; a large one's rows are dealt over the device first. One launch :
+// two, us a call: a resize of 16 sequences 3.8 : 4.7, 32 4.6 : 5.1, 48 5.5 : 5.1, 128 9.3 : 6.0, about
+// the same for tables of 8 to 4096 columns. A fork writes whole rows of the table (with a 2 us reset of the
+// counts): 8 sequences into 8 9.9 : 10.2 with 256 columns, 13.2 : 12.4 with 1024; 16 into 16 10.2 : 10.0
+// with 64, 11.3 : 10.6 with 256; 64 into 64 16.7 : 11.3 with 64.
+static bool plan_in_one(const PageArgs& a, int rows, bool whole_rows) {
+    return rows <= PLAN_ONE && (!whole_rows || (long long)rows * a.max_pages <= 1 << 12);
+}
 
 hipError_t launch_resize(const PageArgs& a, hipStream_t stream) {
-    if (plan_in_one(a, a.B)) {
+    if (plan_in_one(a, a.B, false)) {
         hipLaunchKernelGGL((pages_take<false, true>), dim3(1), dim3(PLAN_T), 0, stream, a);
         return hipGetLastError();
     }
@@ -330,7 +334,7 @@ hipError_t launch_resize(const PageArgs& a, hipStream_t stream) {
 
 hipError_t launch_fork(const PageArgs& a, hipStream_t stream) {
     hipError_t e;
-    if (plan_in_one(a, a.children + a.B)) {
+    if (plan_in_one(a, a.children + a.B, true)) {
         hipLaunchKernelGGL((pages_take<true, true>), dim3(1), dim3(PLAN_T), 0, stream, a);
         e = hipGetLastError();
     } else {

@@ -32,8 +32,8 @@ template <int KIND, int D, int G>
 static hipError_t launch(const TreeArgs& a, hipStream_t stream) {
     const dim3 grid((unsigned)(a.nwg + 7) / 8 * 8), block(256);
     // rows to a merging work-group, and waves to a row's pieces: 32 and 1, or 8 and 4 where the former
-    // would leave CUs idle (512 rows: 19.5 us the whole call with the former, 17.5 with the latter;
-    // 16384 rows 65.0 : 66.2 us)
+    // would leave CUs idle. The whole call, 8 and 4 : 32 and 1, 16 drafts and 32 query heads over 8192
+    // positions q8: 512 rows 24.7 : 32.5 us, 2048 46.5 : 48.4, 4096 69.5 : 70.1, 8192 114.3 : 114.1, 16384 203.8 : 201.6
     const bool few = (long long)a.B * a.T * a.hkv * a.group <= 8192;
     const int mr = few ? 8 : 32;
     const dim3 mgrid((unsigned)((size_t)a.B * a.hkv * ((a.T * a.group + mr - 1) / mr)));
