@@ -89,3 +89,26 @@ def test_pools_made_in_inference_mode():
             ops.compact_kv(pool, pool.clone(), None, None, table, _int([0]), _int([[1]]), _int([1]), "f16+")
             ops.fork_pages(table, _int([100]), _int([0]), refs, pool, pool.clone(), None, None, "f16+")
             assert int(ops.resize_pages(table, refs, _int([100]), _int([100]), 64)) == 0
+
+
+@pytest.mark.gpu
+def test_under_autocast_modes_and_compile():
+    """The ways into the operators that do not take the plain call's short cut."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Through(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    for _, call in _calls(False):
+        want = call()
+        with torch.autocast("cuda"):
+            assert torch.equal(call(), want)
+        with Through():
+            assert torch.equal(call(), want)
+        with torch.inference_mode():
+            assert torch.equal(call(), want)
+    q = torch.randn((40, 4, 64), device="cuda").half()
+    cu = _int([0, 40])
+    traced = torch.compile(lambda x: ops.prefill(x, x[:, :2], x[:, 2:], cu) * 2, backend="aot_eager", fullgraph=True)
+    assert torch.equal(traced(q), ops.prefill(q, q[:, :2], q[:, 2:], cu) * 2)
