@@ -411,11 +411,12 @@ def _op(schema: str, fake):
         if "!" not in schema:                           # its outputs are computed from its inputs
 
             def autograd(keys, *args):
-                below = keys & torch._C._after_autograd_keyset
-                if torch._C.is_grad_enabled() and torch._C._any_requires_grad(*args):
-                    return _NoGradient.apply(name, lambda *a: op.default.redispatch(below, *a), *args)
-                if keys.raw_repr() == _PLAIN:           # plain tensors on a GPU: the dispatcher's second turn takes 3 us
+                grads = torch._C.is_grad_enabled() and torch._C._any_requires_grad(*args)
+                if not grads and keys.raw_repr() == _PLAIN:     # on a GPU: the dispatcher's second turn takes 3 us
                     return fn(*args)
+                below = keys & torch._C._after_autograd_keyset
+                if grads:
+                    return _NoGradient.apply(name, lambda *a: op.default.redispatch(below, *a), *args)
                 with torch._C._AutoDispatchBelowAutograd():
                     return op.default.redispatch(below, *args)
 
@@ -444,9 +445,22 @@ def _contiguous(*ts) -> None:
             _fail(f"a tensor of shape {tuple(t.shape)} must be contiguous")
 
 
-def _changed(*ts) -> None:
-    """Notes that the tensors have changed in place, so that backward() does not take them for what was saved."""
-    torch.autograd.graph.increment_version([t for t in ts if t is not None and not t.is_inference()])
+# Notes that tensors have changed in place, so that backward() does not take them for what was saved;
+# those made in inference mode keep no such count and are passed over.
+_changed = torch._C._increment_version
+
+
+def _ready(t: torch.Tensor, *others) -> int:
+    """_on_device and _contiguous in one pass."""
+    at = t.get_device()
+    ok = t.is_contiguous()
+    for x in others:
+        if x is not None and (x.get_device() != at or not x.is_contiguous()):
+            ok = False
+    if not ok or at < 0 or not t.is_cuda or at != torch._C._cuda_getDevice():
+        _on_device(t, *others)
+        _contiguous(t, *others)
+    return torch._C._cuda_getCurrentRawStream(at)
 
 
 def _validate_prefill(q, k, v, cu) -> None:
@@ -547,9 +561,7 @@ def decode_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k
     f = _fmt(fmt)
     _validate_tree(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask, f,
                    group)
-    stream = _on_device(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask)
-    _contiguous(q, k_pages, v_pages, k_scale_pages, v_scale_pages,
-                block_table, ctx_lens, tree_sizes, tree_mask)
+    stream = _ready(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, ctx_lens, tree_sizes, tree_mask)
     B, T, Hq, D = q.shape
     num_pages, Hkv, page_rows = k_pages.shape[:3]
     shape = _PagedShape(B, Hq, Hkv, D, group, page_rows, block_table.shape[1], num_pages, max_seq_len)
@@ -607,13 +619,11 @@ def compact_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: Opti
     """For i < counts[b], row base[b] + i of sequence b becomes what row base[b] + keep[b, i] was (K, V, scales)."""
     f = _fmt(fmt)
     _validate_compact(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts, f, group)
-    stream = _on_device(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts)
-    _contiguous(k_pages, v_pages, k_scale_pages, v_scale_pages,
-                block_table, base, keep, counts)
+    stream = _ready(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, base, keep, counts)
     p, shape = _pools(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, f, group)
     check(lib.va_compact_kv(int(f), C.byref(p), C.byref(shape), _ptr(block_table), _ptr(base), _ptr(keep),
                             _ptr(counts), keep.shape[1], stream))
-    _changed(k_pages, v_pages, k_scale_pages, v_scale_pages)
+    _changed((k_pages, v_pages) if k_scale_pages is None else (k_pages, v_pages, k_scale_pages, v_scale_pages))
 
 
 def _validate_fork(block_table, seq_lens, parents, refs, kp, vp, ksp, vsp, f: Fmt, group: int) -> None:
@@ -642,16 +652,14 @@ def fork_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch
     [children, max_pages], seq_lens [children], missing [1]: pages that the pool did not have)."""
     f = _fmt(fmt)
     _validate_fork(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages, f, group)
-    stream = _on_device(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages)
-    _contiguous(block_table, seq_lens, parents, refs, k_pages,
-                v_pages, k_scale_pages, v_scale_pages)
+    stream = _ready(block_table, seq_lens, parents, refs, k_pages, v_pages, k_scale_pages, v_scale_pages)
     p, shape = _pools(k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, f, group)
     n = parents.shape[0]
     table = block_table.new_empty((n, block_table.shape[1]))
     lens, missing = block_table.new_empty((n,)), block_table.new_empty((1,))
     check(lib.va_fork_pages(int(f), C.byref(p), C.byref(shape), _ptr(block_table), _ptr(seq_lens), _ptr(parents), n,
                             _ptr(refs), _ptr(table), _ptr(lens), _ptr(missing), stream))
-    _changed(refs, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    _changed((refs, k_pages, v_pages) if k_scale_pages is None else (refs, k_pages, v_pages, k_scale_pages, v_scale_pages))
     return table, lens, missing
 
 
@@ -678,12 +686,11 @@ def resize_pages(block_table: torch.Tensor, refs: torch.Tensor, old_lens: torch.
     """Every sequence from old_lens[b] to new_lens[b] positions: pages no longer held are given up (0 frees the
     sequence), missing ones handed out, lowest free id (refs 0) first. Returns how many the pool did not have, [1]."""
     _validate_resize(block_table, refs, old_lens, new_lens, page_rows)
-    stream = _on_device(block_table, refs, old_lens, new_lens)
-    _contiguous(block_table, refs, old_lens, new_lens)
+    stream = _ready(block_table, refs, old_lens, new_lens)
     missing = block_table.new_empty((1,))
     check(lib.va_resize_pages(block_table.shape[0], page_rows, block_table.shape[1], refs.shape[0], _ptr(block_table),
                               _ptr(refs), _ptr(old_lens), _ptr(new_lens), _ptr(missing), stream))
-    _changed(block_table, refs)
+    _changed((block_table, refs))
     return missing
 
 
