@@ -88,8 +88,8 @@ def _fail(msg: str):
 # decode loop whose L grows does not recompile on every step. Only the head
 # dimension D (64 or 128) and the group size decide which kernel runs.
 
-def _check(cond, msg) -> None:
-    if cond is True:                     # plain sizes: nothing to record
+def _check(cond, msg) -> None:           # callers may skip it where cond is True: nothing to record
+    if cond is True:
         return
     torch._check(cond, lambda: f"voltattn: {msg()}")
 
@@ -108,11 +108,13 @@ def _expect(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> Non
 
 
 def _check_dg(f: Fmt, D, group: int) -> None:
-    _check((D == 64) | (D == 128), lambda: f"D must be 64 or 128 (got {D})")
+    if (ok := (D == 64) | (D == 128)) is not True:
+        _check(ok, lambda: f"D must be 64 or 128 (got {D})")
     if _BITS[f] != 16:
         if group not in (32, 64):
             _fail(f"group must be 32 or 64 (got {group})")
-        _check(D >= group, lambda: f"group must be <= D (got {group}, D={D})")
+        if (ok := D >= group) is not True:
+            _check(ok, lambda: f"group must be <= D (got {group}, D={D})")
 
 
 def _row_shape(f: Fmt, D) -> tuple[tuple, torch.dtype]:
@@ -468,19 +470,24 @@ def _validate_prefill(q, k, v, cu) -> None:
         _fail(f"q must be [T, Hq, D] (got {tuple(q.shape)})")
     T, Hq, D = q.shape
     _expect(q, "q", (T, Hq, D), torch.float16)
-    _check((D == 64) | (D == 128), lambda: f"D must be 64 or 128 (got {D})")
+    if (ok := (D == 64) | (D == 128)) is not True:
+        _check(ok, lambda: f"D must be 64 or 128 (got {D})")
     if k.dim() != 3:
         _fail(f"k must be [T, Hkv, D] (got {tuple(k.shape)})")
     Hkv = k.shape[1]
-    _check(Hkv >= 1, lambda: f"k must have at least one head (got {Hkv})")
-    _check(Hq >= 1, lambda: f"q must have at least one head (got {Hq})")
-    _check(Hq % Hkv == 0, lambda: f"query heads ({Hq}) must be a multiple of K/V heads ({Hkv})")
+    if (ok := Hkv >= 1) is not True:
+        _check(ok, lambda: f"k must have at least one head (got {Hkv})")
+    if (ok := Hq >= 1) is not True:
+        _check(ok, lambda: f"q must have at least one head (got {Hq})")
+    if (ok := Hq % Hkv == 0) is not True:
+        _check(ok, lambda: f"query heads ({Hq}) must be a multiple of K/V heads ({Hkv})")
     _expect(k, "k", (T, Hkv, D), torch.float16)
     _expect(v, "v", (T, Hkv, D), torch.float16)
     if cu.dim() != 1:
         _fail(f"cu_seqlens must be [B + 1] (got {tuple(cu.shape)})")
     _expect(cu, "cu_seqlens", (cu.shape[0],), torch.int32)
-    _check(cu.shape[0] >= 2, lambda: f"cu_seqlens must be [B + 1] with B >= 1 (got {tuple(cu.shape)})")
+    if (ok := cu.shape[0] >= 2) is not True:
+        _check(ok, lambda: f"cu_seqlens must be [B + 1] with B >= 1 (got {tuple(cu.shape)})")
 
 
 def _strides(name: str, t: torch.Tensor):
@@ -525,13 +532,16 @@ def _validate_tree(q, kp, vp, ksp, vsp, block_table, ctx_lens, sizes, mask, f: F
         _fail(f"q must be [B, T, Hq, D] (got {tuple(q.shape)})")
     B, T, Hq, D = q.shape
     _expect(q, "q", (B, T, Hq, D), torch.float16)
-    _check((T >= 1) & (T <= TREE_MAX), lambda: f"T must be 1 .. {TREE_MAX} (got {T})")
+    if (ok := (T >= 1) & (T <= TREE_MAX)) is not True:
+        _check(ok, lambda: f"T must be 1 .. {TREE_MAX} (got {T})")
     _check_dg(f, D, group)
     if kp.dim() != 4:
         _fail(f"k_pages must be [num_pages, Hkv, page_rows, row] (got {tuple(kp.shape)})")
     num_pages, Hkv, page_rows, _ = kp.shape
-    _check(Hkv >= 1, lambda: f"k_pages must have at least one head (got {Hkv})")
-    _check(Hq % Hkv == 0, lambda: f"query heads ({Hq}) must be a multiple of K/V heads ({Hkv})")
+    if (ok := Hkv >= 1) is not True:
+        _check(ok, lambda: f"k_pages must have at least one head (got {Hkv})")
+    if (ok := Hq % Hkv == 0) is not True:
+        _check(ok, lambda: f"query heads ({Hq}) must be a multiple of K/V heads ({Hkv})")
     _check_kv(f, kp, vp, ksp, vsp, (num_pages, Hkv, page_rows), D, group)
     if block_table.dim() != 2:
         _fail(f"block_table must be [B={B}, max_pages] (got {tuple(block_table.shape)})")
