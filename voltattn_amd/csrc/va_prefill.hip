@@ -15,7 +15,8 @@
 // the exponentials between the products take the rest. Twelve prompts of up to 4001 tokens 335 us
 // (half-empty diagonal tiles), five of up to 261 12.1 us (latency). 128 rows to a work-group
 // read K and V half as often as 64; three work-groups to a CU cover each other's softmax. The
-// last tiles, and so the longest rows, are begun first, so that short ones fill the tail.
+// row tiles are begun from the batch's last: of one prompt the longest first, so that short ones
+// fill the tail; of several, whose order is the caller's, prompt by prompt from the last one.
 #include "va_wide.hpp"
 #include "va_kernels.hpp"
 

@@ -460,7 +460,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
             if constexpr (QW == 2) __builtin_amdgcn_sched_barrier(0);
         };
         f32x16 o[DB] = {};
-        float m = -__builtin_inff(), l = 0.f;               // m: raw scores; p = exp2((s - m) qscale + OFF - ve)
+        float m = -__builtin_inff(), l = 0.f;               // m: raw scores; p = exp2((s - m) qscale + OFF - ve); QW = 4: as wide_weights'
         int ve = -24;                                       // SCALED: V's scales so far are below 2^ve; else unused
         if constexpr (AHEAD) fetch(t0);
         const uint64_t mask = sq.n < 64 ? bits & ((1ull << sq.n) - 1) : bits;
@@ -706,7 +706,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                 } else {
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), part, (uint32_t)(r * D + c0 + c) * 4, 0, PART_AUX);
                     if (c0 == 0 && c == 0)
-                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, (f32x2{mm * qs, ll})), part, (uint32_t)(BM * D + 2 * r) * 4, 0, PART_AUX);
+                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, (f32x2{QW == 4 ? mm : mm * qs, ll})), part, (uint32_t)(BM * D + 2 * r) * 4, 0, PART_AUX);
                 }
             }
         }

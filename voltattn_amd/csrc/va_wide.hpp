@@ -48,9 +48,9 @@ template <int D> __device__ __forceinline__ int swz(int row) {
 
 // The running maximum that weights are relative to follows lazily: the largest weight is held as
 // 2^WIDE_OFF at least (fp16 keeps the digits of a weight down to 2^-14, so down to 2^-24 of it)
-// and may grow by 2^WIDE_SLACK before sums and output are rescaled. More room to grow costs weights'
-// digits: 2^4 with 2^8 takes five prompts of up to 261 tokens from 12.4 to 12.2 us, 4 x 64 drafts f16
-// from 64.5 to 64.4, but leaves weights 16 below a row's maximum (e^-16) 5 bits.
+// and may grow by 2^WIDE_SLACK before sums and output are rescaled, which a wave then rarely does.
+// (2^4 with room for 2^8 left the weights 16 below a row's maximum, e^-16, 5 bits; five prompts of up
+// to 261 tokens took 12.2 us with it, 12.3 now, the longer ones the same.)
 constexpr float WIDE_OFF = 10.f, WIDE_SLACK = 5.f;
 
 // x combined over the two half-waves (lanes l and l^32).
@@ -164,8 +164,8 @@ __device__ __forceinline__ void wide_scores(const lds_u8* k, const lds_u8* k2, c
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// The weights of NB blocks of scores, relative to the lazy maximum m (raw scores; a weight is
-// exp2((s - m) qs + WIDE_OFF)), their part of the sum l, and the rescale of what is there.
+// The weights of NB blocks of scores, exp2(s qs - m) with m = the lazy maximum times qs, less
+// WIDE_OFF; their part of the sum l, and the rescale of what is there.
 template <int D, int NB>
 __device__ __forceinline__ void wide_weights(const f32x16 (&s)[NB], float qs, float& m, float& l, f32x16 (&o)[D / 32], f16x8 (&p)[NB][2]) {
     float top = s[0][0];
@@ -174,14 +174,14 @@ __device__ __forceinline__ void wide_weights(const f32x16 (&s)[NB], float qs, fl
 #pragma unroll
         for (int v = 0; v < 16; ++v) top = fmaxf(top, s[b][v]);
     top = halves_max(top);
-    if (__any((top - m) * qs > WIDE_SLACK)) {               // also at the first one: m = -inf
-        const float to = fmaxf(m, top), f = to == m ? 1.f : fast_exp2((m - to) * qs);
+    if (__any(__builtin_fmaf(top, qs, -m) > WIDE_OFF + WIDE_SLACK)) {   // also at the first one: m = -inf
+        const float to = fmaxf(m, __builtin_fmaf(top, qs, -WIDE_OFF)), f = to == m ? 1.f : fast_exp2(m - to);
         m = to;
         l *= f;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) o[db] *= f;
     }
-    const float base = m == -__builtin_inff() ? 0.f : m * qs - WIDE_OFF;
+    const float base = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
