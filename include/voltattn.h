@@ -387,8 +387,8 @@ typedef struct {
  * Where a K/V head has more than 64 query rows (T * Hq / Hkv) and the batch over
  * four K/V tiles of 64 positions (max_seq_len, per K/V head and 128 query rows)
  * for each CU, V's values are rounded to fp16 (2^-11 of each), and K or V values
- * above 131008 may overflow to infinities; elsewhere code times scale is not
- * rounded by itself. The tiled formats only. The last bits of a sequence's sums depend on the
+ * above 131008 may overflow to infinities; elsewhere V's scale is part of the
+ * weight that is rounded. The tiled formats only. The last bits of a sequence's sums depend on the
  * lengths of the whole batch; the same batch gives the same bits. Asynchronous
  * on `stream`; concurrent calls need distinct ws. */
 #define VA_TREE_MAX 64
@@ -442,7 +442,9 @@ int va_fork_pages(va_fmt fmt, const va_pools* pools, const va_paged_shape* shape
  * entries no longer held are given up and become -1 (new_lens[b] = 0 frees the
  * sequence), then the missing ones are handed out. A page that another sequence
  * still holds stays shared: a sequence cut back into such a page must not append
- * to it. block_table and refs are updated in place. */
+ * to it. A growth that found pages missing is taken back by resizing the sequence
+ * to its old length, before it is asked for again. block_table and refs are
+ * updated in place. */
 int va_resize_pages(int B, int page_rows, int max_pages, int num_pages, int32_t* block_table, int32_t* refs,
                     const int32_t* old_lens, const int32_t* new_lens, int32_t* missing, void* stream);
 

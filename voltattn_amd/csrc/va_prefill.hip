@@ -10,10 +10,10 @@
 // largest, see WIDE_OFF), independently of each other, so that the output's error is mostly its
 // own rounding to fp16.
 //
-// The matrix cores bound it: one prompt of 16384 tokens (Hq 32, Hkv 8, D 128) 2.01 ms, 1092
+// The matrix cores bound it: one prompt of 16384 tokens (Hq 32, Hkv 8, D 128) 1.96 ms, 1121
 // TFLOP/s of the products that the mask leaves, where a plain 8192^3 fp16 product reaches 1465;
-// the exponentials between the products take the rest. Twelve prompts of up to 4001 tokens 335 us
-// (half-empty diagonal tiles), five of up to 261 12.1 us (latency). 128 rows to a work-group
+// the exponentials between the products take the rest. Twelve prompts of up to 4001 tokens 330 us
+// (half-empty diagonal tiles, 1.11 of the products, besides), five of up to 261 12.3 us (latency). 128 rows to a work-group
 // read K and V half as often as 64; three work-groups to a CU cover each other's softmax. The
 // row tiles are begun from the batch's last: of one prompt the longest first, so that short ones
 // fill the tail; of several, whose order is the caller's, prompt by prompt from the last one.

@@ -23,10 +23,10 @@
 //     rounded to fp16, each value off by at most 2^-11 of itself. Both are halved, in the codes,
 //     where it is exact, so that code * scale up to 131008 fits; what is below fp16's normal numbers
 //     there is off by 2^-24 at most. fp16 rows go straight to LDS (wide_walk).
-// Measured (MI355X, D = 128): 24 x 32 drafts over up to 16384 positions q4 137 us (388 TFLOP/s
+// Measured (MI355X, D = 128): 24 x 32 drafts over up to 16384 positions q4 135 us (394 TFLOP/s
 // of the two products; unpacking and K's second term bound it, the pieces' 11 us of joining
-// next), 4 x 64 drafts over up to 8003 positions f16, 8 query heads to a K/V head, 62.5 us
-// (485 TFLOP/s), one sequence's 16 drafts over 4096 positions q8 17.6 us (latency: a launch
+// next), 4 x 64 drafts over up to 8003 positions f16, 8 query heads to a K/V head, 61.5 us
+// (493 TFLOP/s), one sequence's 16 drafts over 4096 positions q8 17.8 us (latency: a launch
 // of two kernels, 2 tiles of work to a CU).
 //
 // Work split: the tiles of all (sequence, K/V head, row block), numbered one behind the
