@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
     constexpr int LDS = TILES > EPI + 1024 ? TILES : EPI + 1024;
     __shared__ __align__(1024) uint8_t lds[LDS + 16];
     lds_int* odd = (lds_int*)((lds_u8*)lds + LDS);          // infinite or NaN values were left out
-    lds_int* scale_top = odd + 1;                           // SCALED: the largest of V's scales in each half of the tile
+    lds_int* scale_top = odd + 1;                           // SCALED: the largest of V's scales so far in each half of a tile
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     // the thread's number, made anew: what is computed from it is not held across loops
@@ -388,6 +388,7 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                 }
             }
         };
+        int ve = -24;                                       // SCALED: V's scales so far are below 2^ve; else unused
         auto hides = [&](int t) { return t * BN > sq.ctx - BN; };   // drafts, or rows behind the sequence
         auto stage = [&](int t) {
             const int tid = fresh_tid();
@@ -442,8 +443,12 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                         int top = 0;                        // as bits, which order like the values
 #pragma unroll
                         for (int g = 0; g < NG; ++g) top = max(top, (int)(y[g / 2] >> (16 * (g & 1)) & 0x7FFFu));
-                        top = wave_scan_max(top);
-                        if ((tid & 63) == 63) scale_top[(tid >> 6) & 1] = top;
+                        // rarely one of 2^ve or more
+                        const int limit = ve < -14 ? 1 << (ve + 24) : (ve + 15) << 10;
+                        if (t == t0 || __any(top >= limit)) {
+                            top = wave_scan_max(top);
+                            if ((tid & 63) == 63) scale_top[(tid >> 6) & 1] = top;
+                        }
                     }
 #pragma unroll
                     for (int g = 0; g < NG; ++g)
@@ -461,7 +466,6 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
         };
         f32x16 o[DB] = {};
         float m = -__builtin_inff(), l = 0.f;               // m: raw scores; p = exp2((s - m) qscale + OFF - ve); QW = 4: as wide_weights'
-        int ve = -24;                                       // SCALED: V's scales so far are below 2^ve; else unused
         if constexpr (AHEAD) fetch(t0);
         const uint64_t mask = sq.n < 64 ? bits & ((1ull << sq.n) - 1) : bits;
         // takes the positions that a row does not see out of a block of scores; d: where the drafts begin,
@@ -523,16 +527,8 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
             stage(t);
             if (t + 1 < t1) fetch(t + 1);
             __syncthreads();
-            float grown = 1.f;                              // 2^-(what ve grows by)
-            if constexpr (SCALED) {
-                static_assert(KB == 1, "one rescale per tile");
-                const float top = h2f((uint32_t)uniform(HALVES == 2 ? max(scale_top[0], scale_top[1]) : scale_top[0]));
-                const int to = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 126;   // top < 2^to
-                if (to > ve) {
-                    grown = __builtin_bit_cast(float, (uint32_t)(127 + ve - to) << 23);
-                    ve = to;
-                }
-            }
+            int vtop = 0;                                   // used when the scores are there
+            if constexpr (SCALED) vtop = HALVES == 2 ? max(scale_top[0], scale_top[1]) : scale_top[0];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 const WideAddr<D> ad = ad0.fresh();
@@ -584,6 +580,15 @@ __global__ __launch_bounds__(256, tree_waves(KIND, D, QW)) void tree_attend(Tree
                 }
                 order();
                 hide(sq.ctx - t * BN - (kw * KB + kb) * 32, s);
+                float grown = 1.f;                          // 2^-(what ve grows by)
+                if constexpr (SCALED) {
+                    static_assert(KB == 1, "one rescale per tile");
+                    const int to = (int)(__builtin_bit_cast(uint32_t, h2f((uint32_t)uniform(vtop))) >> 23) - 126;   // below 2^to
+                    if (to > ve) {
+                        grown = __builtin_bit_cast(float, (uint32_t)(127 + ve - to) << 23);
+                        ve = to;
+                    }
+                }
                 float top = s[0];
 #pragma unroll
                 for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
