@@ -68,7 +68,9 @@ typedef enum VA_ENUM_BASE {
     VA_Q8P  = 3,   /* q8+   tiled  (attn_q8_mlp,  src/voltattn.cu:425-490) */
     VA_Q4   = 4,   /* q4    naive  (attn_q4,      src/voltattn.cu:254-320) */
     VA_Q4P  = 5,   /* q4+   tiled  (attn_q4_mlp,  src/voltattn.cu:492-561) */
-    VA_Q3P  = 6    /* q3+   tiled  (attn_q3_mlp,  src/voltattn.cu:563-649) */
+    VA_Q3P  = 6,   /* q3+   tiled  (attn_q3_mlp,  src/voltattn.cu:563-649) */
+    VA_B8P  = 16   /* b8+   e4m3 codes, a scale for each block of positions and head; only the
+                    *       entry points that name it take it (va_append_rope, va_attend_paged) */
 } va_fmt;
 
 /* Device buffers of one decode step: the reference's struct DeviceBufs
@@ -447,6 +449,91 @@ int va_fork_pages(va_fmt fmt, const va_pools* pools, const va_paged_shape* shape
  * updated in place. */
 int va_resize_pages(int B, int page_rows, int max_pages, int num_pages, int32_t* block_table, int32_t* refs,
                     const int32_t* old_lens, const int32_t* new_lens, int32_t* missing, void* stream);
+
+/* ---- rotating cache write, and a cache in 8 bits with a scale for each block ----
+ * No counterpart in the reference. VA_B8P pages hold [Hkv][page_rows][D] e4m3 codes
+ * (sign, 4 bits of exponent with bias 7, 3 of mantissa; 0x7F and 0xFF are NaN, there
+ * are no infinities) and [Hkv][page_rows / G] fp16 scales, one for G in {32, 64}
+ * consecutive positions of a head; a value is code * scale. G divides page_rows.
+ * va_page_bytes and va_page_scale_bytes give its sizes; va_resize_pages keeps its pages. */
+
+typedef struct {
+    int B;             /* sequences, >= 1 */
+    int total;         /* rows of q, k and v, >= 0 */
+    int Hq, Hkv;       /* >= 1 */
+    int D, G;          /* as va_paged_shape; VA_B8P: positions to a scale */
+    int page_rows;     /* >= 1; VA_B8P: a multiple of G */
+    int max_pages, num_pages;
+    int rot;           /* rotated dimensions: a multiple of 16 in [16, D] */
+    int interleaved;   /* 0: dimensions i and i + rot/2 are a pair; 1: 2i and 2i + 1 */
+    float scaling;     /* of the rotated dimensions (1: none) */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;   /* strides, as va_prefill_shape: multiples of 8, >= 0 */
+} va_rope_shape;
+
+/* Device buffers: fp16 rows, outputs, inv_freq and the pools 16-byte aligned (pools of q8, q4 and
+ * q3 4 bytes), scales 2, the others 4. */
+typedef struct {
+    const uint16_t* q;             /* [total][Hq][D], by the strides */
+    const uint16_t* k;             /* [total][Hkv][D] */
+    const uint16_t* v;
+    const int32_t*  cu;            /* [B+1] bounds of the sequences' rows, as va_prefill_bufs; NULL: total == B, a row each */
+    const int32_t*  start;         /* [B] cache position of each sequence's first row */
+    const int32_t*  positions;     /* [total] positions that the rotation goes by; NULL: the rows' cache positions */
+    const int32_t*  block_table;   /* [B][max_pages] */
+    const float*    inv_freq;      /* [rot / 2] radians a position */
+    uint16_t*       q_out;         /* [total][Hq][D] */
+    uint16_t*       k_out;         /* [total][Hkv][D], or NULL */
+    void*           kp;            /* page pools */
+    void*           vp;
+    uint16_t*       ks;            /* their scales (quantized formats, VA_B8P) */
+    uint16_t*       vs;
+} va_rope_bufs;
+
+/* The cache write of a projection's rows with the position rotation: row i of sequence b
+ * goes to position start[b] + i of its pages, k rotated by the angle positions * inv_freq
+ * (64-bit: any position), v as it is; q rotated goes to q_out, k to k_out (fp16, for
+ * va_prefill) if that is not NULL. Any format: fp16 rows and the packed ones are what
+ * va_append_kv writes of the rotated values, in fp32 before they are rounded once.
+ * VA_B8P: a block that the call begins gets the smallest power of two s in [2^-24, 2^15]
+ * with |x| <= 448 s for all that it writes there. A block that begins before start[b]
+ * keeps its scale if that is large enough, else the codes held for the positions before
+ * start[b] are scaled to the new one (and rounded where e4m3 has no finer step). Codes
+ * are x / s, nearest even, at most 448; what is not finite becomes NaN and does not
+ * count for the scale.
+ * Rows past the block table, before position 0, or on a page id outside the pool are not
+ * written. Rows of no sequence become zero in q_out and k_out. Sequences must not share
+ * the pages written. Asynchronous on `stream`; needs no workspace; the outputs must not
+ * overlap the inputs. */
+int va_append_rope(va_fmt fmt, const va_rope_bufs* b, const va_rope_shape* shape, void* stream);
+
+/* Device buffers. Alignment as va_paged_bufs; out, ws 16 bytes; scales 4. */
+typedef struct {
+    const void*     k;             /* VA_B8P page pools */
+    const void*     v;
+    const uint16_t* sk;            /* [num_pages][Hkv][page_rows / G]: any finite scale, the sign is ignored */
+    const uint16_t* sv;
+    const int32_t*  block_table;   /* [B][max_pages] */
+    const int32_t*  cu;            /* [B+1] bounds of the sequences' rows, as va_prefill_bufs; NULL: total == B, a row each */
+    const int32_t*  seq_lens;      /* [B] positions of each sequence, the rows' own among them */
+    const uint16_t* q;             /* [total][Hq][D] fp16 */
+    uint16_t*       out;           /* [total][Hq][D] fp16 */
+    float*          ws;            /* va_attend_ws_bytes bytes; needs no zeroing */
+} va_attend_bufs;
+
+/* Attention of the newest tokens of every sequence, one or many, over its paged cache
+ * (VA_B8P), where their own rows are already: row i of sequence b's n attends positions
+ * 0 .. seq_lens[b] - n + i, softmax(q.K^T / sqrt(D)) V. A row that sees nothing
+ * (seq_lens[b] < n) is zero, as are rows of no sequence. A length below 0 or above
+ * max_seq_len gives NaN for its sequence; a page id outside the pool, or a scale that is
+ * infinite or NaN, for the rows that see its positions. NaN codes reach the rows that see
+ * them only. G: positions to a scale; page_rows a power of two in [64, 2^24]. The last
+ * bits of a row depend on the batch (how its positions are cut up); the same batch gives
+ * the same bits. Asynchronous on `stream`; concurrent calls, and graphs whose replays may
+ * overlap, need distinct ws. */
+int va_attend_paged(va_fmt fmt, const va_attend_bufs* b, const va_paged_shape* shape, int total, void* stream);
+
+/* Workspace of va_attend_paged; 0 for invalid arguments or total 0. */
+size_t va_attend_ws_bytes(va_fmt fmt, const va_paged_shape* shape, int total);
 
 /* ---- runtime shims (the reference calls the CUDA runtime directly:
  *      cudaMalloc/cudaMemcpy/cudaFree/cudaEvent*, src/voltattn.cu:863-895, 936-955,

@@ -32,6 +32,7 @@ __all__ = [
     "pick_splits_paged", "page_bytes", "page_scale_bytes", "append_kv", "row_bytes",
     "PrefillShape", "PrefillBufs", "prefill", "TreeBufs", "decode_tree", "tree_ws_bytes", "TREE_MAX",
     "Pools", "compact_kv", "fork_pages", "resize_pages",
+    "B8", "RopeShape", "RopeBufs", "append_rope", "AttendBufs", "attend_paged", "attend_ws_bytes",
 ]
 
 LIB_PATH = Path(__file__).resolve().parent / "libvoltattn_hip.so"
@@ -98,6 +99,21 @@ class _Pools(C.Structure):
     _fields_ = [(n, _P) for n in ("k", "v", "sk", "sv")]
 
 
+class _RopeShape(C.Structure):
+    _fields_ = [(n, _I) for n in ("B", "total", "Hq", "Hkv", "D", "G", "page_rows", "max_pages", "num_pages", "rot",
+                                  "interleaved")] + [("scaling", C.c_float)] + [
+        (n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+
+
+class _RopeBufs(C.Structure):
+    _fields_ = [(n, _P) for n in ("q", "k", "v", "cu", "start", "positions", "block_table", "inv_freq", "q_out", "k_out",
+                                  "kp", "vp", "ks", "vs")]
+
+
+class _AttendBufs(C.Structure):
+    _fields_ = [(n, _P) for n in ("k", "v", "sk", "sv", "block_table", "cu", "seq_lens", "q", "out", "ws")]
+
+
 class _DevInfo(C.Structure):
     _fields_ = [("name", C.c_char * 256), ("arch", C.c_char * 64), ("compute_units", _I),
                 ("clock_khz", _I), ("mem_clock_khz", _I), ("mem_bus_bits", _I),
@@ -143,6 +159,9 @@ _sig("va_tree_ws_bytes", _SZ, _I, C.POINTER(_PagedShape), _I)
 _sig("va_compact_kv", _I, _I, C.POINTER(_Pools), C.POINTER(_PagedShape), _P, _P, _P, _P, _I, _P)
 _sig("va_fork_pages", _I, _I, C.POINTER(_Pools), C.POINTER(_PagedShape), _P, _P, _P, _I, _P, _P, _P, _P, _P)
 _sig("va_resize_pages", _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P)
+_sig("va_append_rope", _I, _I, C.POINTER(_RopeBufs), C.POINTER(_RopeShape), _P)
+_sig("va_attend_paged", _I, _I, C.POINTER(_AttendBufs), C.POINTER(_PagedShape), _I, _P)
+_sig("va_attend_ws_bytes", _SZ, _I, C.POINTER(_PagedShape), _I)
 _sig("va_device_count", _I, C.POINTER(_I))
 _sig("va_set_device", _I, _I)
 _sig("va_device_info", _I, C.POINTER(_DevInfo))
@@ -449,6 +468,100 @@ def resize_pages(B: int, page_rows: int, max_pages: int, num_pages: int, block_t
     """Pages given up and handed out so that sequence b holds new_lens[b] positions (va_resize_pages)."""
     check(lib.va_resize_pages(B, page_rows, max_pages, num_pages, block_table or None, refs or None, old_lens or None,
                               new_lens or None, missing or None, _stream(stream)))
+
+
+B8 = 16              # VA_B8P, "b8+": e4m3 codes with a scale for each block of G positions and head (no Fmt of the others')
+
+
+@dataclass
+class RopeShape:
+    """va_rope_shape: `total` rows of B sequences. Strides count fp16 elements; 0 stands for the
+    contiguous [total][heads][D] layout."""
+    B: int
+    total: int
+    Hq: int
+    Hkv: int
+    D: int
+    G: int
+    page_rows: int
+    max_pages: int
+    num_pages: int
+    rot: int
+    interleaved: bool = False
+    scaling: float = 1.0
+    q_row: int = 0
+    q_head: int = 0
+    k_row: int = 0
+    k_head: int = 0
+    v_row: int = 0
+    v_head: int = 0
+
+    def _c(self) -> _RopeShape:
+        return _RopeShape(self.B, self.total, self.Hq, self.Hkv, self.D, self.G, self.page_rows, self.max_pages,
+                          self.num_pages, self.rot, int(self.interleaved), self.scaling,
+                          self.q_row or self.Hq * self.D, self.q_head or self.D,
+                          self.k_row or self.Hkv * self.D, self.k_head or self.D,
+                          self.v_row or self.Hkv * self.D, self.v_head or self.D)
+
+
+@dataclass
+class RopeBufs:
+    """va_rope_bufs: device pointers as ints (0 = NULL; cu 0: a row to each sequence; positions 0: the
+    cache's; k_out 0: none)."""
+    q: int = 0
+    k: int = 0
+    v: int = 0
+    cu: int = 0
+    start: int = 0
+    positions: int = 0
+    block_table: int = 0
+    inv_freq: int = 0
+    q_out: int = 0
+    k_out: int = 0
+    K: int = 0
+    V: int = 0
+    scK: int = 0
+    scV: int = 0
+
+    def _c(self) -> _RopeBufs:
+        return _RopeBufs(*(x or None for x in (self.q, self.k, self.v, self.cu, self.start, self.positions, self.block_table,
+                                               self.inv_freq, self.q_out, self.k_out, self.K, self.V, self.scK, self.scV)))
+
+
+def append_rope(f: int, b: RopeBufs, shape: RopeShape, stream=None) -> None:
+    """A projection's rows, rotated by their positions, into a paged cache of format f (a Fmt or B8)."""
+    cb, cs = b._c(), shape._c()
+    check(lib.va_append_rope(int(f), C.byref(cb), C.byref(cs), _stream(stream)))
+
+
+@dataclass
+class AttendBufs:
+    """va_attend_bufs: device pointers as ints (0 = NULL; cu 0: a row to each sequence)."""
+    K: int = 0
+    V: int = 0
+    scK: int = 0
+    scV: int = 0
+    block_table: int = 0
+    cu: int = 0
+    seq_lens: int = 0
+    q: int = 0
+    out: int = 0
+    ws: int = 0
+
+    def _c(self) -> _AttendBufs:
+        return _AttendBufs(*(x or None for x in (self.K, self.V, self.scK, self.scV, self.block_table, self.cu, self.seq_lens,
+                                                 self.q, self.out, self.ws)))
+
+
+def attend_paged(b: AttendBufs, shape: PagedShape, total: int, stream=None) -> None:
+    """Attention of the newest tokens of every sequence (q/out [total][Hq][D]) over a B8 cache."""
+    cb, cs = b._c(), shape._c()
+    check(lib.va_attend_paged(B8, C.byref(cb), C.byref(cs), total, _stream(stream)))
+
+
+def attend_ws_bytes(shape: PagedShape, total: int) -> int:
+    cs = shape._c()
+    return lib.va_attend_ws_bytes(B8, C.byref(cs), total)
 
 
 def row_bytes(f: Fmt, D: int) -> int:

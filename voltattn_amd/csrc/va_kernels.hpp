@@ -240,6 +240,63 @@ struct TreeForm {
 TreeForm tree_form(int kind, int D, int B, int hkv, int rows, int cap, int cus);   // rows: of a K/V head
 hipError_t launch_tree(int kind, int D, int G, const TreeArgs& a, hipStream_t stream);
 
+// Attention of the newest tokens of every sequence over a block-scaled 8-bit cache
+// (va_attend.hpp): row i of sequence b's n rows sees positions 0 .. seq_lens[b] - n + i.
+struct AttendArgs {
+    const uint8_t*  k;            // e4m3 page pools [num_pages][hkv][page_rows][D]
+    const uint8_t*  v;
+    const uint16_t* sk;           // fp16 scales [num_pages][hkv][page_rows / G]
+    const uint16_t* sv;
+    const int32_t*  block_table;  // [B][max_pages]
+    const int32_t*  cu;           // [B + 1] bounds of the sequences' rows, or null: one row each
+    const int32_t*  seq_lens;     // [B] positions, the rows' own among them
+    const uint16_t* q;            // [total][hkv * group][D]
+    uint16_t*       out;
+    float*          ws;           // attend_ws_floats
+    int   B, total, hkv, group;
+    int   max_pages, page_shift, num_pages;
+    int   cap;                    // seq_lens at most
+    float qscale;                 // log2(e) / sqrt(D)
+    FastDiv by_group;
+    int   nwg, form;              // of its AttendForm
+};
+// Rows to a block (16, 32: attend_few; 128: attend_wide), K/V tiles of the batch at most, and work-groups.
+struct AttendForm {
+    int rows;
+    long long tiles, groups;
+};
+AttendForm attend_form(int D, int B, int total, int hkv, int group, int cap, int cus);
+size_t attend_ws_floats(const AttendForm& f, int D);
+hipError_t launch_attend(int D, int G, const AttendArgs& a, hipStream_t stream);
+
+// Cache write of a projection's rows with the position rotation (va_rope.hip).
+struct RopeArgs {
+    const uint16_t* q;            // rows *_row elements apart, heads *_head; null: not rotated
+    const uint16_t* k;
+    const uint16_t* v;
+    const int32_t*  cu;           // [B + 1] bounds of the sequences' rows, or null: one row each
+    const int32_t*  start;        // [B] cache position of each sequence's first row
+    const int32_t*  places;       // [total] positions that the angles go by, or null: the cache's
+    const int32_t*  block_table;  // [B][max_pages]
+    const float*    freq;         // [rot / 2] radians a position
+    uint16_t*       q_out;        // [total][hq][D]
+    uint16_t*       k_out;        // [total][hkv][D], or null
+    uint8_t*        kp;           // pools
+    uint8_t*        vp;
+    uint16_t*       ks;
+    uint16_t*       vs;
+    long long q_row, q_head, k_row, k_head, v_row, v_head;
+    int   B, total, hq, hkv;
+    int   rot, pairs;             // rotated dimensions; pairs: (2i, 2i + 1), else (i, i + rot/2)
+    float scaling;                // of the rotated values
+    int   page_rows, max_pages, num_pages;
+    FastDiv by_page;              // set by launch_rope, as units:
+    long long units;
+};
+// bits 16, 8, 4, 3: a row format with scales for G values; 0: e4m3 with scales for G positions.
+long long rope_groups(int bits, int D, int G, const RopeArgs& a);   // its work-groups at most
+hipError_t launch_rope(int bits, int D, int G, const RopeArgs& a, hipStream_t stream);
+
 // Page pool bookkeeping and row moves (va_pages.hip). Each launch uses the fields that
 // it needs.
 struct PageArgs {

@@ -291,6 +291,7 @@ const char* va_last_error(void) { return g_err; }
 
 const char* va_fmt_name(va_fmt fmt) {
     static const char* names[] = {"f16", "f16+", "q8", "q8+", "q4", "q4+", "q3+"};
+    if (fmt == VA_B8P) return "b8+";
     return valid_fmt(fmt) ? names[fmt] : "?";
 }
 
@@ -635,11 +636,13 @@ int va_decode_gqa(va_fmt fmt, const va_bufs* b, int Hq, int Hkv, int L, int D, i
 }
 
 size_t va_page_bytes(va_fmt fmt, int Hkv, int page_rows, int D) {
+    if (fmt == VA_B8P && Hkv >= 1 && page_rows >= 1 && D >= 1) return (size_t)Hkv * page_rows * D;
     if (!valid_fmt(fmt) || Hkv < 1 || page_rows < 1 || D < 1) return 0;
     return (size_t)Hkv * page_rows * row_bytes(fmt, D);
 }
 
 size_t va_page_scale_bytes(va_fmt fmt, int Hkv, int page_rows, int D, int G) {
+    if (fmt == VA_B8P && Hkv >= 1 && page_rows >= 1 && (G == 32 || G == 64) && page_rows % G == 0) return (size_t)Hkv * (page_rows / G) * 2;
     if (!valid_fmt(fmt) || is_f16(fmt) || Hkv < 1 || page_rows < 1 || G < 1 || D % G) return 0;
     return (size_t)Hkv * page_rows * (D / G) * 2;
 }
@@ -1034,6 +1037,148 @@ int va_resize_pages(int B, int page_rows, int max_pages, int num_pages, int32_t*
     a.num_pages = num_pages;
     const hipError_t e = va::launch_resize(a, as_stream(stream));
     if (e != hipSuccess) return hip_fail(e, "resize launch");
+    return VA_OK;
+}
+
+int va_append_rope(va_fmt fmt, const va_rope_bufs* b, const va_rope_shape* sh, void* stream) {
+    const bool block = fmt == VA_B8P;
+    if (!block && !valid_fmt(fmt)) return fail(VA_EINVAL, "invalid format %d", (int)fmt);
+    if (!sh) return fail(VA_ENULL, "shape is NULL");
+    if (!b) return fail(VA_ENULL, "bufs is NULL");
+    const bool scales = block || !is_f16(fmt);
+    if (sh->B < 1 || sh->Hkv < 1 || sh->Hq < 1) return fail(VA_EINVAL, "B, Hq and Hkv must be >= 1");
+    if (sh->total < 0) return fail(VA_EINVAL, "total must be >= 0 (got %d)", sh->total);
+    if (sh->D != 64 && sh->D != 128) return fail(VA_EINVAL, "D must be 64 or 128 (got %d)", sh->D);
+    if (scales && sh->G != 32 && sh->G != 64) return fail(VA_EINVAL, "G must be 32 or 64 (got G=%d)", sh->G);
+    if (sh->max_pages < 1 || sh->num_pages < 1) return fail(VA_EINVAL, "max_pages and num_pages must be >= 1");
+    if (sh->page_rows < 1) return fail(VA_EINVAL, "page_rows must be >= 1");
+    if (block && sh->page_rows % sh->G) return fail(VA_EINVAL, "page_rows must be a multiple of G (got %d, G=%d)", sh->page_rows, sh->G);
+    if ((long long)sh->num_pages * sh->Hkv * sh->page_rows > (1LL << 40)) return fail(VA_ERANGE, "page pool too large");
+    if (sh->rot < 16 || sh->rot > sh->D || sh->rot % 16)
+        return fail(VA_EINVAL, "rot must be a multiple of 16 in [16, D] (got %d)", sh->rot);
+    if (sh->interleaved != 0 && sh->interleaved != 1) return fail(VA_EINVAL, "interleaved must be 0 or 1 (got %d)", sh->interleaved);
+    for (const int64_t s : {sh->q_row, sh->q_head, sh->k_row, sh->k_head, sh->v_row, sh->v_head})
+        if (s < 0 || s % 8) return fail(VA_EINVAL, "strides must be multiples of 8 and >= 0 (got %lld)", (long long)s);
+    if (!b->cu && sh->total != sh->B) return fail(VA_EINVAL, "without cu, total must be B (got %d, B=%d)", sh->total, sh->B);
+    va::RopeArgs a{};
+    a.B = sh->B;
+    a.total = sh->total;
+    a.hq = sh->Hq;
+    a.hkv = sh->Hkv;
+    const int bits = block ? 0 : bits_of(fmt), G = scales ? sh->G : 32;
+    if ((long long)sh->Hq + 2LL * sh->Hkv > 1 << 24 || va::rope_groups(bits, sh->D, G, a) > MAX_GROUPS)
+        return fail(VA_ERANGE, "total or the heads too large");
+    if (sh->total == 0) return VA_OK;
+    if (!b->q || !b->k || !b->v || !b->start || !b->block_table || !b->inv_freq || !b->q_out || !b->kp || !b->vp || (scales && (!b->ks || !b->vs)))
+        return fail(VA_ENULL, "q, k, v, start, block_table, inv_freq, q_out and the pools (and scales) must be non-NULL");
+    if (!aligned(b->q, 16) || !aligned(b->k, 16) || !aligned(b->v, 16) || !aligned(b->q_out, 16) || !aligned(b->k_out, 16))
+        return fail(VA_EALIGN, "q, k, v, q_out and k_out must be 16-byte aligned");
+    if (!aligned(b->inv_freq, 16)) return fail(VA_EALIGN, "inv_freq must be 16-byte aligned");
+    const size_t pal = scales && !block ? 4 : 16;
+    if (!aligned(b->kp, pal) || !aligned(b->vp, pal)) return fail(VA_EALIGN, "pages misaligned");
+    if (scales && (!aligned(b->ks, 2) || !aligned(b->vs, 2))) return fail(VA_EALIGN, "scales must be 2-byte aligned");
+    if (!aligned4({b->cu, b->start, b->positions, b->block_table})) return fail(VA_EALIGN, "cu, start, positions or block_table misaligned");
+    a.q = b->q;
+    a.k = b->k;
+    a.v = b->v;
+    a.cu = b->cu;
+    a.start = b->start;
+    a.places = b->positions;
+    a.block_table = b->block_table;
+    a.freq = b->inv_freq;
+    a.q_out = b->q_out;
+    a.k_out = b->k_out;
+    a.kp = static_cast<uint8_t*>(b->kp);
+    a.vp = static_cast<uint8_t*>(b->vp);
+    a.ks = b->ks;
+    a.vs = b->vs;
+    a.q_row = sh->q_row;
+    a.q_head = sh->q_head;
+    a.k_row = sh->k_row;
+    a.k_head = sh->k_head;
+    a.v_row = sh->v_row;
+    a.v_head = sh->v_head;
+    a.rot = sh->rot;
+    a.pairs = sh->interleaved;
+    a.scaling = sh->scaling;
+    a.page_rows = sh->page_rows;
+    a.max_pages = sh->max_pages;
+    a.num_pages = sh->num_pages;
+    const hipError_t e = va::launch_rope(bits, sh->D, G, a, as_stream(stream));
+    if (e != hipSuccess) return hip_fail(e, "append launch");
+    return VA_OK;
+}
+
+} // extern "C"
+
+namespace {
+
+// Checks of va_attend_paged's shape, and its launch form.
+int validate_attend(va_fmt fmt, const va_paged_shape* sh, int total, va::AttendForm* form) {
+    if (fmt != VA_B8P) {
+        if (!valid_fmt(fmt)) return fail(VA_EINVAL, "invalid format %d", (int)fmt);
+        return fail(VA_EINVAL, "va_attend_paged takes the format b8+ only (got %s)", va_fmt_name(fmt));
+    }
+    if (!sh) return fail(VA_ENULL, "shape is NULL");
+    va_paged_shape as_rows = *sh;                          // G is of positions here: not bounded by D
+    if (sh->G == 32 || sh->G == 64) as_rows.G = 32;
+    const int rc = validate_shape(VA_Q8P, &as_rows, true);
+    if (rc) return rc;
+    if (total < 0) return fail(VA_EINVAL, "total must be >= 0 (got %d)", total);
+    const int group = sh->Hq / sh->Hkv;
+    if ((long long)total * sh->Hq > 1 << 30) return fail(VA_ERANGE, "total*Hq too large");
+    *form = va::attend_form(sh->D, sh->B, total, sh->Hkv, group, sh->max_seq_len, cus_or_default());
+    if (form->tiles > 1 << 30) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
+    return VA_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+size_t va_attend_ws_bytes(va_fmt fmt, const va_paged_shape* sh, int total) {
+    va::AttendForm form;
+    if (validate_attend(fmt, sh, total, &form) || total == 0) return 0;
+    return va::attend_ws_floats(form, sh->D) * sizeof(float);
+}
+
+int va_attend_paged(va_fmt fmt, const va_attend_bufs* b, const va_paged_shape* sh, int total, void* stream) {
+    va::AttendForm form;
+    const int rc = validate_attend(fmt, sh, total, &form);
+    if (rc) return rc;
+    if (!b) return fail(VA_ENULL, "bufs is NULL");
+    if (!b->cu && total != sh->B) return fail(VA_EINVAL, "without cu, total must be B (got %d, B=%d)", total, sh->B);
+    if (total == 0) return VA_OK;
+    if (!b->k || !b->v || !b->sk || !b->sv || !b->q || !b->out || !b->ws || !b->block_table || !b->seq_lens)
+        return fail(VA_ENULL, "k, v, sk, sv, q, out, ws, block_table and seq_lens must be non-NULL");
+    if (!aligned(b->k, 16) || !aligned(b->v, 16)) return fail(VA_EALIGN, "k and v must be 16-byte aligned");
+    if (!aligned(b->q, 16) || !aligned(b->out, 16) || !aligned(b->ws, 16)) return fail(VA_EALIGN, "q, out and ws must be 16-byte aligned");
+    if (!aligned4({b->sk, b->sv, b->block_table, b->cu, b->seq_lens}))
+        return fail(VA_EALIGN, "sk, sv, block_table, cu or seq_lens misaligned");
+    va::AttendArgs a{};
+    a.k = static_cast<const uint8_t*>(b->k);
+    a.v = static_cast<const uint8_t*>(b->v);
+    a.sk = b->sk;
+    a.sv = b->sv;
+    a.block_table = b->block_table;
+    a.cu = b->cu;
+    a.seq_lens = b->seq_lens;
+    a.q = b->q;
+    a.out = b->out;
+    a.ws = b->ws;
+    a.B = sh->B;
+    a.total = total;
+    a.hkv = sh->Hkv;
+    a.group = sh->Hq / sh->Hkv;
+    a.max_pages = sh->max_pages;
+    a.page_shift = log2i(sh->page_rows);
+    a.num_pages = sh->num_pages;
+    a.cap = sh->max_seq_len;
+    a.qscale = (float)(1.4426950408889634074 / std::sqrt((double)sh->D));
+    a.nwg = (int)form.groups;
+    a.form = form.rows;
+    const hipError_t e = va::launch_attend(sh->D, sh->G, a, as_stream(stream));
+    if (e != hipSuccess) return hip_fail(e, "attend launch");
     return VA_OK;
 }
 

@@ -16,6 +16,10 @@ Importing this module registers
   (va_fork_pages; mutates refs and the pools);
 * ``voltattn::resize_pages(...) -> missing`` — pages given up and handed out (va_resize_pages;
   mutates block_table and refs);
+* ``voltattn::append_rope(...) -> (q, k)`` — a projection's rows rotated by their positions, k and v
+  written into a paged cache (va_append_rope; mutates the pools);
+* ``voltattn::attend_paged(...) -> out`` — the newest tokens of every sequence over a cache in 8 bits
+  with a scale for each block of positions and head (va_attend_paged);
 * ``voltattn::quantize(x, bits, group) -> (packed, scales)`` (va_quantize; the reference's
   quantize(), src/voltattn.cu:705-745);
 * ``voltattn::dequantize(packed, scales, bits, group) -> x`` (va_dequantize; the reference's
@@ -38,11 +42,11 @@ from typing import Optional
 
 import torch
 
-from . import (TREE_MAX, Fmt, _Bufs, _PagedBufs, _PagedShape, _Pools, _PrefillBufs, _PrefillShape, _TreeBufs, check,
-               fmt_bits, lib, ws_bytes)
+from . import (B8, TREE_MAX, Fmt, _AttendBufs, _Bufs, _PagedBufs, _PagedShape, _Pools, _PrefillBufs, _PrefillShape,
+               _RopeBufs, _RopeShape, _TreeBufs, check, fmt_bits, lib, ws_bytes)
 
 __all__ = ["decode", "decode_gqa", "decode_paged", "append_kv", "quantize", "dequantize",
-           "prefill", "decode_tree", "compact_kv", "fork_pages", "resize_pages"]
+           "prefill", "decode_tree", "compact_kv", "fork_pages", "resize_pages", "append_rope", "attend_paged"]
 
 
 # What an op does on the host per call is most of a small call's time: the names are
@@ -400,8 +404,9 @@ class _NoGradient(torch.autograd.Function):
         _fail(f"backward through voltattn::{ctx.name}, which has no gradient formula")
 
 
-def _op(schema: str, fake):
-    """Registers the decorated function and its fake implementation; what it returns is the op."""
+def _op(schema: str, fake, computes: Optional[bool] = None):
+    """Registers the decorated function and its fake implementation; what it returns is the op.
+    computes: whether its outputs are computed from its inputs (None: if it changes none in place)."""
     name = schema.split("(")[0]
 
     def register(fn):
@@ -410,7 +415,7 @@ def _op(schema: str, fake):
         torch.library.register_fake(f"voltattn::{name}", fake, lib=_LIBRARY)
         op = getattr(torch.ops.voltattn, name)
         op.__doc__ = fn.__doc__
-        if "!" not in schema:                           # its outputs are computed from its inputs
+        if "!" not in schema if computes is None else computes:
 
             def autograd(keys, *args):
                 grads = torch._C.is_grad_enabled() and torch._C._any_requires_grad(*args)
@@ -702,6 +707,162 @@ def resize_pages(block_table: torch.Tensor, refs: torch.Tensor, old_lens: torch.
                               _ptr(refs), _ptr(old_lens), _ptr(new_lens), _ptr(missing), stream))
     _changed((block_table, refs))
     return missing
+
+
+# ------------------------------------- rotating cache write, block-scaled cache --
+
+def _block_pools(kp, vp, ksp, vsp, num_pages, Hkv, page_rows, D, group: int) -> None:
+    """Checks of pools of the format b8+: e4m3 codes, a scale for `group` positions of a head."""
+    if group not in (32, 64):
+        _fail(f"group must be 32 or 64 (got {group})")
+    if (ok := page_rows % group == 0) is not True:
+        _check(ok, lambda: f"page_rows must be a multiple of group (got {page_rows}, group={group})")
+    _expect(kp, "k_pages", (num_pages, Hkv, page_rows, D), torch.float8_e4m3fn)
+    _expect(vp, "v_pages", (num_pages, Hkv, page_rows, D), torch.float8_e4m3fn)
+    _expect(ksp, "k_scale_pages", (num_pages, Hkv, page_rows // group), torch.float16)
+    _expect(vsp, "v_scale_pages", (num_pages, Hkv, page_rows // group), torch.float16)
+
+
+def _validate_bounds(cu, T, B) -> None:
+    if cu is None:
+        if (ok := T == B) is not True:
+            _check(ok, lambda: f"without cu_seqlens there is a row to each sequence (got {T} rows, {B} sequences)")
+    else:
+        _expect(cu, "cu_seqlens", (B + 1,), torch.int32)
+
+
+def _validate_rope(q, k, v, inv_freq, cu, start, positions, block_table, kp, vp, ksp, vsp, fmt: str, group: int) -> None:
+    if q.dim() != 3:
+        _fail(f"q must be [T, Hq, D] (got {tuple(q.shape)})")
+    T, Hq, D = q.shape
+    _expect(q, "q", (T, Hq, D), torch.float16)
+    if (ok := (D == 64) | (D == 128)) is not True:
+        _check(ok, lambda: f"D must be 64 or 128 (got {D})")
+    if k.dim() != 3:
+        _fail(f"k must be [T, Hkv, D] (got {tuple(k.shape)})")
+    Hkv = k.shape[1]
+    if (ok := (Hkv >= 1) & (Hq >= 1)) is not True:
+        _check(ok, lambda: f"q and k must have at least one head (got {Hq} and {Hkv})")
+    _expect(k, "k", (T, Hkv, D), torch.float16)
+    _expect(v, "v", (T, Hkv, D), torch.float16)
+    if inv_freq.dim() != 1:
+        _fail(f"inv_freq must be [rot / 2] (got {tuple(inv_freq.shape)})")
+    half = inv_freq.shape[0]
+    _expect(inv_freq, "inv_freq", (half,), torch.float32)
+    if (ok := (half >= 8) & (half % 8 == 0) & (2 * half <= D)) is not True:
+        _check(ok, lambda: f"inv_freq must have a multiple of 8 entries, D / 2 at most (got {half})")
+    if start.dim() != 1:
+        _fail(f"start must be [B] (got {tuple(start.shape)})")
+    B = start.shape[0]
+    _expect(start, "start", (B,), torch.int32)
+    if (ok := B >= 1) is not True:
+        _check(ok, lambda: "start must have at least one sequence")
+    _validate_bounds(cu, T, B)
+    if positions is not None:
+        _expect(positions, "positions", (T,), torch.int32)
+    if block_table.dim() != 2:
+        _fail(f"block_table must be [B={B}, max_pages] (got {tuple(block_table.shape)})")
+    _expect(block_table, "block_table", (B, block_table.shape[1]), torch.int32)
+    if kp.dim() != 4:
+        _fail(f"k_pages must be [num_pages, Hkv, page_rows, row] (got {tuple(kp.shape)})")
+    num_pages, _, page_rows, _ = kp.shape
+    if fmt == "b8+":
+        _block_pools(kp, vp, ksp, vsp, num_pages, Hkv, page_rows, D, group)
+    else:
+        f = _fmt(fmt)
+        _check_dg(f, D, group)
+        _check_kv(f, kp, vp, ksp, vsp, (num_pages, Hkv, page_rows), D, group)
+
+
+def _append_rope_fake(q, k, v, inv_freq, cu_seqlens, start, positions, block_table, k_pages, v_pages, k_scale_pages, v_scale_pages, fmt,
+                      group=32, interleaved=False, rotated_k=False, scaling=1.0):
+    _validate_rope(q, k, v, inv_freq, cu_seqlens, start, positions, block_table, k_pages, v_pages, k_scale_pages, v_scale_pages, fmt, group)
+    return q.new_empty(q.shape), k.new_empty(k.shape if rotated_k else (0,) + k.shape[1:])
+
+
+@_op("append_rope(Tensor q, Tensor k, Tensor v, Tensor inv_freq, Tensor? cu_seqlens, Tensor start, Tensor? positions, Tensor block_table, "
+     "Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scale_pages, Tensor(d!)? v_scale_pages, str fmt, int group=32, "
+     "bool interleaved=False, bool rotated_k=False, float scaling=1.0) -> (Tensor, Tensor)", _append_rope_fake, computes=True)
+def append_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor, cu_seqlens: Optional[torch.Tensor],
+                start: torch.Tensor, positions: Optional[torch.Tensor], block_table: torch.Tensor, k_pages: torch.Tensor,
+                v_pages: torch.Tensor, k_scale_pages: Optional[torch.Tensor], v_scale_pages: Optional[torch.Tensor], fmt: str,
+                group: int = 32, interleaved: bool = False, rotated_k: bool = False,
+                scaling: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """q fp16 [T, Hq, D], k and v [T, Hkv, D], dense in D only (slices of a fused projection); rows cu_seqlens[b] ..
+    cu_seqlens[b+1] - 1 (None: row b) are sequence b's, written at positions start[b] on. q and k are rotated by
+    inv_freq fp32 [rot / 2] times their cache position, or positions int32 [T]; dimensions i and i + rot/2 are a pair
+    (interleaved: 2i and 2i + 1). fmt: any; "b8+": pages float8_e4m3fn [num_pages, Hkv, page_rows, D], scales fp16
+    [num_pages, Hkv, page_rows / group]. Returns q [T, Hq, D] and, if rotated_k, k [T, Hkv, D] (else [0, Hkv, D])."""
+    _validate_rope(q, k, v, inv_freq, cu_seqlens, start, positions, block_table, k_pages, v_pages, k_scale_pages, v_scale_pages, fmt, group)
+    stream = _on_device(q, k, v, inv_freq, cu_seqlens, start, positions, block_table, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    _contiguous(inv_freq, cu_seqlens, start, positions, block_table, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    q_out = torch.empty((T, Hq, D), dtype=torch.float16, device=q.device)
+    k_out = torch.empty((T if rotated_k else 0, Hkv, D), dtype=torch.float16, device=q.device)
+    if T == 0:
+        return q_out, k_out
+    num_pages, _, page_rows, _ = k_pages.shape
+    shape = _RopeShape(start.shape[0], T, Hq, Hkv, D, group, page_rows, block_table.shape[1], num_pages, 2 * inv_freq.shape[0],
+                       interleaved, scaling, *_strides("q", q), *_strides("k", k), *_strides("v", v))
+    b = _RopeBufs(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(cu_seqlens), start.data_ptr(), _ptr(positions), block_table.data_ptr(),
+                  inv_freq.data_ptr(), q_out.data_ptr(), k_out.data_ptr() if rotated_k else None, k_pages.data_ptr(), v_pages.data_ptr(),
+                  _ptr(k_scale_pages), _ptr(v_scale_pages))
+    check(lib.va_append_rope(B8 if fmt == "b8+" else int(_fmt(fmt)), C.byref(b), C.byref(shape), stream))
+    _changed((k_pages, v_pages) if k_scale_pages is None else (k_pages, v_pages, k_scale_pages, v_scale_pages))
+    return q_out, k_out
+
+
+def _validate_attend(q, kp, vp, ksp, vsp, block_table, cu, seq_lens, fmt: str, group: int) -> None:
+    if fmt != "b8+":
+        _fail(f"attend_paged takes the format b8+ only (got {fmt!r})")
+    if q.dim() != 3:
+        _fail(f"q must be [T, Hq, D] (got {tuple(q.shape)})")
+    T, Hq, D = q.shape
+    _expect(q, "q", (T, Hq, D), torch.float16)
+    if (ok := (D == 64) | (D == 128)) is not True:
+        _check(ok, lambda: f"D must be 64 or 128 (got {D})")
+    if kp.dim() != 4:
+        _fail(f"k_pages must be [num_pages, Hkv, page_rows, D] (got {tuple(kp.shape)})")
+    num_pages, Hkv, page_rows, _ = kp.shape
+    if (ok := (Hkv >= 1) & (Hq >= 1)) is not True:
+        _check(ok, lambda: f"q and k_pages must have at least one head (got {Hq} and {Hkv})")
+    if (ok := Hq % Hkv == 0) is not True:
+        _check(ok, lambda: f"query heads ({Hq}) must be a multiple of K/V heads ({Hkv})")
+    _block_pools(kp, vp, ksp, vsp, num_pages, Hkv, page_rows, D, group)
+    if block_table.dim() != 2:
+        _fail(f"block_table must be [B, max_pages] (got {tuple(block_table.shape)})")
+    B = block_table.shape[0]
+    _expect(block_table, "block_table", (B, block_table.shape[1]), torch.int32)
+    _expect(seq_lens, "seq_lens", (B,), torch.int32)
+    _validate_bounds(cu, T, B)
+
+
+def _attend_paged_fake(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, cu_seqlens, seq_lens, fmt, max_seq_len, group=32):
+    _validate_attend(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, cu_seqlens, seq_lens, fmt, group)
+    return q.new_empty(q.shape)
+
+
+@_op("attend_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scale_pages, Tensor v_scale_pages, Tensor block_table, "
+     "Tensor? cu_seqlens, Tensor seq_lens, str fmt, SymInt max_seq_len, int group=32) -> Tensor", _attend_paged_fake)
+def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: torch.Tensor, v_scale_pages: torch.Tensor,
+                 block_table: torch.Tensor, cu_seqlens: Optional[torch.Tensor], seq_lens: torch.Tensor, fmt: str, max_seq_len: int,
+                 group: int = 32) -> torch.Tensor:
+    """q fp16 [T, Hq, D], the newest tokens of every sequence, whose rows are in the cache already: rows cu_seqlens[b] ..
+    cu_seqlens[b+1] - 1 (int32 [B + 1]; None: row b) are the last of sequence b's seq_lens[b] positions; each attends
+    the positions up to its own. fmt "b8+": pages float8_e4m3fn [num_pages, Hkv, page_rows, D], scales fp16
+    [num_pages, Hkv, page_rows / group]. max_seq_len >= every length."""
+    _validate_attend(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, cu_seqlens, seq_lens, fmt, group)
+    stream = _ready(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, cu_seqlens, seq_lens)
+    T, Hq, D = q.shape
+    num_pages, Hkv, page_rows, _ = k_pages.shape
+    shape = _PagedShape(block_table.shape[0], Hq, Hkv, D, group, page_rows, block_table.shape[1], num_pages, max_seq_len)
+    out = torch.empty_like(q)
+    ws = torch.empty(lib.va_attend_ws_bytes(B8, C.byref(shape), T) // 4, dtype=torch.float32, device=q.device)
+    b = _AttendBufs(k_pages.data_ptr(), v_pages.data_ptr(), k_scale_pages.data_ptr(), v_scale_pages.data_ptr(), block_table.data_ptr(),
+                    _ptr(cu_seqlens), seq_lens.data_ptr(), q.data_ptr(), out.data_ptr(), ws.data_ptr())
+    check(lib.va_attend_paged(B8, C.byref(b), C.byref(shape), T, stream))
+    return out
 
 
 def row_format_bits(fmt: str) -> int:
