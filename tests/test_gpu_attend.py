@@ -87,6 +87,43 @@ def test_new_tokens(n, D, G):
         c.check(c.run(), what=(Hq, Hkv))
 
 
+@pytest.mark.parametrize("D,G", [(64, 64), (128, 32), (128, 64)])
+@pytest.mark.parametrize("lens,new", [([700, 800], [700, 520]), ([513], [512]), ([3000, 900], [257, 900]), ([1100, 70], [1090, 1])])
+def test_long_chunks(D, G, lens, new):
+    """Blocks of 256 rows, whole and in part."""
+    c = Case(lens, new, 16, 2, D, G, 128, seed=sum(new))
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_long_chunks_with_values_that_are_not_finite(which):
+    """NaN codes, a page outside the pool and an infinite scale among the new rows of blocks of 256 rows."""
+    c = Case([800], [700], 8, 1, 128, 32, 64, seed=20)
+    want = c.run()
+    sees = 100 + torch.arange(700, device="cuda")
+    page = c.host[0][6]                                          # positions 384 .. 447
+    c.pools[which].view(torch.uint8)[page, 0, 7, 9] = 0x7F
+    got = c.run()
+    bad = sees >= 391
+    assert torch.equal(got[~bad], want[~bad])
+    assert (got[bad][..., 9] if which else got[bad]).isnan().all()
+    if which:
+        got[..., 9] = want[..., 9]
+        assert torch.equal(got, want)
+    c.pools[which].view(torch.uint8)[page, 0, 7, 9] = 0
+    want = c.run()
+    c.scales[which][page, 0, 1] = math.inf
+    got = c.run()
+    bad = sees >= 416
+    assert torch.equal(got[~bad], want[~bad]) and got[bad].isnan().all()
+    c.scales[which][page, 0, 1] = 1.0
+    table = c.table.clone()
+    table[0, 9] = c.pages
+    got = c.run(table=table)
+    bad = sees >= 576
+    assert got[bad].isnan().all() and got[~bad].isfinite().all()
+
+
 @pytest.mark.parametrize("G", [32, 64])
 @pytest.mark.parametrize("lens,new", [
     ([300, 5, 1000, 77, 1], [1, 5, 130, 0, 1]),                  # whole prompts, chunks, none, single tokens

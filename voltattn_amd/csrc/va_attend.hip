@@ -4,14 +4,12 @@
 
 namespace va {
 
-constexpr int few_rows(int form) { return form; }
-
 AttendForm attend_form(int D, int B, int total, int hkv, int group, int cap, int cus) {
     (void)D;
     AttendForm f;
     const double mean = (double)total * group / B;
-    f.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
-    const long long bn = f.rows == 128 ? 64 : 128;
+    f.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 2048 ? 128 : 256;
+    const long long bn = f.rows >= 128 ? 64 : 128;
     // every sequence's last block may be a part, as may the rows before the first and behind the last one
     const long long blocks = std::min((long long)total * group, (long long)total * group / f.rows + B + 2) * hkv;
     f.tiles = blocks * std::max(1LL, (cap + bn - 1) / bn);
@@ -37,7 +35,8 @@ static hipError_t launch(const AttendArgs& a, hipStream_t stream) {
     } while (0)
     if (a.form == 16) VA_ATTEND((attend_few<D, G, 1>), 16, 128, 4);
     else if (a.form == 32) VA_ATTEND((attend_few<D, G, 2>), 32, 128, 4);
-    else VA_ATTEND((attend_wide<D, G>), 128, 64, 1);
+    else if (a.form == 128) VA_ATTEND((attend_wide<D, G, 1>), 128, 64, 1);
+    else VA_ATTEND((attend_wide<D, G, 2>), 256, 64, 1);
 #undef VA_ATTEND
     return e;
 }

@@ -42,6 +42,24 @@ struct AttendBlock {
     int first, tiles;     // its first tile in the numbering, how many
 };
 
+// The lane's (thread's) number, made anew: what is computed from it is not held across loops.
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// Constants that are not held in registers across loops either.
+__device__ __forceinline__ float local_nan() {
+    float x;
+    asm volatile("v_mov_b32 %0, 0x7fc00000" : "=v"(x));
+    return x;
+}
+__device__ __forceinline__ float local_minus_inf() {
+    float x;
+    asm volatile("v_mov_b32 %0, 0xff800000" : "=v"(x));
+    return x;
+}
+
 // The numbering, by one wave: lane i has span from + i of the current 64.
 template <int BM, int BN> struct AttendPlan {
     const AttendArgs& a;
@@ -60,7 +78,7 @@ template <int BM, int BN> struct AttendPlan {
     }
     __device__ __forceinline__ void load(int at, int before, int bound) {
         from = at;
-        const int i = at + (int)__lane_id();
+        const int i = at + (fresh((int)threadIdx.x) & 63);
         if (a.cu) {
             int e = i <= a.B ? a.cu[i] : a.total;
             e = max(0, min(e, a.total));
@@ -107,7 +125,7 @@ template <int BM, int BN> struct AttendPlan {
         b.hk = (at - b.s.first) / per;
         int in = at - b.s.first - b.hk * per;
         for (int r0 = 0;; r0 += 64) {
-            const int rb = r0 + (int)__lane_id();
+            const int rb = r0 + (fresh((int)threadIdx.x) & 63);
             const int t = rb < nb ? tiles(b.s.seq, b.s.n, b.s.len, rb) : 0;
             const int up = wave_scan(t), all = __builtin_amdgcn_readlane(up, 63);
             if (in < all) {
@@ -133,7 +151,7 @@ template <int STEP, int G> struct Places {
     // at: position of tile `first`'s part, `stride` positions from tile to tile; those from `end` on are not looked at
     __device__ __forceinline__ void load(const AttendArgs& a, const int32_t* table, int hk, int tile, int tiles, int stride, int off, int end) {
         base = tile;
-        const int t = tile + (int)__lane_id();
+        const int t = tile + (fresh((int)threadIdx.x) & 63);
         const long long j64 = (long long)t * stride + off;
         const bool on = t < tiles && j64 < end;
         const int j = on ? (int)j64 : 0;
@@ -154,10 +172,11 @@ template <int STEP, int G> struct Places {
 };
 
 // A tile's part under one pair of scales, all uniform: K's scale times the scores' factor, V's
-// scale as 2^e times `more` in [1, 2), and whether the part has no finite values (a page outside
-// the pool, a scale that is infinite or NaN): rows that see it are NaN.
+// scale as 2^(e + more), 0 <= more < 1, and whether the part has no finite values (a page outside
+// the pool, a scale that is infinite or NaN): rows that see it are NaN. `more` goes into the
+// exponent of the weights, and what it adds to their sum is taken out with less = 2^-more.
 struct Scales {
-    float qs, more;
+    float qs, more, less;
     int e;                // NONE: V's scale is 0
     bool bad;
     static constexpr int NONE = -1000;
@@ -165,12 +184,24 @@ struct Scales {
         sk &= 0x7FFFu;
         sv &= 0x7FFFu;
         bad = !there || sk >= 0x7C00u || sv >= 0x7C00u;
+        const uint32_t k = bad ? 0u : wide_bits(sk), v = bad ? 0u : wide_bits(sv);
         // a hidden position's score is -infinity, which a factor of 0 would make NaN
-        const float k = uniformf(h2f(bad ? 0u : sk)), v = uniformf(h2f(bad ? 0u : sv));
-        qs = k > 0.f ? qscale * k : 0x1p-100f;
-        const uint32_t b = __builtin_bit_cast(uint32_t, v);
-        e = b ? (int)(b >> 23) - 127 : NONE;
-        more = b ? __builtin_bit_cast(float, (b & 0x7FFFFFu) | 0x3F800000u) : 1.f;
+        qs = uniformf(qscale * __builtin_bit_cast(float, k ? k : 0x0D800000u));      // 2^-100
+        e = v ? (int)(v >> 23) - 127 : NONE;
+        more = 0.f;
+        less = 1.f;
+        if (v & 0x7FFFFFu) {                     // no power of two
+            const float x = __builtin_bit_cast(float, (v & 0x7FFFFFu) | 0x3F800000u);
+            more = uniformf(__builtin_amdgcn_logf(x));
+            less = uniformf(1.f / x);
+        }
+    }
+    // The bits of a finite fp16 number's fp32 value, on the scalar unit.
+    static __device__ __forceinline__ uint32_t wide_bits(uint32_t h) {
+        if (h >= 0x400u) return (h << 13) + (112u << 23);
+        if (h == 0) return 0;
+        const int p = 31 - __builtin_clz(h);     // h 2^-24, its highest bit 2^p
+        return ((uint32_t)(p + 103) << 23) + ((h << (23 - p)) & 0x7FFFFFu);
     }
 };
 __device__ __forceinline__ float power(int e) { return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23); }   // -126 <= e <= 127
@@ -192,12 +223,13 @@ __device__ __forceinline__ int unit_for(Scales (&s)[2], int unit) {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
         if (s[b].e != Scales::NONE && s[b].e < u - 15) {
-            s[b].more *= power(s[b].e - u + 15);
+            s[b].more += (float)(s[b].e - u + 15);
+            s[b].less *= power(u - 15 - s[b].e);
             s[b].e = u - 15;
         }
     return u;
 }
-__device__ __forceinline__ float factor_of(const Scales& s, int unit) { return s.e == Scales::NONE ? 0x1p-120f : power(s.e - unit); }
+__device__ __forceinline__ float factor_of(const Scales& s, int unit) { return power(s.e == Scales::NONE ? -120 : s.e - unit); }
 
 // Four codes as fp16, times the power of two f.
 __device__ __forceinline__ void codes_to_f16(uint32_t w, float f, f16x2& a, f16x2& b) {
@@ -223,18 +255,17 @@ __device__ __forceinline__ bool codes_clean(u32x4& w) {
     }
     return any != 0;
 }
-// NaN where one of the codes c .. c + 3 of position j's V row is NaN, else 0.
+// Which of the codes c .. c + 3 of position j's V row are NaN, a bit to each.
 template <int D>
-__device__ __forceinline__ f32x4 attend_odd(const AttendArgs& a, const int32_t* table, int hk, int j, int c) {
-    f32x4 x = {};
+__device__ __forceinline__ uint32_t attend_odd(const AttendArgs& a, const int32_t* table, int hk, int j, int c) {
     const int page = table[j >> a.page_shift];
-    if (page < 0 || page >= a.num_pages) return x;
+    if (page < 0 || page >= a.num_pages) return 0;
     const size_t r = (((size_t)page * a.hkv + hk) << a.page_shift) + (size_t)(j & ((1 << a.page_shift) - 1));
     const uint32_t w = *reinterpret_cast<const uint32_t*>(a.v + r * D + c);
+    uint32_t nan = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (((w >> (8 * e)) & 0x7Fu) == 0x7Fu) x[e] = __builtin_nanf("");
-    return x;
+    for (int e = 0; e < 4; ++e) nan |= (((w >> (8 * e)) & 0x7Fu) == 0x7Fu ? 1u : 0u) << e;
+    return nan;
 }
 
 // The lazy maximum, as WIDE_OFF and WIDE_SLACK, with room for the part of V's scale below 2.
@@ -275,12 +306,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
     int at = wg * share;
     const int end = min(plan.total, at + share);
 
-    // the thread's number, made anew: what is computed from it is not held across loops
-    auto fresh_lane = [&]() {
-        int x = lane;
-        asm volatile("" : "+v"(x));
-        return x;
-    };
+    auto fresh_lane = [&]() { return fresh(lane); };
     while (at < end) {
         const AttendBlock blk = plan.find(at);
         const int hk = uniform(blk.hk), rb = uniform(blk.rb), n = uniform(blk.s.n), begin = uniform(blk.s.begin), seq = uniform(blk.s.seq);
@@ -289,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
         at += t1 - t0;
         if (seq < 0 || blk.s.bad(a.cap)) {
             const float x = seq < 0 ? 0.f : __builtin_nanf("");
-            for (int i = tid; i < BM * (D / 8); i += 256) {
+            for (int i = fresh(tid); i < BM * (D / 8); i += 256) {
                 const int r = rb * BM + i / (D / 8);
                 if (r >= rows) break;
                 const int tok = (int)a.by_group.div((uint32_t)r);
@@ -423,13 +449,15 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
             f16x8 p[NB];
 #pragma unroll
             for (int y = 0; y < NB; ++y) {
-                const float base = m[y] == -__builtin_inff() ? 0.f : m[y];
+                const float up = s.more - (m[y] == -__builtin_inff() ? 0.f : m[y]);
+                float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float w = fast_exp2(__builtin_fmaf(x[e / 4][y][e % 4], s.qs, -base));
-                    l[y] += w;
-                    p[y][e] = (_Float16)(w * s.more);
+                    const float w = fast_exp2(__builtin_fmaf(x[e / 4][y][e % 4], s.qs, up));
+                    sum += w;
+                    p[y][e] = (_Float16)w;
                 }
+                l[y] = __builtin_fmaf(sum, s.less, l[y]);
             }
             const float f = factor_of(s, unit);
 #pragma unroll
@@ -485,9 +513,12 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
                     for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(f, z[e], x[e]);
                 }
                 const int tok = (int)a.by_group.div((uint32_t)to);
-                if (*odd)                                    // NaN codes that were left out, to the rows that see them
-                    for (int j = max(t0 * BN, all + 1 - BN); j <= min(ctx + tok, t1 * BN - 1); ++j)
-                        if (j >= 0) x += attend_odd<D>(a, table, hk, j, c);
+                if (*odd) {                                  // NaN codes that were left out, to the rows that see them
+                    uint32_t nan = 0;
+                    for (int j = max(max(t0 * BN, all + 1 - BN), 0); j <= min(ctx + tok, t1 * BN - 1); ++j) nan |= attend_odd<D>(a, table, hk, j, c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = nan >> e & 1 ? __builtin_nanf("") : x[e];
+                }
                 if (whole) {
                     const float inv = ll == 0.f ? 0.f : 1.f / ll;
                     f16x4 w;
@@ -506,60 +537,172 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
 }
 
 // ----------------------------------------------------------------- many rows --
-// The weights of two parts of 32 positions; qs, more: of each.
-template <int D>
-__device__ __forceinline__ void attend_weights(const f32x16 (&s)[2], const Scales (&sc)[2], int to_unit, int& unit, float& m, float& l, f32x16 (&o)[D / 32], f16x8 (&p)[2][2]) {
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        float x = s[b][0];
-#pragma unroll
-        for (int v = 1; v < 16; ++v) x = fmaxf(x, s[b][v]);
-        top = fmaxf(top, x * sc[b].qs);
-    }
-    top = halves_max(top);
-    if (__any(top - m > ATT_OFF + ATT_SLACK) || to_unit != unit) {   // also at the first one: m = -inf
-        const float to = fmaxf(m, top - ATT_OFF), f = to == m ? 1.f : fast_exp2(m - to);
-        m = to;
-        l *= f;
-        const float g = f * power(unit - to_unit);
-        unit = to_unit;
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db) o[db] *= g;
-    }
-    const float base = m == -__builtin_inff() ? 0.f : m;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const float e = fast_exp2(__builtin_fmaf(s[b][v], sc[b].qs, -base));
-            l += e;
-            p[b][v / 8][v % 8] = (_Float16)(e * sc[b].more);
-        }
+// Block: 128 CB rows, 32 CB to a wave as the columns of 32x32x16 products (S^T = K Q^T, O^T = V^T P^T,
+// lane layout as in va_wide.hpp). A tile of 64 positions comes straight to LDS as codes (16 KB of K and
+// V) while its predecessor is computed, and every wave turns them into fp16 as it reads its operands.
+// K: a lane reads 16 codes of its row, two steps' worth (chunk 2j + half: the k index is a free
+// permutation, q is laid out likewise). V: ds_read_b64_tr_b8, the slots of wide_values' positions.
+// The 16-byte chunks of a row lie XORed with wide_swz_k / wide_swz_v, so that neither read meets a
+// bank twice. CB = 2: every operand, once converted, feeds two products; more than half of the wave's
+// query operands wait in LDS (step by step, 16 bytes of each lane), which its registers do not hold
+// beside the sums of 64 rows.
+//
+// A wave's products go before the other waves' weights (s_setprio): they need the issue port for a
+// moment each and the matrix cores for long; without it the oldest wave of a SIMD goes first, the
+// others fall behind, and the last work-groups of a CU finish alone.
+//
+// A lane has two score blocks of 32 positions at a time: both halves of a tile against one row (CB =
+// 1), or one half against a row of each group (CB = 2).
+template <int D> __device__ __forceinline__ int wide_swz_k(int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+template <int D> __device__ __forceinline__ int wide_swz_v(int row) {
+    return D == 128 ? ((row >> 1) & 1) << 1 | ((row >> 3) & 1) << 2 : ((row >> 3) & 1) << 1;
 }
 
-// Block: 128 rows, 32 to a wave as the columns of va_wide.hpp's tiles. A tile of 64 positions comes
-// to LDS as codes while its predecessor is computed (16 KB of K and V, each wave a quarter), and every
-// wave turns what it fetched into fp16 rows that all four read.
-template <int D, int G>
-__global__ __launch_bounds__(256, 3) void attend_wide(AttendArgs a) {
-    constexpr int BM = 128, BN = 64, KS = D / 16, DB = D / 32, TILE = BN * 2 * D, RAW = BN * D, N = RAW / 4096;
-    __shared__ __align__(1024) uint8_t lds[2 * TILE + 2 * RAW + 16];
+// Steps whose query operands of the first group are in registers.
+constexpr int wide_steps(int D, int CB) { return CB == 2 && D == 128 ? 5 : D / 16; }
+
+// S^T; at: the tile's K (CB = 2: the half's); q2: this lane's query operands in LDS, the first group's
+// that are not in registers, and the second group's.
+// The next step's reads are on their way while a step's codes are converted and multiplied.
+template <int D, int CB>
+__device__ __forceinline__ void wide_keys(const lds_u8* k, uint32_t at, const f16x8 (&q)[wide_steps(D, CB)], const lds_u8* q2, f32x16 (&s)[2]) {
+    s[0] = s[1] = f32x16{};
+    if constexpr (CB == 1) {
+        u32x4 w[2][2];
+        auto read = [&](int j) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) w[j & 1][b] = *reinterpret_cast<const lds_u32x4*>(k + (at ^ (uint32_t)(j << 5)) + b * 32 * D);
+        };
+        read(0);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (j + 1 < D / 32) read(j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) s[b] = mfma_32x32x16(codes_to_f16x8(w[j & 1][b][2 * x], w[j & 1][b][2 * x + 1], 1.f), q[2 * j + x], s[b]);
+        }
+    } else {
+        constexpr int KS = D / 16, QR = wide_steps(D, CB);
+        u32x4 w[2];
+        f16x8 z[2][2];
+        auto read_k = [&](int j) { w[j & 1] = *reinterpret_cast<const lds_u32x4*>(k + (at ^ (uint32_t)(j << 5))); };
+        auto read_q = [&](int i) {
+            z[i & 1][1] = lds_row8(q2, (uint32_t)((KS - QR + i) * 1024));
+            if (i >= QR) z[i & 1][0] = lds_row8(q2, (uint32_t)((i - QR) * 1024));
+        };
+        read_k(0);
+        read_q(0);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i % 2 == 0 && i / 2 + 1 < KS / 2) read_k(i / 2 + 1);
+            if (i + 1 < KS) read_q(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const f16x8 y = codes_to_f16x8(w[(i >> 1) & 1][2 * (i & 1)], w[(i >> 1) & 1][2 * (i & 1) + 1], 1.f);
+            s[0] = mfma_32x32x16(y, i < QR ? q[i < QR ? i : 0] : z[i & 1][0], s[0]);
+            s[1] = mfma_32x32x16(y, z[i & 1][1], s[1]);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+// O^T += V^T P^T; at: the tile's V (CB = 2: the half's); f: what the blocks' codes are multiplied by.
+template <int D, int CB>
+__device__ __forceinline__ void wide_sums(lds_u8* v, uint32_t at, const float (&f)[2], const f16x8 (&p)[2][2], f32x16 (&o)[CB][D / 32]) {
+    constexpr int DB = D / 32, N = 4 / CB;                   // 16 positions to a step
+    i32x2 w[2][DB];
+    auto read = [&](int i) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+            w[i & 1][db] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<lds_i32x2*>(v + (at ^ (uint32_t)(db << 5)) + i * 16 * D));
+    };
+    read(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + 1 < N) read(i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            const f16x8 y = codes_to_f16x8((uint32_t)w[i & 1][db].x, (uint32_t)w[i & 1][db].y, f[CB == 1 ? i >> 1 : 0]);
+            o[0][db] = mfma_32x32x16(y, p[CB == 1 ? i >> 1 : 0][i & 1], o[0][db]);
+            if constexpr (CB == 2) o[1][db] = mfma_32x32x16(y, p[1][i & 1], o[1][db]);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+// The weights of two score blocks: of one row under the scales sc[0] and sc[1] (CB = 1), or of two rows
+// under sc[0]. The maxima and the unit of the sums follow where they have to.
+template <int D, int CB>
+__device__ __forceinline__ void wide_softmax(const f32x16 (&s)[2], const Scales* sc, int to_unit, int& unit, float (&m)[CB], float (&l)[CB],
+                                             f32x16 (&o)[CB][D / 32], f16x8 (&p)[2][2]) {
+    float top[CB];
+#pragma unroll
+    for (int c = 0; c < CB; ++c) top[c] = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float x = s[i][0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) x = fmaxf(x, s[i][v]);
+        const int c = CB == 1 ? 0 : i;
+        top[c] = fmaxf(top[c], x * sc[CB == 1 ? i : 0].qs);
+    }
+    bool grows = false;
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+        top[c] = halves_max(top[c]);
+        grows |= top[c] - m[c] > ATT_OFF + ATT_SLACK;        // also at the first one: m = -inf
+    }
+    if (__any(grows) || to_unit != unit) {
+        const float u = power(unit - to_unit);
+        unit = to_unit;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+            const float to = fmaxf(m[c], top[c] - ATT_OFF), f = to == m[c] ? 1.f : fast_exp2(m[c] - to);
+            m[c] = to;
+            l[c] *= f;
+            const float g = f * u;
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db) o[c][db] *= g;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = CB == 1 ? 0 : i;
+        const Scales& x = sc[CB == 1 ? i : 0];
+        const float up = x.more - (m[c] == -__builtin_inff() ? 0.f : m[c]);
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const float w = fast_exp2(__builtin_fmaf(s[i][v], x.qs, up));
+            sum += w;
+            p[i][v / 8][v % 8] = (_Float16)w;
+        }
+        l[c] = __builtin_fmaf(sum, x.less, l[c]);
+    }
+}
+
+template <int D, int G, int CB>
+__global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a) {
+    constexpr int BM = 128 * CB, BN = 64, KS = D / 16, DB = D / 32, RAW = BN * D, N = RAW / 4096;
+    constexpr int QR = wide_steps(D, CB), QB = (CB * KS - QR) * 1024;   // bytes of a wave's query operands in LDS
+    __shared__ __align__(1024) uint8_t lds[4 * RAW + 4 * QB];   // K of two tiles, V of two
     lds_u8* kt = (lds_u8*)lds;
-    lds_u8* vt = kt + TILE;
-    lds_u8* rk = vt + TILE;
-    lds_u8* rv = rk + RAW;
-    lds_int* odd = (lds_int*)(rv + RAW);
+    lds_u8* vt = kt + 2 * RAW;
 
     const int tid = (int)threadIdx.x, wave = uniform(tid >> 6);
-    if (tid == 0) *odd = 0;
-    WideAddr<D> ad0;
-    ad0.init(tid & 63);
-    // the lane, made anew: what is computed from it is not held across loops
-    auto fresh_lane = [&]() {
-        int x = tid & 63;
-        asm volatile("" : "+v"(x));
-        return x;
+    lds_u8* q2 = vt + 2 * RAW + wave * QB;
+    auto fresh_lane = [&]() { return fresh(tid) & 63; };
+    // addresses of the lane's operands in a tile, and in q2
+    auto key_at = [&](int tile) {
+        const int x = fresh_lane(), row = x & 31;
+        return (uint32_t)(tile + row * D + (((x >> 5) ^ wide_swz_k<D>(row)) << 4));
+    };
+    auto value_at = [&](int tile) {
+        const int x = fresh_lane(), e = (x & 15) >> 1, pos = 4 * (x >> 5) + (e & 3) + 8 * (e >> 2);
+        return (uint32_t)(tile + pos * D + ((((x >> 4) & 1) ^ wide_swz_v<D>(pos)) << 4) + (x & 1) * 8);
     };
     int at = 0, end = 0, wg = 0;
     do {
@@ -582,7 +725,7 @@ __global__ __launch_bounds__(256, 3) void attend_wide(AttendArgs a) {
         at += t1 - t0;
         if (seq < 0 || blk.s.bad(a.cap)) {
             const float x = seq < 0 ? 0.f : __builtin_nanf("");
-            for (int i = tid; i < BM * (D / 8); i += 256) {
+            for (int i = fresh(tid); i < BM * (D / 8); i += 256) {
                 const int r = rb * BM + i / (D / 8);
                 if (r >= rows) break;
                 const int tok = (int)a.by_group.div((uint32_t)r);
@@ -592,134 +735,162 @@ __global__ __launch_bounds__(256, 3) void attend_wide(AttendArgs a) {
         }
         const int ctx = len - n;
         const int32_t* table = a.block_table + (size_t)seq * a.max_pages;
-        // the lane's row of the block
-        auto row_of = [&](int& half, int& row, int& rc, int& tok) {
+        // the wave's rows; the work-groups of a CU begin with different waves, so that the few rows of
+        // short blocks do not all meet on one SIMD
+        const int row0 = uniform(rb * BM + ((wave + (int)(blockIdx.x >> 8)) & 3) * CB * 32);
+        // the lane's row of the block in the wave's group c
+        auto row_of = [&](int c, int& half, int& row, int& rc, int& tok) {
             const int x = fresh_lane();
             half = x >> 5;
-            row = rb * BM + wave * 32 + (x & 31);
+            row = row0 + c * 32 + (x & 31);
             rc = min(row, rows - 1);
             tok = (int)a.by_group.div((uint32_t)rc);
         };
         const int all = ctx + (int)a.by_group.div((uint32_t)(rb * BM));                                       // that every row of the block sees
-        const int mine = ctx + (int)a.by_group.div((uint32_t)min(rb * BM + wave * 32, rows - 1));             // .. of the wave
-        f16x8 q[KS];
-        {
-            int half, row, rc, tok;
-            row_of(half, row, rc, tok);
-            const uint16_t* qp = a.q + ((size_t)(begin + tok) * hq + hk * a.group + (rc - tok * a.group)) * D + 8 * half;
+        const int mine = ctx + (int)a.by_group.div((uint32_t)min(row0, rows - 1));                            // .. of the wave
+        const int most = row0 < rows ? ctx + (int)a.by_group.div((uint32_t)min(row0 + CB * 32, rows) - 1u) : -1;   // that some row of the wave sees
+        f16x8 q[QR];
 #pragma unroll
-            for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const f16x8*>(qp + 16 * s);
+        for (int c = CB - 1; c >= 0; --c) {
+            int half, row, rc, tok;
+            row_of(c, half, row, rc, tok);
+            const uint16_t* qp = a.q + ((size_t)(begin + tok) * hq + hk * a.group + (rc - tok * a.group)) * D + 16 * half;
+            lds_u8* to = q2 + fresh_lane() * 16;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const f16x8 x = *reinterpret_cast<const f16x8*>(qp + (s >> 1) * 32 + (s & 1) * 8);
+                if (c == 0 && s < QR) q[s < QR ? s : 0] = x;
+                else *reinterpret_cast<lds_f16x8*>(to + (c == 1 ? KS - QR + s : s - QR) * 1024) = x;
+            }
         }
         Places<64, G> pl;
         uint32_t sk = 0, sv = 0;                             // of the tile that is fetched
         bool there = false;
-        auto fetch = [&](int t) {
+        auto fetch = [&](int t, int to) {
             if (pl.base < 0 || t >= pl.base + 64) pl.load(a, table, hk, t, t1, BN, 0, len);
             const int x = t - pl.base, page = __builtin_amdgcn_readlane(pl.page, x), j = t * BN;
             sk = (uint32_t)__builtin_amdgcn_readlane((int)pl.sk, x);
             sv = (uint32_t)__builtin_amdgcn_readlane((int)pl.sv, x);
             there = page >= 0;
-            const int left = there ? max(0, min(BN, len - j)) : 0;
-            const size_t r = uniform64((((size_t)(there ? page : 0) * a.hkv + hk) << a.page_shift) + (size_t)(j & ((1 << a.page_shift) - 1)));
-            const uint32_t bytes = (uint32_t)(uniform(left) * D);
-            const __amdgpu_buffer_rsrc_t k = make_rsrc(a.k + r * D, bytes), v = make_rsrc(a.v + r * D, bytes);
-            const int lane = fresh_lane();
+            const uint32_t bytes = (uint32_t)(there ? max(0, min(BN, len - j)) : 0) * D;
+            const size_t r = ((((size_t)(there ? page : 0) * a.hkv + hk) << a.page_shift) + (size_t)(j & ((1 << a.page_shift) - 1))) * D;
+            const __amdgpu_buffer_rsrc_t k = make_rsrc(a.k + uniform64(r), uniform((int)bytes)), v = make_rsrc(a.v + uniform64(r), uniform((int)bytes));
+            // the lane's place in LDS, and the chunk that belongs there; the next KB's is the same with another XOR
+            const int lane = fresh_lane(), off = wave * N * 1024, row = (off + lane * 16) / D, c = lane % (D / 16);
+            const uint32_t kc = (uint32_t)(row * D + ((c ^ wide_swz_k<D>(row)) << 4)), vc = (uint32_t)(row * D + ((c ^ wide_swz_v<D>(row)) << 4));
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const uint32_t off = (uint32_t)((wave * N + i) * 1024);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(k, rk + off, 16, off + (uint32_t)lane * 16u, 0, 0, 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(v, rv + off, 16, off + (uint32_t)lane * 16u, 0, 0, 0);
+                static_assert(D == 128 || N == 1, "1 KB is 8 rows: bit 2 of row >> 1, bit 0 of row >> 3");
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(k, kt + to + off + i * 1024, 16, (kc ^ (uint32_t)(i << 6)) + (uint32_t)(i * 1024), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(v, vt + to + off + i * 1024, 16, (vc ^ (uint32_t)(i << 6)) + (uint32_t)(i * 1024), 0, 0, 0);
             }
         };
-        f32x16 o[DB] = {};
-        float m = -__builtin_inff(), l = 0.f;
+        f32x16 o[CB][DB] = {};
+        float m[CB], l[CB];
+#pragma unroll
+        for (int c = 0; c < CB; ++c) {
+            m[c] = -__builtin_inff();
+            l[c] = 0.f;
+        }
         int unit = 0;
-        fetch(t0);
-        for (int t = t0; t < t1; ++t) {
-            Scales sc[2];
-            sc[0].set(sk & 0xFFFFu, sv & 0xFFFFu, a.qscale, there);
-            sc[1].set(sk >> 16, sv >> 16, a.qscale, there || t * BN + 32 >= len);
-            const int to_unit = unit_for(sc, unit);
-            const bool hides = t * BN + BN - 1 > all;
-            // what this wave fetched has arrived; every wave has read the last tile (or the last piece's flag)
+        bool odd = false;                                    // this wave has left out NaN codes
+        __syncthreads();                                     // the last piece's tiles are read
+        fetch(t0, 0);
+        // tile t is there, for every wave; its successor is on its way
+        auto arrive = [&](int t, int cur) {
             __builtin_amdgcn_sched_barrier(0);
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
-            {
-                const float f = wave < 2 ? factor_of(sc[0], to_unit) : factor_of(sc[1], to_unit);
-                const int lane = fresh_lane();
+            if (t * BN + BN - 1 > all) {                     // positions that some row of the block does not see
+                lds_u32x4* p = reinterpret_cast<lds_u32x4*>(vt + cur + wave * (N * 1024)) + fresh_lane();
                 bool any = false;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int off = (wave * N + i) * 1024 + lane * 16, r = off / D, c = off % D / 8;
-                    const int to0 = r * 2 * D + ((c ^ swz<D>(r)) << 4), to1 = r * 2 * D + (((c + 1) ^ swz<D>(r)) << 4);
-                    const u32x4 kw = *reinterpret_cast<lds_u32x4*>(rk + off);
-                    u32x4 vw = *reinterpret_cast<lds_u32x4*>(rv + off);
-                    *reinterpret_cast<lds_f16x8*>(kt + to0) = codes_to_f16x8(kw.x, kw.y, 1.f);
-                    *reinterpret_cast<lds_f16x8*>(kt + to1) = codes_to_f16x8(kw.z, kw.w, 1.f);
-                    if (hides) any |= codes_clean(vw);
-                    *reinterpret_cast<lds_f16x8*>(vt + to0) = codes_to_f16x8(vw.x, vw.y, f);
-                    *reinterpret_cast<lds_f16x8*>(vt + to1) = codes_to_f16x8(vw.z, vw.w, f);
+                    u32x4 w = p[i * 64];
+                    if (codes_clean(w)) {
+                        any = true;
+                        p[i * 64] = w;
+                    }
                 }
-                if (any) *odd = 1;
+                odd |= __any(any) != 0;
             }
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 1 < t1) fetch(t + 1);
-            const WideAddr<D> ad = ad0.fresh();
-            f32x16 s[2];
-            wide_scores<D, 2, 2, false>(kt, nullptr, ad, q, s);
-            if (sc[0].bad || sc[1].bad) {
+            if (t + 1 < t1) fetch(t + 1, cur ^ RAW);
+        };
+        const int tw = most < 0 ? t0 : max(t0, min(t1, most / BN + 1));   // tiles that this wave sees a part of
+        int t = t0, cur = 0;
+        for (; t < tw; ++t, cur ^= RAW) {
+            Scales sc[2];
+            sc[0].set(sk & 0xFFFFu, sv & 0xFFFFu, a.qscale, there);
+            sc[1].set(sk >> 16, sv >> 16, a.qscale, there || t * BN + 32 >= len);
+            const int to_unit = unit_for(sc, unit);
+            arrive(t, cur);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+            for (int h = 0; h < CB; ++h) {                   // CB = 2: half by half
+                f32x16 s[2];
+                __builtin_amdgcn_s_setprio(1);
+                wide_keys<D, CB>(kt, key_at(cur) + (uint32_t)(h * 32 * D), q, q2 + (QB ? fresh_lane() * 16 : 0), s);
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) s[b][v] = sc[b].bad ? __builtin_nanf("") : s[b][v];
+                for (int i = 0; i < 2; ++i)
+                    if (sc[CB == 1 ? i : h].bad) s[i] = f32x16(local_nan());
+                if (t * BN + BN - 1 > mine) {
+                    const float hidden = local_minus_inf();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        int half, row, rc, tok;
+                        row_of(CB == 1 ? 0 : i, half, row, rc, tok);
+                        const int lim = ctx + tok - t * BN - 32 * (CB == 1 ? i : h) - 4 * half;   // the last position that the row sees, from the lane's first one
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[i][v] = 8 * (v / 4) + v % 4 > lim ? hidden : s[i][v];
+                    }
+                }
+                f16x8 p[2][2];
+                __builtin_amdgcn_s_setprio(0);
+                wide_softmax<D, CB>(s, sc + (CB == 1 ? 0 : h), to_unit, unit, m, l, o, p);
+                __builtin_amdgcn_s_setprio(1);
+                const float f[2] = {factor_of(sc[CB == 1 ? 0 : h], unit), factor_of(sc[1], unit)};
+                wide_sums<D, CB>(vt, value_at(cur) + (uint32_t)(h * 32 * D), f, p, o);
             }
-            if (t * BN + BN - 1 > mine) {
-                int half, row, rc, tok;
-                row_of(half, row, rc, tok);
-                const int lim = ctx + tok - t * BN - 4 * half;   // the last position that the row sees, from the lane's first one
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) s[b][v] = 32 * b + 8 * (v / 4) + v % 4 > lim ? -__builtin_inff() : s[b][v];
-            }
-            f16x8 p[2][2];
-            attend_weights<D>(s, sc, to_unit, unit, m, l, o, p);
-            wide_values<D, 2>(vt, ad, p, o);
+            __builtin_amdgcn_s_setprio(0);
         }
-        l = halves_sum(l);
-        __syncthreads();                                     // the last tile is read, odd is whole
-        const bool whole = t0 == 0 && t1 == tiles, any = *odd != 0;
+        for (; t < t1; ++t, cur ^= RAW) arrive(t, cur);
+        const bool whole = t0 == 0 && t1 == tiles;
+        __syncthreads();                                     // the last tile is read
+        if ((fresh(tid) & 63) == 0) reinterpret_cast<lds_int*>(kt)[wave] = odd;
         __syncthreads();
-        if (tid == 0) *odd = 0;
+        bool any = false;                                    // some wave has
+#pragma unroll
+        for (int w = 0; w < 4; ++w) any |= uniform(reinterpret_cast<lds_int*>(kt)[w]) != 0;
         const float scale = power(unit);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] *= scale;
-        int half, row, rc, tok;
-        row_of(half, row, rc, tok);
-        const int last = ctx + tok;
-        if (row < rows) {
-            if (any)                                         // NaN codes that were left out, to the rows that see them
+        for (int c = 0; c < CB; ++c) {
+            const float lc = halves_sum(l[c]);
+            int half, row, rc, tok;
+            row_of(c, half, row, rc, tok);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[c][db] *= scale;
+            if (row >= rows) continue;
+            if (any) {                                       // NaN codes that were left out, to the rows that see them
+                uint64_t nan = 0;                            // of the lane's values, in order
 #pragma unroll 1
-                for (int j = max(max(t0 * BN, all + 1 - BN), 0); j <= min(last, t1 * BN - 1); ++j)
+                for (int j = max(max(t0 * BN, all + 1 - BN), 0); j <= min(ctx + tok, t1 * BN - 1); ++j)
+#pragma unroll 1
+                    for (int d = 0; d < D / 8; ++d) nan |= (uint64_t)attend_odd<D>(a, table, hk, j, 8 * d + 4 * half) << (4 * d);
 #pragma unroll
-                    for (int d = 0; d < D / 8; ++d) {
-                        const f32x4 x = attend_odd<D>(a, table, hk, j, 8 * d + 4 * half);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[d / 4][4 * (d % 4) + i] += x[i];
-                    }
+                for (int d = 0; d < D / 2; ++d) o[c][d / 16][d % 16] = nan >> d & 1 ? local_nan() : o[c][d / 16][d % 16];
+            }
             if (whole) {
                 uint16_t* out = a.out + ((size_t)(begin + tok) * hq + hk * a.group + (rc - tok * a.group)) * D + 4 * half;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = lc == 0.f ? 0.f : 1.f / lc;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         f16x4 w;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = (_Float16)(l == 0.f ? 0.f : o[db][4 * g + i] * inv);
+                        for (int i = 0; i < 4; ++i) w[i] = (_Float16)(lc == 0.f ? 0.f : o[c][db][4 * g + i] * inv);
                         *reinterpret_cast<f16x4*>(out + 32 * db + 8 * g) = w;
                     }
             } else {
@@ -729,8 +900,9 @@ __global__ __launch_bounds__(256, 3) void attend_wide(AttendArgs a) {
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
-                        *reinterpret_cast<f32x4*>(part + r * D + 32 * db + 8 * g + 4 * half) = f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-                if (half == 0) *reinterpret_cast<f32x2*>(part + BM * D + 2 * r) = f32x2{m, l};
+                        *reinterpret_cast<f32x4*>(part + r * D + 32 * db + 8 * g + 4 * half) =
+                            f32x4{o[c][db][4 * g], o[c][db][4 * g + 1], o[c][db][4 * g + 2], o[c][db][4 * g + 3]};
+                if (half == 0) *reinterpret_cast<f32x2*>(part + BM * D + 2 * r) = f32x2{m[c], lc};
             }
         }
     } while (at < end);

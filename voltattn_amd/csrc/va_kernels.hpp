@@ -260,7 +260,7 @@ struct AttendArgs {
     FastDiv by_group;
     int   nwg, form;              // of its AttendForm
 };
-// Rows to a block (16, 32: attend_few; 128: attend_wide), K/V tiles of the batch at most, and work-groups.
+// Rows to a block (16, 32: attend_few; 128, 256: attend_wide), K/V tiles of the batch at most, and work-groups.
 struct AttendForm {
     int rows;
     long long tiles, groups;
