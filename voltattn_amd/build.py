@@ -14,6 +14,8 @@
   (``va_runtime.hip``) with its host code built under AddressSanitizer and
   UndefinedBehaviorSanitizer (device code unchanged), for the CPU sanitizer
   run of ``tests/test_sanitizers.py``.
+* ``voltattn_amd/libvoltattn_torch.so`` — the PyTorch ops whose plain calls go to
+  the C ABI without Python (``host/torch_calls.cpp``, g++).
 * ``oracle/liboracle.so`` — the CPU checker (test infrastructure, g++).
 * ``build/voltattn`` — the C++ selftest/bench/probe harness (tests/cli), linked
   against both.
@@ -24,6 +26,7 @@ go to ``build/obj`` and the shared library is replaced atomically.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -159,6 +162,24 @@ def build_library(jobs: int = 8, out: Path = LIB, defines: tuple[str, ...] = (),
     return Path(out)
 
 
+def build_torch() -> Path:
+    """host/torch_calls.cpp against the installed PyTorch's headers and libraries."""
+    out = PKG / "libvoltattn_torch.so"
+    found = importlib.util.find_spec("torch")
+    if found is None or not found.origin:
+        raise RuntimeError("PyTorch not found (voltattn_amd/host/torch_calls.cpp compiles against its headers)")
+    torch = Path(found.origin).parent
+    rocm = Path(hipcc()).resolve().parent.parent
+    tmp = out.with_suffix(".so.tmp")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra", "-Werror",
+          "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", str(ROOT / "include"),
+          *(x for d in (torch / "include", torch / "include/torch/csrc/api/include", rocm / "include") for x in ("-isystem", str(d))),
+          str(PKG / "host" / "torch_calls.cpp"), "-o", str(tmp),
+          f"-L{torch / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch"])
+    os.replace(tmp, out)
+    return out
+
+
 def build_oracle() -> Path:
     _run(["make", "-s", "-C", str(ROOT / "oracle")])
     return ROOT / "oracle" / "liboracle.so"
@@ -182,7 +203,10 @@ def build_cli() -> Path:
 
 
 def build_all(jobs: int = 8) -> None:
-    build_library(jobs, variants=tuple(VARIANTS))
+    with cf.ThreadPoolExecutor(max_workers=1) as ex:
+        calls = ex.submit(build_torch)
+        build_library(jobs, variants=tuple(VARIANTS))
+        calls.result()
     build_oracle()
     if (ROOT / "tests" / "cli" / "voltattn_cli.cpp").exists():
         build_cli()

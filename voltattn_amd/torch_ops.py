@@ -38,6 +38,7 @@ torch.compile.
 from __future__ import annotations
 
 import ctypes as C
+from pathlib import Path
 from typing import Optional
 
 import torch
@@ -404,12 +405,17 @@ class _NoGradient(torch.autograd.Function):
         _fail(f"backward through voltattn::{ctx.name}, which has no gradient formula")
 
 
-def _op(schema: str, fake, computes: Optional[bool] = None):
+def _op(schema: str, fake, computes: Optional[bool] = None, native: bool = False):
     """Registers the decorated function and its fake implementation; what it returns is the op.
-    computes: whether its outputs are computed from its inputs (None: if it changes none in place)."""
+    computes: whether its outputs are computed from its inputs (None: if it changes none in place).
+    native: its plain calls on a GPU are host/torch_calls.cpp's, which hands the others to <name>_checked."""
     name = schema.split("(")[0]
+    if native:
+        checked = _op(f"{name}_checked{schema[len(name):]}", fake, computes)
 
     def register(fn):
+        if native:
+            checked(fn)
         _LIBRARY.define(schema)
         _LIBRARY.impl(name, fn, "CompositeExplicitAutograd")
         torch.library.register_fake(f"voltattn::{name}", fake, lib=_LIBRARY)
@@ -782,7 +788,7 @@ def _append_rope_fake(q, k, v, inv_freq, cu_seqlens, start, positions, block_tab
 
 @_op("append_rope(Tensor q, Tensor k, Tensor v, Tensor inv_freq, Tensor? cu_seqlens, Tensor start, Tensor? positions, Tensor block_table, "
      "Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scale_pages, Tensor(d!)? v_scale_pages, str fmt, int group=32, "
-     "bool interleaved=False, bool rotated_k=False, float scaling=1.0) -> (Tensor, Tensor)", _append_rope_fake, computes=True)
+     "bool interleaved=False, bool rotated_k=False, float scaling=1.0) -> (Tensor, Tensor)", _append_rope_fake, computes=True, native=True)
 def append_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor, cu_seqlens: Optional[torch.Tensor],
                 start: torch.Tensor, positions: Optional[torch.Tensor], block_table: torch.Tensor, k_pages: torch.Tensor,
                 v_pages: torch.Tensor, k_scale_pages: Optional[torch.Tensor], v_scale_pages: Optional[torch.Tensor], fmt: str,
@@ -844,7 +850,7 @@ def _attend_paged_fake(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_
 
 
 @_op("attend_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scale_pages, Tensor v_scale_pages, Tensor block_table, "
-     "Tensor? cu_seqlens, Tensor seq_lens, str fmt, SymInt max_seq_len, int group=32) -> Tensor", _attend_paged_fake)
+     "Tensor? cu_seqlens, Tensor seq_lens, str fmt, SymInt max_seq_len, int group=32) -> Tensor", _attend_paged_fake, native=True)
 def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale_pages: torch.Tensor, v_scale_pages: torch.Tensor,
                  block_table: torch.Tensor, cu_seqlens: Optional[torch.Tensor], seq_lens: torch.Tensor, fmt: str, max_seq_len: int,
                  group: int = 32) -> torch.Tensor:
@@ -853,6 +859,8 @@ def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     the positions up to its own. fmt "b8+": pages float8_e4m3fn [num_pages, Hkv, page_rows, D], scales fp16
     [num_pages, Hkv, page_rows / group]. max_seq_len >= every length."""
     _validate_attend(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, cu_seqlens, seq_lens, fmt, group)
+    if max_seq_len > 2147483647:
+        _fail(f"max_seq_len must be below 2^31 (got {max_seq_len})")
     stream = _ready(q, k_pages, v_pages, k_scale_pages, v_scale_pages, block_table, cu_seqlens, seq_lens)
     T, Hq, D = q.shape
     num_pages, Hkv, page_rows, _ = k_pages.shape
@@ -867,3 +875,18 @@ def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
 
 def row_format_bits(fmt: str) -> int:
     return _BITS[_fmt(fmt)]
+
+
+def _load_calls() -> None:
+    """host/torch_calls.cpp's plain calls: the C ABI's functions by their addresses in the library
+    that is loaded. Without a GPU nothing calls them, and the built file need not be there."""
+    path = Path(__file__).resolve().parent / "libvoltattn_torch.so"
+    if not path.exists():
+        if torch.cuda.device_count() > 0:
+            raise ImportError(f"{path} is not built; run `python voltattn_amd/build.py` (needs g++)")
+        return
+    torch.ops.load_library(str(path))
+    torch.ops.voltattn._bind([C.cast(f, C.c_void_p).value for f in (lib.va_append_rope, lib.va_attend_paged, lib.va_attend_ws_bytes)])
+
+
+_load_calls()
