@@ -11,10 +11,11 @@
 // rounded to fp16 (RNE) for the second product, each off by at most 2^-11 of itself.
 //
 // The n * (Hq/Hkv) rows (token, head of the group) of a K/V head are cut into blocks; a block's
-// work is the tiles of positions up to its last row's. All blocks' tiles, numbered one behind the
-// other (sequence, K/V head, block, tile), are cut into equal shares, one to a work-group; the
-// pieces of blocks that several shares cut go to ws (slot 2w: the piece that work-group w begins
-// with, 2w + 1: the one it ends with) and attend_merge joins them.
+// work is the tiles of positions up to its last row's. Blocks have costs in units (a tile's and
+// what it takes to begin one); all blocks' units, numbered one behind the other (sequence, K/V
+// head, block), are cut into shares, one to a work-group, and a block's tiles go to the shares as its
+// units do. The pieces of blocks that several shares cut go to ws (slot 2w: the piece that
+// work-group w begins with, 2w + 1: the one it ends with) and attend_merge joins them.
 #pragma once
 #include "va_kernels.hpp"
 #include "va_wide.hpp"
@@ -22,26 +23,12 @@
 namespace va {
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) float lds_float;
 
 // ------------------------------------------------------------- work split --
-// The rows between two consecutive bounds 0, cu[0], .., cu[B], total (each limited to what lies
-// between its predecessor and total); those before the first and behind the last sequence, and
-// sequences whose lengths are out of range, are blocks of one tile that only store their rows.
-struct AttendSpan {
-    int seq;              // -1: rows of no sequence
-    int begin, n, len;
-    int first;            // its first tile in the numbering
-    __device__ __forceinline__ bool bad(int cap) const { return len < 0 || len > cap; }
-};
-struct AttendBlock {
-    AttendSpan s;
-    int hk, rb;           // K/V head, block of rows
-    int first, tiles;     // its first tile in the numbering, how many
-};
-
 // The lane's (thread's) number, made anew: what is computed from it is not held across loops.
 __device__ __forceinline__ int fresh(int x) {
     asm volatile("" : "+v"(x));
@@ -60,25 +47,71 @@ __device__ __forceinline__ float local_minus_inf() {
     return x;
 }
 
-// The numbering, by one wave: lane i has span from + i of the current 64.
-template <int BM, int BN> struct AttendPlan {
-    const AttendArgs& a;
-    int from = -1, prev = 0;                     // prev: the bound ahead of the next 64
-    int begin = 0, n = 0, len = 0;
-    int count = 0, upto = 0;                     // tiles of the lane's span, and up to and with it
-    int total = 0;                               // tiles of the batch
-    __device__ __forceinline__ int spans() const { return a.cu ? a.B + 2 : a.B; }
-    __device__ __forceinline__ int seq_of(int i) const { return !a.cu ? (i < a.B ? i : -1) : i >= 1 && i <= a.B ? i - 1 : -1; }
-    __device__ __forceinline__ int blocks(int rows) const { return (rows + BM - 1) / BM; }
-    __device__ __forceinline__ int tiles(int seq, int n, int len, int rb) const {
-        if (seq < 0 || len < 0 || len > a.cap) return 1;
+// A block of BM rows of a sequence and K/V head; uniform. The rows are those between two consecutive
+// bounds 0, cu[0], .., cu[B], total (each limited to what lies between its predecessor and total);
+// those before the first and behind the last sequence (seq: -1), and of sequences whose lengths are
+// out of range, are blocks of one tile that only store their rows.
+template <int BM, int BN> struct AttendBlock {
+    int seq, begin, n, len;
+    int hk, rb;               // K/V head, block of rows
+    int first, units, tiles;  // its first unit in the numbering, how many; its tiles
+    static __device__ __forceinline__ int blocks(const AttendArgs& a, int n) { return (n * a.group + BM - 1) / BM; }
+    static __device__ __forceinline__ bool bad(const AttendArgs& a, int seq, int len) { return seq < 0 || len < 0 || len > a.cap; }
+    static __device__ __forceinline__ int tiles_of(const AttendArgs& a, int seq, int n, int len, int rb) {
+        if (bad(a, seq, len)) return 1;
         const int i1 = min(n - 1, (int)a.by_group.div((uint32_t)(rb * BM + BM - 1)));
         const int seen = len - n + i1 + 1;       // positions that the block's last row sees
         return seen <= 0 ? 1 : (seen - 1) / BN + 1;
     }
+    // The units of block rb are head + rb * slope, which for blocks that begin ever later is near its tiles.
+    static __device__ __forceinline__ int head(const AttendArgs& a, int seq, int n, int len) {
+        if (bad(a, seq, len)) return 1 << a.shift;
+        return (tiles_of(a, seq, n, len, n <= len ? 0 : max(blocks(a, n), 1) - 1) + a.setup) << a.shift;
+    }
+    static __device__ __forceinline__ int slope(const AttendArgs& a, int seq, int n, int len) { return bad(a, seq, len) || n > len ? 0 : a.slope; }
+    __device__ __forceinline__ bool bad(const AttendArgs& a) const { return bad(a, seq, len); }
+    __device__ __forceinline__ void size(const AttendArgs& a) {
+        units = uniform(head(a, seq, n, len) + rb * slope(a, seq, n, len));
+        tiles = uniform(tiles_of(a, seq, n, len, rb));
+    }
+    // The block behind this one, unless that is another sequence's.
+    __device__ __forceinline__ bool next(const AttendArgs& a) {
+        if (rb + 1 < blocks(a, n)) ++rb;
+        else if (hk + 1 < a.hkv) {
+            ++hk;
+            rb = 0;
+        } else return false;
+        first += units;
+        size(a);
+        return true;
+    }
+    // The tiles ahead of unit first + x: in the numbering's proportion, the first tile with the first unit.
+    __device__ __forceinline__ int ahead(int x) const { return x >= units ? tiles : x <= 0 ? 0 : (int)__builtin_ceil((double)x * tiles / units); }
+};
+
+// The numbering, by one wave: lane i has span from + i of the current 64. The work-groups of a CU do not
+// get on equally: its oldest waves go first. With equal shares of many rows those of 128-row blocks, three
+// to a CU, ended after 508, 650 and 752 us (10 prompts' chunks over up to 16 K positions), those of 256-row
+// blocks, two, after 3272 and 3977 (8 K tokens over 32 K positions); shares by age (10 : 8 : 6 and 8 : 6)
+// take these calls from 670 to 650 us and from 3900 to 3810. A launch fills the GPU in the order of its
+// blocks, an age after the other, eight XCDs in turn.
+template <int BM, int BN> struct AttendPlan {
+    using Block = AttendBlock<BM, BN>;
+    static constexpr int AGES = BM == 128 ? 3 : BM == 256 ? 2 : 1;
+    static constexpr int AGE[4] = {0, AGES == 3 ? 10 : 8, AGES == 3 ? 18 : 14, 24};   // what the work-groups up to an age take
+    const AttendArgs& a;
+    int from = -1, prev = 0;                     // prev: the bound ahead of the next 64
+    int begin = 0, n = 0, len = 0;
+    int count = 0, upto = 0;                     // units of the lane's span, and up to and with it
+    int total = 0;                               // units of the batch
+    __device__ __forceinline__ int spans() const { return a.cu ? a.B + 2 : a.B; }
+    __device__ __forceinline__ int seq_of(int i) const { return !a.cu ? (i < a.B ? i : -1) : i >= 1 && i <= a.B ? i - 1 : -1; }
+    static __device__ __forceinline__ int ahead(int head, int slope, int rb) { return rb * head + (int)((long long)rb * (rb - 1) / 2) * slope; }   // units of blocks 0 .. rb - 1
     __device__ __forceinline__ void load(int at, int before, int bound) {
         from = at;
         const int i = at + (fresh((int)threadIdx.x) & 63);
+        const int seq = seq_of(i);
+        len = seq >= 0 ? a.seq_lens[seq] : 0;
         if (a.cu) {
             int e = i <= a.B ? a.cu[i] : a.total;
             e = max(0, min(e, a.total));
@@ -90,11 +123,7 @@ template <int BM, int BN> struct AttendPlan {
             begin = i;
             n = i < a.B;
         }
-        const int seq = seq_of(i);
-        len = seq >= 0 ? a.seq_lens[seq] : 0;
-        int sum = 0;
-        for (int rb = 0, nb = blocks(n * a.group); rb < nb; ++rb) sum += tiles(seq, n, len, rb);
-        count = sum * a.hkv;
+        count = ahead(Block::head(a, seq, n, len), Block::slope(a, seq, n, len), Block::blocks(a, n)) * a.hkv;
         upto = before + wave_scan(count);
     }
     __device__ __forceinline__ explicit AttendPlan(const AttendArgs& args) : a(args) {
@@ -103,8 +132,8 @@ template <int BM, int BN> struct AttendPlan {
             total = __builtin_amdgcn_readlane(upto, 63);
         }
     }
-    // The block that tile `at` < total is in.
-    __device__ __forceinline__ AttendBlock find(int at) {
+    // The block that unit `at` < total is in.
+    __device__ __forceinline__ Block find(int at) {
         if (spans() > 64) {
             int before = 0, bound = 0;
             for (int f = 0; f < spans(); f += 64) {
@@ -115,31 +144,71 @@ template <int BM, int BN> struct AttendPlan {
             }
         }
         const int l = __builtin_ctzll(__ballot(upto > at));
-        AttendBlock b;
-        b.s.seq = seq_of(from + l);
-        b.s.begin = __builtin_amdgcn_readlane(begin, l);
-        b.s.n = __builtin_amdgcn_readlane(n, l);
-        b.s.len = __builtin_amdgcn_readlane(len, l);
-        const int nb = blocks(b.s.n * a.group), of = __builtin_amdgcn_readlane(count, l), per = of / a.hkv;
-        b.s.first = __builtin_amdgcn_readlane(upto, l) - of;
-        b.hk = (at - b.s.first) / per;
-        int in = at - b.s.first - b.hk * per;
-        for (int r0 = 0;; r0 += 64) {
-            const int rb = r0 + (fresh((int)threadIdx.x) & 63);
-            const int t = rb < nb ? tiles(b.s.seq, b.s.n, b.s.len, rb) : 0;
-            const int up = wave_scan(t), all = __builtin_amdgcn_readlane(up, 63);
-            if (in < all) {
-                const int k = __builtin_ctzll(__ballot(up > in));
-                b.rb = r0 + k;
-                b.tiles = __builtin_amdgcn_readlane(t, k);
-                b.first = at - in + __builtin_amdgcn_readlane(up, k) - b.tiles;
-                return b;
-            }
-            in -= all;
+        Block b;
+        b.seq = seq_of(from + l);
+        b.begin = __builtin_amdgcn_readlane(begin, l);
+        b.n = __builtin_amdgcn_readlane(n, l);
+        b.len = __builtin_amdgcn_readlane(len, l);
+        const int nb = Block::blocks(a, b.n), of = __builtin_amdgcn_readlane(count, l), per = of / a.hkv;
+        const int head = Block::head(a, b.seq, b.n, b.len), slope = Block::slope(a, b.seq, b.n, b.len);
+        const int start = __builtin_amdgcn_readlane(upto, l) - of;
+        b.hk = uniform((at - start) / per);
+        const int in = at - start - b.hk * per;
+        b.rb = 0;
+        for (int step = nb; step > 1;) {         // the last block whose units begin at `in` or before: among step from rb on
+            step = (step + 63) / 64;
+            const int rb = b.rb + (fresh((int)threadIdx.x) & 63) * step;
+            b.rb += step * (__builtin_popcountll(__ballot(rb < nb && ahead(head, slope, rb) <= in)) - 1);
         }
+        b.rb = uniform(b.rb);
+        b.first = uniform(start + b.hk * per + ahead(head, slope, b.rb));
+        b.size(a);
+        return b;
     }
-    __device__ __forceinline__ int share() const { return max((total + a.nwg - 1) / a.nwg, 1); }
-    __device__ __forceinline__ int shares(int share) const { return (total + share - 1) / share; }
+    // The shares: units start(w) .. start(w + 1) - 1 are work-group w's.
+    __device__ __forceinline__ bool by_age() const { return AGES > 1 && a.nwg % (8 * AGES) == 0 && total >> (a.shift + 4) >= a.nwg; }
+    __device__ __forceinline__ int share() const {
+        const int x = (total + a.nwg - 1) / a.nwg, tile = 1 << a.shift;
+        return x >= 8 * tile ? x : (x + tile - 1) & -tile;   // whole tiles, where they are few
+    }
+    __device__ __forceinline__ int shares() const { return by_age() ? a.nwg : (total + share() - 1) / share(); }
+    __device__ __forceinline__ int start(int w) const {
+        if (!by_age()) return (int)min((long long)w * share(), (long long)total);
+        if (w >= a.nwg) return total;
+        const int per = a.nwg / 8, of = per / AGES, x = w / per, j = w - x * per, age = j / of;
+        const int p = (x * AGE[AGES] + AGE[age]) * of + (j - age * of) * (AGE[age + 1] - AGE[age]), all = 8 * AGE[AGES] * of;
+        return total / all * p + (int)((uint32_t)(total % all) * (uint32_t)p / (uint32_t)all);
+    }
+};
+
+// What attend_merge has to know of work-group w, behind the pieces in ws: whether it begins a block
+// that others go on with (its rows, else 0; its first token, K/V head and number), and whether it goes
+// on with one (head: 1, and 2 if it ends it).
+struct AttendNote {
+    int rows, begin, hk, rb;
+    int head, unused[3];
+};
+template <int D, int BM> __device__ __forceinline__ AttendNote* attend_note(const AttendArgs& a, int w) {
+    return reinterpret_cast<AttendNote*>(a.ws + (size_t)2 * a.nwg * BM * (D + 2)) + w;
+}
+template <int D, int BM, int BN> __device__ __forceinline__ void attend_write_note(const AttendArgs& a, int w, const AttendBlock<BM, BN>& b, int t0, int t1) {
+    AttendNote* to = attend_note<D, BM>(a, w);
+    if (t0 == 0) *reinterpret_cast<i32x4*>(to) = i32x4{min(BM, b.n * a.group - b.rb * BM), b.begin, b.hk, b.rb};
+    else to->head = t1 == b.tiles ? 2 : 1;
+}
+// The share of a work-group; its note is empty at first.
+template <int D, int BM, int BN> struct AttendShare {
+    int wg, at, end;
+    __device__ __forceinline__ AttendShare(const AttendArgs& a, const AttendPlan<BM, BN>& plan) {
+        const int per = (plan.shares() + 7) >> 3, x = (int)blockIdx.x & 7, j = (int)blockIdx.x >> 3;   // neighbours on one XCD
+        wg = j < per ? x * per + j : 8 * per + x * ((int)(gridDim.x >> 3) - per) + j - per;
+        if (wg < a.nwg && threadIdx.x == 0) {
+            i32x4* to = reinterpret_cast<i32x4*>(attend_note<D, BM>(a, wg));
+            to[0] = to[1] = i32x4{};
+        }
+        at = j < per ? uniform(plan.start(wg)) : 0;
+        end = j < per ? uniform(plan.start(wg + 1)) : 0;
+    }
 };
 
 // -------------------------------------------------------------- cache tiles --
@@ -300,20 +369,21 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
     lds_u8* vt = (lds_u8*)lds + wave * VB;
     if (tid == 0) *odd = 0;
     AttendPlan<BM, BN> plan(a);
-    const int share = plan.share(), per = (plan.shares(share) + 7) >> 3;
-    if ((int)(blockIdx.x >> 3) >= per) return;
-    const int wg = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    int at = wg * share;
-    const int end = min(plan.total, at + share);
+    const AttendShare<D, BM, BN> share(a, plan);
+    const int wg = share.wg, end = share.end;
+    int at = share.at;
+    AttendBlock<BM, BN> blk;
+    blk.tiles = 0;
 
     auto fresh_lane = [&]() { return fresh(lane); };
     while (at < end) {
-        const AttendBlock blk = plan.find(at);
-        const int hk = uniform(blk.hk), rb = uniform(blk.rb), n = uniform(blk.s.n), begin = uniform(blk.s.begin), seq = uniform(blk.s.seq);
-        const int len = uniform(blk.s.len), tiles = uniform(blk.tiles), t0 = uniform(at - blk.first), t1 = uniform(min(tiles, t0 + (end - at)));
+        if (blk.tiles == 0 || !blk.next(a)) blk = plan.find(at);
+        const int hk = blk.hk, rb = blk.rb, n = blk.n, begin = blk.begin, seq = blk.seq, len = blk.len, tiles = blk.tiles;
+        const int t0 = uniform(blk.ahead(at - blk.first)), t1 = uniform(blk.ahead(end - blk.first));
         const int rows = n * a.group, hq = a.hkv * a.group;
-        at += t1 - t0;
-        if (seq < 0 || blk.s.bad(a.cap)) {
+        at = uniform(min(end, blk.first + blk.units));
+        if (t0 >= t1) continue;
+        if (blk.bad(a)) {
             const float x = seq < 0 ? 0.f : __builtin_nanf("");
             for (int i = fresh(tid); i < BM * (D / 8); i += 256) {
                 const int r = rb * BM + i / (D / 8);
@@ -481,6 +551,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
         } while (t < t1);
 
         const bool whole = t0 == 0 && t1 == tiles;
+        if (!whole && fresh(tid) == 0) attend_write_note<D, BM, BN>(a, wg, blk, t0, t1);
         float* part = a.ws + (size_t)(2 * wg + (t0 == 0 ? 1 : 0)) * BM * (D + 2);   // [BM][D] sums, then [BM][2] (m, l)
         lds_float* es = (lds_float*)lds;
         lds_float* ml = es + EPI / 4;
@@ -705,25 +776,26 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
         return (uint32_t)(tile + pos * D + ((((x >> 4) & 1) ^ wide_swz_v<D>(pos)) << 4) + (x & 1) * 8);
     };
     int at = 0, end = 0, wg = 0;
+    AttendBlock<BM, BN> blk;
+    blk.tiles = 0;
     do {
-        AttendBlock blk;
-        {
+        if (blk.tiles == 0 || !blk.next(a)) {
             AttendPlan<BM, BN> plan(a);                      // (holding the plan would cost the loop's registers)
             if (end == 0) {
-                const int share = plan.share(), per = (plan.shares(share) + 7) >> 3;
-                if ((int)(blockIdx.x >> 3) >= per) return;
-                wg = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-                at = wg * share;
-                end = min(plan.total, at + share);
+                const AttendShare<D, BM, BN> share(a, plan);
+                wg = share.wg;
+                at = share.at;
+                end = share.end;
                 if (at >= end) return;
             }
             blk = plan.find(at);
         }
-        const int hk = uniform(blk.hk), rb = uniform(blk.rb), n = uniform(blk.s.n), begin = uniform(blk.s.begin), seq = uniform(blk.s.seq);
-        const int len = uniform(blk.s.len), tiles = uniform(blk.tiles), t0 = uniform(at - blk.first), t1 = uniform(min(tiles, t0 + (end - at)));
+        const int hk = blk.hk, rb = blk.rb, n = blk.n, begin = blk.begin, seq = blk.seq, len = blk.len, tiles = blk.tiles;
+        const int t0 = uniform(blk.ahead(at - blk.first)), t1 = uniform(blk.ahead(end - blk.first));
         const int rows = n * a.group, hq = a.hkv * a.group;
-        at += t1 - t0;
-        if (seq < 0 || blk.s.bad(a.cap)) {
+        at = uniform(min(end, blk.first + blk.units));
+        if (t0 >= t1) continue;
+        if (blk.bad(a)) {
             const float x = seq < 0 ? 0.f : __builtin_nanf("");
             for (int i = fresh(tid); i < BM * (D / 8); i += 256) {
                 const int r = rb * BM + i / (D / 8);
@@ -857,6 +929,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
         }
         for (; t < t1; ++t, cur ^= RAW) arrive(t, cur);
         const bool whole = t0 == 0 && t1 == tiles;
+        if (!whole && fresh(tid) == 0) attend_write_note<D, BM, BN>(a, wg, blk, t0, t1);
         __syncthreads();                                     // the last tile is read
         if ((fresh(tid) & 63) == 0) reinterpret_cast<lds_int*>(kt)[wave] = odd;
         __syncthreads();
@@ -909,35 +982,41 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
 }
 
 // ------------------------------------------------------------------- merge --
-// Joins the pieces of the block that share w begins and does not end (if it does): MR rows to a
+// Joins the pieces of the block that work-group w begins and does not end (if it does): MR rows to a
 // work-group, eight lanes to a row with D/8 columns each; PW of the waves share the same rows' pieces.
-template <int D, int BM, int BN, int PW>
+template <int D, int BM, int PW>
 __global__ __launch_bounds__(256) void attend_merge(AttendArgs a) {
     constexpr int MR = 32 / PW, V = D / 32, U = 4;           // U: pieces in flight
     __shared__ float s_part[PW > 1 ? 4 * 8 * D : 1], s_ml[PW > 1 ? 4 * 8 * 2 : 1];
     const int lane = (int)__lane_id(), wave = uniform((int)threadIdx.x >> 6);
     const int w0 = (int)blockIdx.x / (BM / MR), base = (int)(blockIdx.x % (BM / MR)) * MR;
-    AttendPlan<BM, BN> plan(a);
-    const int share = plan.share(), cut = (w0 + 1) * share;
-    if ((long long)(w0 + 1) * share >= plan.total) return;
-    const AttendBlock blk = plan.find(cut - 1);
-    const int rows = blk.s.n * a.group - blk.rb * BM;        // of the block, BM at most
-    if (blk.first < w0 * share || blk.first + blk.tiles <= cut || base >= rows) return;
-    const int w1 = (blk.first + blk.tiles - 1) / share;
+    const AttendNote note = *attend_note<D, BM>(a, w0);
+    const int rows = uniform(note.rows);
+    if (base >= rows) return;
     const int r = base + (PW > 1 ? 0 : wave * 8) + (lane >> 3), pw = PW > 1 ? wave : 0;
     constexpr size_t STEP = (size_t)BM * (D + 2);
-    const float* col = a.ws + (size_t)r * D + (lane & 7) * 4;
-    const float* ml = a.ws + (size_t)BM * D + 2 * r;
+    const int rc = min(r, rows - 1);                         // (a row that is there)
+    const float* col = a.ws + (size_t)rc * D + (lane & 7) * 4;
+    const float* ml = a.ws + (size_t)BM * D + 2 * rc;
     float m = -__builtin_inff(), l = 0.f;
     f32x4 x[V] = {};
-    if (r < rows) {
-        for (int p0 = w0 + pw; p0 <= w1; p0 += U * PW) {
+    for (int from = w0;; from += 64) {
+        // which of the 64 work-groups from there on have a piece; with PW > 1 the waves share them
+        const int p = from + lane, head = p == w0 ? 1 : p < a.nwg ? attend_note<D, BM>(a, p)->head : 2;
+        const uint64_t last = __ballot(head == 2);
+        uint64_t there = __ballot(head != 0 && (PW == 1 || lane % PW == pw));
+        if (last) there &= (last ^ (last - 1));              // up to the first that ends it
+        while (there) {
             f32x2 s[U];
             f32x4 y[U][V];
+            bool on[U];
+            int k = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int p = min(p0 + u * PW, w1);          // the last one again: not used
-                const size_t at = (size_t)(2 * p + (p == w0 ? 1 : 0)) * STEP;
+                on[u] = there != 0;
+                if (on[u]) k = __builtin_ctzll(there);       // else the last one again: not used
+                there &= there - 1;
+                const size_t at = (size_t)(2 * (from + k) + (from + k == w0 ? 1 : 0)) * STEP;
                 s[u] = *reinterpret_cast<const f32x2*>(ml + at);
 #pragma unroll
                 for (int v = 0; v < V; ++v) y[u][v] = *reinterpret_cast<const f32x4*>(col + at + 32 * v);
@@ -952,7 +1031,7 @@ __global__ __launch_bounds__(256) void attend_merge(AttendArgs a) {
             for (int v = 0; v < V; ++v) x[v] *= f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (p0 + u * PW > w1) continue;
+                if (!on[u]) continue;
                 const float g = s[u].x == to ? 1.f : fast_exp2(s[u].x - to);
                 l = __builtin_fmaf(g, s[u].y, l);
 #pragma unroll
@@ -961,6 +1040,7 @@ __global__ __launch_bounds__(256) void attend_merge(AttendArgs a) {
                     for (int e = 0; e < 4; ++e) x[v][e] = __builtin_fmaf(g, y[u][v][e], x[v][e]);
             }
         }
+        if (last) break;
     }
     if constexpr (PW > 1) {
         float* mine = s_part + (wave * 8 + (lane >> 3)) * D + (lane & 7) * 4;
@@ -992,8 +1072,8 @@ __global__ __launch_bounds__(256) void attend_merge(AttendArgs a) {
         }
     }
     if (r >= rows) return;
-    const int row = blk.rb * BM + r, tok = (int)a.by_group.div((uint32_t)row);
-    uint16_t* out = a.out + ((size_t)(blk.s.begin + tok) * a.hkv * a.group + blk.hk * a.group + (row - tok * a.group)) * D + (lane & 7) * 4;
+    const int row = note.rb * BM + r, tok = (int)a.by_group.div((uint32_t)row);
+    uint16_t* out = a.out + ((size_t)(note.begin + tok) * a.hkv * a.group + note.hk * a.group + (row - tok * a.group)) * D + (lane & 7) * 4;
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int v = 0; v < V; ++v) {

@@ -258,12 +258,15 @@ struct AttendArgs {
     int   cap;                    // seq_lens at most
     float qscale;                 // log2(e) / sqrt(D)
     FastDiv by_group;
-    int   nwg, form;              // of its AttendForm
+    int   nwg, form, setup, shift; // of its AttendForm
+    int   slope;                  // units that a block has more than the one before it
 };
-// Rows to a block (16, 32: attend_few; 128, 256: attend_wide), K/V tiles of the batch at most, and work-groups.
+// Rows to a block (16, 32: attend_few; 128, 256: attend_wide), K/V tiles of the batch at most, work-groups,
+// tiles that beginning a block is worth, and units of a tile (2^shift).
 struct AttendForm {
     int rows;
     long long tiles, groups;
+    int setup, shift;
 };
 AttendForm attend_form(int D, int B, int total, int hkv, int group, int cap, int cus);
 size_t attend_ws_floats(const AttendForm& f, int D);

@@ -859,7 +859,7 @@ int validate_tree(va_fmt fmt, const va_paged_shape* sh, int T, va::TreeForm* for
     if (rows > 1 << 20 || (long long)sh->B * T * sh->Hq > 0x7FFFFFFFLL / 64) return fail(VA_ERANGE, "B*T*Hq too large");
     if ((long long)sh->B * sh->Hkv * ((rows + 31) / 32) > MAX_GROUPS) return fail(VA_ERANGE, "B*Hkv too large");
     *form = va::tree_form(kind_of(fmt), sh->D, sh->B, sh->Hkv, (int)rows, sh->max_seq_len, cus_or_default());
-    if (form->tiles > 1 << 30) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
+    if (form->tiles > 1 << 27) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
     return VA_OK;
 }
 
@@ -1128,7 +1128,7 @@ int validate_attend(va_fmt fmt, const va_paged_shape* sh, int total, va::AttendF
     const int group = sh->Hq / sh->Hkv;
     if ((long long)total * sh->Hq > 1 << 30) return fail(VA_ERANGE, "total*Hq too large");
     *form = va::attend_form(sh->D, sh->B, total, sh->Hkv, group, sh->max_seq_len, cus_or_default());
-    if (form->tiles > 1 << 30) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
+    if (form->tiles > 1 << 27) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
     return VA_OK;
 }
 
@@ -1177,6 +1177,8 @@ int va_attend_paged(va_fmt fmt, const va_attend_bufs* b, const va_paged_shape* s
     a.qscale = (float)(1.4426950408889634074 / std::sqrt((double)sh->D));
     a.nwg = (int)form.groups;
     a.form = form.rows;
+    a.setup = form.setup;
+    a.shift = form.shift;
     const hipError_t e = va::launch_attend(sh->D, sh->G, a, as_stream(stream));
     if (e != hipSuccess) return hip_fail(e, "attend launch");
     return VA_OK;
