@@ -86,7 +86,12 @@ template <int BM, int BN> struct AttendBlock {
         return true;
     }
     // The tiles ahead of unit first + x: in the numbering's proportion, the first tile with the first unit.
-    __device__ __forceinline__ int ahead(int x) const { return x >= units ? tiles : x <= 0 ? 0 : (int)__builtin_ceil((double)x * tiles / units); }
+    __device__ __forceinline__ int ahead(const AttendArgs& a, int x) const {
+        if (x >= units) return tiles;
+        if (x <= 0) return 0;
+        if (units == tiles << a.shift) return (x + (1 << a.shift) - 1) >> a.shift;   // the same, without the division
+        return (int)__builtin_ceil((double)x * tiles / units);
+    }
 };
 
 // The numbering, by one wave: lane i has span from + i of the current 64. The work-groups of a CU do not
@@ -379,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
     while (at < end) {
         if (blk.tiles == 0 || !blk.next(a)) blk = plan.find(at);
         const int hk = blk.hk, rb = blk.rb, n = blk.n, begin = blk.begin, seq = blk.seq, len = blk.len, tiles = blk.tiles;
-        const int t0 = uniform(blk.ahead(at - blk.first)), t1 = uniform(blk.ahead(end - blk.first));
+        const int t0 = uniform(blk.ahead(a, at - blk.first)), t1 = uniform(blk.ahead(a, end - blk.first));
         const int rows = n * a.group, hq = a.hkv * a.group;
         at = uniform(min(end, blk.first + blk.units));
         if (t0 >= t1) continue;
@@ -791,7 +796,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
             blk = plan.find(at);
         }
         const int hk = blk.hk, rb = blk.rb, n = blk.n, begin = blk.begin, seq = blk.seq, len = blk.len, tiles = blk.tiles;
-        const int t0 = uniform(blk.ahead(at - blk.first)), t1 = uniform(blk.ahead(end - blk.first));
+        const int t0 = uniform(blk.ahead(a, at - blk.first)), t1 = uniform(blk.ahead(a, end - blk.first));
         const int rows = n * a.group, hq = a.hkv * a.group;
         at = uniform(min(end, blk.first + blk.units));
         if (t0 >= t1) continue;
@@ -990,7 +995,9 @@ __global__ __launch_bounds__(256) void attend_merge(AttendArgs a) {
     __shared__ float s_part[PW > 1 ? 4 * 8 * D : 1], s_ml[PW > 1 ? 4 * 8 * 2 : 1];
     const int lane = (int)__lane_id(), wave = uniform((int)threadIdx.x >> 6);
     const int w0 = (int)blockIdx.x / (BM / MR), base = (int)(blockIdx.x % (BM / MR)) * MR;
+    auto head_of = [&](int p) { return p == w0 ? 1 : p < a.nwg ? attend_note<D, BM>(a, p)->head : 2; };
     const AttendNote note = *attend_note<D, BM>(a, w0);
+    int head = head_of(w0 + lane);                           // (with the note, not after it)
     const int rows = uniform(note.rows);
     if (base >= rows) return;
     const int r = base + (PW > 1 ? 0 : wave * 8) + (lane >> 3), pw = PW > 1 ? wave : 0;
@@ -1002,7 +1009,7 @@ __global__ __launch_bounds__(256) void attend_merge(AttendArgs a) {
     f32x4 x[V] = {};
     for (int from = w0;; from += 64) {
         // which of the 64 work-groups from there on have a piece; with PW > 1 the waves share them
-        const int p = from + lane, head = p == w0 ? 1 : p < a.nwg ? attend_note<D, BM>(a, p)->head : 2;
+        if (from != w0) head = head_of(from + lane);
         const uint64_t last = __ballot(head == 2);
         uint64_t there = __ballot(head != 0 && (PW == 1 || lane % PW == pw));
         if (last) there &= (last ^ (last - 1));              // up to the first that ends it
