@@ -463,6 +463,57 @@ bool serving_case(Fmt f, int G, double* maxerr) {
     return ok;
 }
 
+// The wrappers of the block format: a prompt of two sequences written without a turn (frequencies of 0)
+// and attended from its own cache. A row that sees itself alone is its value as the cache holds it, off
+// by half a step of e4m3: 2^-4 of itself, or 2^-10 of a scale that is below its block's largest / 224,
+// and rounded to fp16.
+bool block_case(int G, double* maxerr) {
+    const int B = 2, Hq = 8, Hkv = 2, D = 128, P = 64, pages = 4, wide = 2, total = 71;
+    DeviceBuffer K(page_bytes(Fmt::B8M, Hkv, P, D) * pages), V(page_bytes(Fmt::B8M, Hkv, P, D) * pages);
+    DeviceBuffer SK(page_scale_bytes(Fmt::B8M, Hkv, P, D, G) * pages), SV(page_scale_bytes(Fmt::B8M, Hkv, P, D, G) * pages);
+    auto ints = [](std::vector<int32_t> x) {
+        DeviceBuffer d(x.size() * 4);
+        d.upload(x.data(), x.size() * 4);
+        return d;
+    };
+    DeviceBuffer table = ints({3, 1, 0, -1}), cu = ints({0, 70, 71}), start = ints({0, 0}), lens = ints({70, 1}), freq = ints(std::vector<int32_t>(D / 2, 0));
+    const int heads = Hq + 2 * Hkv;
+    const size_t n = (size_t)total * heads * D, nq = (size_t)total * Hq * D;
+    DeviceBuffer wide_x(n * 4), x(n * 2), q(nq * 2), out(nq * 2);
+    check(va_fill_normal(wide_x.as<float>(), n, 11, nullptr));
+    check(va_f32_to_f16(wide_x.as<float>(), n, x.as<uint16_t>(), nullptr));
+    const RopeShape rs{B, total, Hq, Hkv, D, G, P, wide, pages, D, 0, 1.f, (int64_t)heads * D, D, (int64_t)heads * D, D, (int64_t)heads * D, D};
+    uint16_t* rows = x.as<uint16_t>();
+    append_rope(Fmt::B8M, RopeBufs{rows, rows + Hq * D, rows + (Hq + Hkv) * D, cu.as<int32_t>(), start.as<int32_t>(), nullptr, table.as<int32_t>(),
+                                   freq.as<float>(), q.as<uint16_t>(), nullptr, K.get(), V.get(), SK.as<uint16_t>(), SV.as<uint16_t>()}, rs);
+    PagedShape sh{B, Hq, Hkv, D, G, P, wide, pages, wide * P};
+    DeviceBuffer ws(attend_ws_bytes(Fmt::B8M, sh, total));
+    attend_paged(Fmt::B8M, AttendBufs{K.get(), V.get(), SK.as<uint16_t>(), SV.as<uint16_t>(), table.as<int32_t>(), cu.as<int32_t>(), lens.as<int32_t>(),
+                                      q.as<uint16_t>(), out.as<uint16_t>(), ws.as<float>()}, sh, total);
+    check(va_sync());
+    std::vector<uint16_t> hx(n), hq(nq), ho(nq);
+    x.download(hx.data(), n * 2);
+    q.download(hq.data(), nq * 2);
+    out.download(ho.data(), nq * 2);
+    bool ok = true;
+    for (int t = 0; t < total; ++t)
+        for (int i = 0; i < Hq * D; ++i) ok = ok && hq[(size_t)t * Hq * D + i] == hx[(size_t)t * heads * D + i];
+    for (int t : {0, 70})
+        for (int h = 0; h < Hq; ++h) {
+            const size_t v = ((size_t)t * heads + Hq + Hkv + h * Hkv / Hq) * D;
+            double top = 0;
+            const int block = t == 0 ? G : 1;                // rows under its scale
+            for (int r = 0; r < block; ++r)
+                for (int d = 0; d < D; ++d) top = std::max(top, std::fabs(half_to_double(hx[v + (size_t)r * heads * D + d])));
+            for (int d = 0; d < D; ++d) {
+                const double want = half_to_double(hx[v + d]), off = std::fabs(half_to_double(ho[((size_t)t * Hq + h) * D + d]) - want);
+                *maxerr = std::max(*maxerr, off);
+                ok = ok && off <= (std::fabs(want) / 16 + top / 224 / 1024) * 1.001 + std::fabs(want) / 1024;
+            }
+        }
+    return ok;
+}
+
 int selftest_ex() {
     const Fmt tiled[] = {Fmt::F16M, Fmt::Q8M, Fmt::Q4M, Fmt::Q3M};
     struct GqaCase { int Hq, Hkv, L, D, S; };
@@ -497,6 +548,12 @@ int selftest_ex() {
         double maxerr = 0.0;
         const bool ok = serving_case(f, 64, &maxerr);
         std::printf("serve  %-4s Hq=8  Hkv=2  lens=100,63 G=64  maxerr=%.2e  %s\n", fmt_name(f), maxerr, ok ? "PASS" : "FAIL");
+        fails += !ok;
+    }
+    for (int G : {32, 64}) {
+        double maxerr = 0.0;
+        const bool ok = block_case(G, &maxerr);
+        std::printf("block  %-4s Hq=8  Hkv=2  lens=70,1   G=%-2d  maxerr=%.2e  %s\n", fmt_name(Fmt::B8M), G, maxerr, ok ? "PASS" : "FAIL");
         fails += !ok;
     }
     if (fails) { std::printf("%d serving case(s) FAILED\n", fails); return 1; }

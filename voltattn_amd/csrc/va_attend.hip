@@ -19,7 +19,7 @@ AttendForm attend_form(int D, int B, int total, int hkv, int group, int cap, int
     // every sequence's last block may be a part, as may the rows before the first and behind the last one
     const long long blocks = std::min((long long)total * group, (long long)total * group / f.rows + B + 2) * hkv;
     f.tiles = blocks * std::max(1LL, (cap + bn - 1) / bn);
-    f.groups = std::min(f.tiles, (f.rows == 128 ? 3LL : 2LL) * cus);
+    f.groups = std::max(1LL, std::min(f.tiles, (f.rows == 128 ? 3LL : 2LL) * cus));   // total = 0: no tiles
     f.setup = f.tiles / f.groups >= 8 ? SETUP : 0;
     // the numbering, of which the slope may make twice the tiles, has to end below 2^31
     f.shift = 4;

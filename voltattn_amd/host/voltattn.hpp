@@ -12,8 +12,8 @@
 //
 // Beyond the reference (its README.md:205-206 lists GQA and paged KV as
 // missing): launch_gqa, launch_paged, append_kv, prefill, decode_tree,
-// compact_kv, fork_pages, resize_pages, and the Stream / Graph helpers for
-// replaying captured decode steps.
+// compact_kv, fork_pages, resize_pages, append_rope, attend_paged, and the
+// Stream / Graph helpers for replaying captured decode steps.
 //
 // Errors throw voltattn::Error (status code + message), where the reference
 // exits through CUDA_CHECK (src/voltattn.cu:49-58).
@@ -29,7 +29,8 @@
 namespace voltattn {
 
 enum class Fmt : int {
-    F16 = VA_F16, F16M = VA_F16P, Q8 = VA_Q8, Q8M = VA_Q8P, Q4 = VA_Q4, Q4M = VA_Q4P, Q3M = VA_Q3P
+    F16 = VA_F16, F16M = VA_F16P, Q8 = VA_Q8, Q8M = VA_Q8P, Q4 = VA_Q4, Q4M = VA_Q4P, Q3M = VA_Q3P,
+    B8M = VA_B8P                                            // append_rope and attend_paged only
 };
 inline constexpr Fmt kAllFormats[] = {Fmt::F16, Fmt::F16M, Fmt::Q8, Fmt::Q8M, Fmt::Q4, Fmt::Q4M, Fmt::Q3M};
 
@@ -38,7 +39,7 @@ inline bool is_f16(Fmt f) { return f == Fmt::F16 || f == Fmt::F16M; }
 inline int qbits(Fmt f) {
     switch (f) {
         case Fmt::F16: case Fmt::F16M: return 16;
-        case Fmt::Q8:  case Fmt::Q8M:  return 8;
+        case Fmt::Q8:  case Fmt::Q8M: case Fmt::B8M: return 8;
         case Fmt::Q4:  case Fmt::Q4M:  return 4;
         default:                       return 3;
     }
@@ -267,6 +268,22 @@ inline void resize_pages(int B, int page_rows, int max_pages, int num_pages, int
                          const int32_t* old_lens, const int32_t* new_lens, int32_t* missing = nullptr,
                          void* stream = nullptr) {
     check(va_resize_pages(B, page_rows, max_pages, num_pages, block_table, refs, old_lens, new_lens, missing, stream));
+}
+
+// The cache write of a projection's rows with the position rotation (any format), and attention of the
+// newest tokens over a cache of the format b8+.
+using RopeShape = va_rope_shape;
+using RopeBufs = va_rope_bufs;
+using AttendBufs = va_attend_bufs;
+
+inline void append_rope(Fmt f, const RopeBufs& b, const RopeShape& shape, void* stream = nullptr) {
+    check(va_append_rope(static_cast<va_fmt>(f), &b, &shape, stream));
+}
+inline size_t attend_ws_bytes(Fmt f, const PagedShape& shape, int total) {
+    return va_attend_ws_bytes(static_cast<va_fmt>(f), &shape, total);
+}
+inline void attend_paged(Fmt f, const AttendBufs& b, const PagedShape& shape, int total, void* stream = nullptr) {
+    check(va_attend_paged(static_cast<va_fmt>(f), &b, &shape, total, stream));
 }
 
 // Device quantize() of fp32 rows [rows][D] into packed codes and fp16 scales.
