@@ -353,7 +353,11 @@ constexpr float ATT_OFF = 10.f, ATT_SLACK = 4.f;
 // ds_read_b64_tr_b8 (lane i of 16 addresses half i%2 of row i/2 and receives column i of the eight
 // rows; probed on MI355X). A lane's slots of the second product are the positions whose scores it
 // holds: 4h + 0..3 and 16 + 4h + 0..3.
-typedef float f32x4v __attribute__((ext_vector_type(4)));
+//
+// Bound by memory: 32 heads over 64 K positions (537 MB) 85.5 us, 6.3 TB/s of the 7.3 that plain reads reach; 64
+// sequences over up to 8 K positions (303 MB) 56 us, where every work-group begins two blocks; one token over
+// 4 K positions 7 us, the chain of lengths, table, scales and tile. Three work-groups on a CU (161 registers,
+// one V tile ahead) do 64 K positions in 91 us.
 
 template <int D> __device__ __forceinline__ int few_swz(int row) {
     return D == 128 ? ((row >> 1) & 1) | ((row >> 4) & 1) << 1 | ((row >> 2) & 1) << 2 : ((row >> 4) & 1) | ((row >> 2) & 1) << 1;
@@ -625,7 +629,12 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
 //
 // A wave's products go before the other waves' weights (s_setprio): they need the issue port for a
 // moment each and the matrix cores for long; without it the oldest wave of a SIMD goes first, the
-// others fall behind, and the last work-groups of a CU finish alone.
+// others fall behind, and the last work-groups of a CU finish alone (8 K tokens over 32 K positions: 4336
+// us without, 3998 with it, before shares went by age).
+//
+// Bound by the matrix cores and what shares the issue port with them: those 8 K tokens (32 heads, 8 K/V
+// heads of 128 dimensions) take 3590 to 3690 us, 1050 TFLOP/s at the 1.9 GHz that the power allows; a
+// large product of the library does 1173 to 1465.
 //
 // A lane has two score blocks of 32 positions at a time: both halves of a tile against one row (CB =
 // 1), or one half against a row of each group (CB = 2).
@@ -989,6 +998,8 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
 // ------------------------------------------------------------------- merge --
 // Joins the pieces of the block that work-group w begins and does not end (if it does): MR rows to a
 // work-group, eight lanes to a row with D/8 columns each; PW of the waves share the same rows' pieces.
+// 4 to 5 us for few rows (the launch, the notes, the pieces); 22 and 31 us for 128- and 256-row blocks on
+// a full card (65 and 130 KB a piece, written and read again).
 template <int D, int BM, int PW>
 __global__ __launch_bounds__(256) void attend_merge(AttendArgs a) {
     constexpr int MR = 32 / PW, V = D / 32, U = 4;           // U: pieces in flight

@@ -268,7 +268,7 @@ struct AttendForm {
     long long tiles, groups;
     int setup, shift;
 };
-AttendForm attend_form(int D, int B, int total, int hkv, int group, int cap, int cus);
+AttendForm attend_form(int B, int total, int hkv, int group, int cap, int cus);
 size_t attend_ws_floats(const AttendForm& f, int D);
 hipError_t launch_attend(int D, int G, const AttendArgs& a, hipStream_t stream);
 

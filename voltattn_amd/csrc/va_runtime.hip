@@ -1127,7 +1127,7 @@ int validate_attend(va_fmt fmt, const va_paged_shape* sh, int total, va::AttendF
     if (total < 0) return fail(VA_EINVAL, "total must be >= 0 (got %d)", total);
     const int group = sh->Hq / sh->Hkv;
     if ((long long)total * sh->Hq > 1 << 30) return fail(VA_ERANGE, "total*Hq too large");
-    *form = va::attend_form(sh->D, sh->B, total, sh->Hkv, group, sh->max_seq_len, cus_or_default());
+    *form = va::attend_form(sh->B, total, sh->Hkv, group, sh->max_seq_len, cus_or_default());
     if (form->tiles > 1 << 27) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
     return VA_OK;
 }
