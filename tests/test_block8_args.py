@@ -214,3 +214,25 @@ def test_backward_raises(name, args):
     out = out[0] if isinstance(out, tuple) else out
     with pytest.raises(RuntimeError, match=name):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name,args", [("append_rope", _rope_args), ("attend_paged", _attend_args)])
+def test_fake_gpu_tensors(name, args, grad):
+    """What torch.compile runs: fake tensors of a GPU, through the keys that the calls without Python have."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        a = args("cuda")
+        a[0].requires_grad_(grad)
+        out = getattr(ops, name)(*a)
+        out = out[0] if isinstance(out, tuple) else out
+        assert tuple(out.shape) == (10, 8, 128) and out.device.type == "cuda" and out.requires_grad == grad
+        a[0] = _t((10, 8, 96), device="cuda")
+        with pytest.raises(RuntimeError, match="D must be"):
+            getattr(ops, name)(*a)
+
+
+def test_trees_are_as_large_as_they_were():
+    """The limit of this format's batches is none of the other cache formats'."""
+    shape = va._PagedShape(1 << 8, 32, 32, 128, 32, 64, 1 << 15, 256, 1 << 21)
+    assert va.lib.va_tree_ws_bytes(int(va.Fmt.parse("q8+")), C.byref(shape), 4) > 0

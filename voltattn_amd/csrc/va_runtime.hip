@@ -859,7 +859,7 @@ int validate_tree(va_fmt fmt, const va_paged_shape* sh, int T, va::TreeForm* for
     if (rows > 1 << 20 || (long long)sh->B * T * sh->Hq > 0x7FFFFFFFLL / 64) return fail(VA_ERANGE, "B*T*Hq too large");
     if ((long long)sh->B * sh->Hkv * ((rows + 31) / 32) > MAX_GROUPS) return fail(VA_ERANGE, "B*Hkv too large");
     *form = va::tree_form(kind_of(fmt), sh->D, sh->B, sh->Hkv, (int)rows, sh->max_seq_len, cus_or_default());
-    if (form->tiles > 1 << 27) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
+    if (form->tiles > 1 << 30) return fail(VA_ERANGE, "batch too large: %lld K/V tiles", form->tiles);
     return VA_OK;
 }
 
