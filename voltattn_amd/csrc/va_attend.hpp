@@ -427,11 +427,10 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
 #pragma unroll
             for (int i = 0; i < VL; ++i) vr[b % VAHEAD][i] = ld128(rv, (uint32_t)(i * 1024 + fresh_lane() * 16), 0);
         };
-        auto fetch = [&](int t, int b) {
+        auto fetch_rows = [&](int t, int b) {
             if (t >= pl.base + 64 || pl.base < 0) pl.load(a, table, hk, t, t1, BN, wave * 32, len);
             const int l = t - pl.base, page = __builtin_amdgcn_readlane(pl.page, l), j = t * BN + wave * 32;
             const int left = page < 0 ? 0 : max(0, min(32, len - j));
-            sc[b].set((uint32_t)__builtin_amdgcn_readlane((int)pl.sk, l), (uint32_t)__builtin_amdgcn_readlane((int)pl.sv, l), a.qscale, page >= 0);
             on[b] = j < len;
             const size_t row = uniform64((((size_t)(page < 0 ? 0 : page) * a.hkv + hk) << a.page_shift) + (size_t)(j & ((1 << a.page_shift) - 1)));
             const uint32_t bytes = (uint32_t)(uniform(left) * D);
@@ -444,6 +443,15 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
 #pragma unroll
                 for (int c = 0; c < KC; ++c) kr[b][i * KC + c] = ld128(rk, (uint32_t)((16 * i + c16) * D + 64 * c + 16 * h), 0);
             if (VAHEAD == 2) fetch_v(b);
+        };
+        auto scales_of = [&](int t, int b) {
+            const int l = t - pl.base;
+            sc[b].set((uint32_t)__builtin_amdgcn_readlane((int)pl.sk, l), (uint32_t)__builtin_amdgcn_readlane((int)pl.sv, l), a.qscale,
+                      __builtin_amdgcn_readlane(pl.page, l) >= 0);
+        };
+        auto fetch = [&](int t, int b) {
+            fetch_rows(t, b);
+            scales_of(t, b);
         };
         f32x4 o[NB][DT] = {};
         float m[NB], l[NB];
@@ -547,9 +555,11 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
                 for (int y = 0; y < NB; ++y) o[y][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, p[y], o[y][d], 0, 0, 0);
             }
         };
-        fetch(t0, 0);
+        fetch_rows(t0, 0);                                   // the first rows do not wait for their scales
         if (VAHEAD == 1) fetch_v(0);
-        if (t0 + 1 < t1) fetch(t0 + 1, 1);
+        if (t0 + 1 < t1) fetch_rows(t0 + 1, 1);
+        scales_of(t0, 0);
+        if (t0 + 1 < t1) scales_of(t0 + 1, 1);
         int t = t0;
         do {
             tile(t, 0);
