@@ -105,15 +105,16 @@ template <int BM, int BN> struct AttendPlan {
     static constexpr int AGES = BM == 128 ? 3 : BM == 256 ? 2 : 1;
     static constexpr int AGE[4] = {0, AGES == 3 ? 10 : 8, AGES == 3 ? 18 : 14, 24};   // what the work-groups up to an age take
     const AttendArgs& a;
-    int from = -1, prev = 0;                     // prev: the bound ahead of the next 64
+    int from = -1, before = 0, prev = 0;         // before: units ahead of the 64; prev: the bound ahead of the next ones
     int begin = 0, n = 0, len = 0;
     int count = 0, upto = 0;                     // units of the lane's span, and up to and with it
     int total = 0;                               // units of the batch
     __device__ __forceinline__ int spans() const { return a.cu ? a.B + 2 : a.B; }
     __device__ __forceinline__ int seq_of(int i) const { return !a.cu ? (i < a.B ? i : -1) : i >= 1 && i <= a.B ? i - 1 : -1; }
     static __device__ __forceinline__ int ahead(int head, int slope, int rb) { return rb * head + (int)((long long)rb * (rb - 1) / 2) * slope; }   // units of blocks 0 .. rb - 1
-    __device__ __forceinline__ void load(int at, int before, int bound) {
+    __device__ __forceinline__ void load(int at, int units, int bound) {
         from = at;
+        before = units;
         const int i = at + (fresh((int)threadIdx.x) & 63);
         const int seq = seq_of(i);
         len = seq >= 0 ? a.seq_lens[seq] : 0;
@@ -131,22 +132,18 @@ template <int BM, int BN> struct AttendPlan {
         count = ahead(Block::head(a, seq, n, len), Block::slope(a, seq, n, len), Block::blocks(a, n)) * a.hkv;
         upto = before + wave_scan(count);
     }
-    __device__ __forceinline__ explicit AttendPlan(const AttendArgs& args) : a(args) {
-        for (int at = 0; at < spans(); at += 64) {
+    // all: counts the batch's units (else only to find blocks)
+    __device__ __forceinline__ explicit AttendPlan(const AttendArgs& args, bool all = true) : a(args) {
+        for (int at = 0; at < (all ? spans() : 1); at += 64) {
             load(at, total, prev);
             total = __builtin_amdgcn_readlane(upto, 63);
         }
     }
     // The block that unit `at` < total is in.
     __device__ __forceinline__ Block find(int at) {
-        if (spans() > 64) {
-            int before = 0, bound = 0;
-            for (int f = 0; f < spans(); f += 64) {
-                load(f, before, bound);
-                before = __builtin_amdgcn_readlane(upto, 63);
-                bound = prev;
-                if (at < before) break;
-            }
+        if (spans() > 64) {                      // on from the last block's, if this one is behind it
+            if (at < before) load(0, 0, 0);
+            while (at >= __builtin_amdgcn_readlane(upto, 63)) load(from + 64, __builtin_amdgcn_readlane(upto, 63), prev);
         }
         const int l = __builtin_ctzll(__ballot(upto > at));
         Block b;
@@ -804,7 +801,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
     blk.tiles = 0;
     do {
         if (blk.tiles == 0 || !blk.next(a)) {
-            AttendPlan<BM, BN> plan(a);                      // (holding the plan would cost the loop's registers)
+            AttendPlan<BM, BN> plan(a, end == 0);            // (holding the plan would cost the loop's registers)
             if (end == 0) {
                 const AttendShare<D, BM, BN> share(a, plan);
                 wg = share.wg;
