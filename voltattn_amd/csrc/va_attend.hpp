@@ -369,11 +369,10 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
     constexpr int EPI = 4 * 16 * ES * 4, ML = 4 * 16 * 2 * 4;
     constexpr int LDS = 4 * VB > EPI + ML ? 4 * VB : EPI + ML;
     __shared__ __align__(1024) uint8_t lds[LDS + 16];
-    lds_int* odd = (lds_int*)((lds_u8*)lds + LDS);
+    lds_int* odds = (lds_int*)((lds_u8*)lds + LDS);          // of each wave, in the epilogue: whether it has left out NaN codes
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 4, c16 = lane & 15;
     lds_u8* vt = (lds_u8*)lds + wave * VB;
-    if (tid == 0) *odd = 0;
     AttendPlan<BM, BN> plan(a);
     const AttendShare<D, BM, BN> share(a, plan);
     const int wg = share.wg, end = share.end;
@@ -458,6 +457,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
             l[b] = 0.f;
         }
         int unit = 0;
+        bool odd = false;                                    // this lane has left out NaN codes
         auto tile = [&](int t, int b) {
             if (!on[b]) return;                              // nothing there, nor behind it: uniform
             const int j0 = t * BN + wave * 32;
@@ -482,16 +482,14 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
                     }
                 }
             const bool hides = j0 + 31 > all;
-            bool any = false;
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < VL; ++i) {
                 u32x4 w = vr[b % VAHEAD][i];
-                if (hides) any |= codes_clean(w);
+                if (hides) odd |= codes_clean(w);
                 const int row = vrow + i * (1024 / D);
                 *reinterpret_cast<lds_u32x4*>(vt + row * D + ((vchunk ^ few_swz<D>(row)) << 4)) = w;
             }
-            if (any) *odd = 1;
             if (VAHEAD == 1 && t + 1 < t1) fetch_v(b ^ 1);
             if (s.bad) {
 #pragma unroll
@@ -572,6 +570,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
         lds_float* es = (lds_float*)lds;
         lds_float* ml = es + EPI / 4;
         const float scale = power(unit);
+        odds[wave] = __any(odd) != 0;                        // read between this epilogue's barriers only: nothing to clear
 #pragma unroll
         for (int y = 0; y < NB; ++y) {
             const float ly = rows_sum(l[y]);
@@ -583,6 +582,8 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
                 ml[(wave * 16 + c16) * 2 + 1] = ly;
             }
             __syncthreads();
+            const i32x4 left = *reinterpret_cast<__attribute__((address_space(3))) i32x4*>(odds);
+            const bool any = uniform(left.x | left.y | left.z | left.w) != 0;
             for (int i = tid; i < 16 * (D / 4); i += 256) {
                 const int r = i / (D / 4), c = i % (D / 4) * 4, to = rb * BM + y * 16 + r;
                 if (to >= rows) break;
@@ -600,7 +601,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
                     for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(f, z[e], x[e]);
                 }
                 const int tok = (int)a.by_group.div((uint32_t)to);
-                if (*odd) {                                  // NaN codes that were left out, to the rows that see them
+                if (any) {                                   // NaN codes that were left out, to the rows that see them
                     uint32_t nan = 0;
                     for (int j = max(max(t0 * BN, all + 1 - BN), 0); j <= min(ctx + tok, t1 * BN - 1); ++j) nan |= attend_odd<D>(a, table, hk, j, c);
 #pragma unroll
@@ -618,8 +619,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
                 }
             }
         }
-        __syncthreads();                                     // the sums are read, odd too
-        if (tid == 0) *odd = 0;
+        __syncthreads();                                     // the sums are read, odds too
     }
 }
 
