@@ -342,6 +342,24 @@ __device__ __forceinline__ uint32_t attend_odd(const AttendArgs& a, const int32_
 // The lazy maximum, as WIDE_OFF and WIDE_SLACK, with room for the part of V's scale below 2.
 constexpr float ATT_OFF = 10.f, ATT_SLACK = 4.f;
 
+// A weight is exp2 of a fused product less the maximum, whose product was rounded: where the maximum is far from 0,
+// digits that only one of the two has are whole powers of two (from 2^27 on weights would pass fp16's range, from 2^30
+// on the largest may become 0), and `more` is lost in the maximum's last step. A wave with a row whose maximum is far
+// therefore makes its scores less the maximum first, of products rounded once. (Scores far from a maximum that is not
+// have the weight 0.) No model has such scores; whether there are any is looked at where a maximum grows. (10 prompts'
+// chunks 645 us without, 651 with it; 8 K tokens over 32 K positions 3674 and 3689.)
+constexpr float ATT_FAR = 4096.f;
+__device__ __forceinline__ bool is_far(float m) { return __builtin_fabsf(m) >= ATT_FAR && m != -__builtin_inff(); }
+__device__ __forceinline__ float rounded_product(float x, float y) {
+#pragma clang fp contract(off)
+    return x * y;
+}
+// The lazy maximum's next value. Its last step may be more than ATT_OFF.
+__device__ __forceinline__ float next_max(float m, float top) {
+    const float to = fmaxf(m, top - ATT_OFF);
+    return top - to > ATT_OFF + ATT_SLACK ? top : to;
+}
+
 // ---------------------------------------------------------------- one or few rows --
 // Block: 16 NB rows as columns of 16x16x32 products; the four waves take 32 positions each of a tile
 // of 128, every wave by itself until the piece ends. K comes from memory in the operand's layout
@@ -456,7 +474,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
             m[b] = -__builtin_inff();
             l[b] = 0.f;
         }
-        int unit = 0;
+        int unit = 0, far = 0;                               // far: some row's maximum is
         bool odd = false;                                    // this lane has left out NaN codes
         auto tile = [&](int t, int b) {
             if (!on[b]) return;                              // nothing there, nor behind it: uniform
@@ -512,30 +530,40 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
                 top[y] = x[0][y][0];
 #pragma unroll
                 for (int e = 1; e < 8; ++e) top[y] = fmaxf(top[y], x[e / 4][y][e % 4]);
-                top[y] = rows_max(top[y]) * s.qs;
+                top[y] = rounded_product(rows_max(top[y]), s.qs);
                 grows |= top[y] - m[y] > ATT_OFF + ATT_SLACK;    // also at the first one: m = -inf
             }
             const int to_unit = unit_for(s, unit);
             if (__any(grows) || to_unit != unit) {
                 const float u = power(unit - to_unit);
                 unit = to_unit;
+                bool away = false;
 #pragma unroll
                 for (int y = 0; y < NB; ++y) {
-                    const float to = fmaxf(m[y], top[y] - ATT_OFF), f = to == m[y] ? 1.f : fast_exp2(m[y] - to);
+                    const float to = next_max(m[y], top[y]), f = to == m[y] ? 1.f : fast_exp2(m[y] - to);
                     m[y] = to;
                     l[y] *= f;
 #pragma unroll
                     for (int d = 0; d < DT; ++d) o[y][d] *= f * u;
+                    away |= is_far(m[y]);
                 }
+                far = __any(away);
             }
+            if (__builtin_expect(far, 0)) {                  // from here on the scores are less the maximum
+#pragma unroll
+                for (int y = 0; y < NB; ++y)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e / 4][y][e % 4] = rounded_product(x[e / 4][y][e % 4], s.qs) - (m[y] == -__builtin_inff() ? 0.f : m[y]);
+            }
+            const float qs = uniformf(far ? 1.f : s.qs);
             f16x8 p[NB];
 #pragma unroll
             for (int y = 0; y < NB; ++y) {
-                const float up = s.more - (m[y] == -__builtin_inff() ? 0.f : m[y]);
+                const float up = s.more - (far || m[y] == -__builtin_inff() ? 0.f : m[y]);
                 float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float w = fast_exp2(__builtin_fmaf(x[e / 4][y][e % 4], s.qs, up));
+                    const float w = fast_exp2(__builtin_fmaf(x[e / 4][y][e % 4], qs, up));
                     sum += w;
                     p[y][e] = (_Float16)w;
                 }
@@ -728,7 +756,7 @@ __device__ __forceinline__ void wide_sums(lds_u8* v, uint32_t at, const float (&
 // The weights of two score blocks: of one row under the scales sc[0] and sc[1] (CB = 1), or of two rows
 // under sc[0]. The maxima and the unit of the sums follow where they have to.
 template <int D, int CB>
-__device__ __forceinline__ void wide_softmax(const f32x16 (&s)[2], const Scales* sc, int to_unit, int& unit, float (&m)[CB], float (&l)[CB],
+__device__ __forceinline__ void wide_softmax(f32x16 (&s)[2], const Scales* sc, int to_unit, int& unit, int& far, float (&m)[CB], float (&l)[CB],
                                              f32x16 (&o)[CB][D / 32], f16x8 (&p)[2][2]) {
     float top[CB];
 #pragma unroll
@@ -739,7 +767,7 @@ __device__ __forceinline__ void wide_softmax(const f32x16 (&s)[2], const Scales*
 #pragma unroll
         for (int v = 1; v < 16; ++v) x = fmaxf(x, s[i][v]);
         const int c = CB == 1 ? 0 : i;
-        top[c] = fmaxf(top[c], x * sc[CB == 1 ? i : 0].qs);
+        top[c] = fmaxf(top[c], rounded_product(x, sc[CB == 1 ? i : 0].qs));
     }
     bool grows = false;
 #pragma unroll
@@ -750,25 +778,36 @@ __device__ __forceinline__ void wide_softmax(const f32x16 (&s)[2], const Scales*
     if (__any(grows) || to_unit != unit) {
         const float u = power(unit - to_unit);
         unit = to_unit;
+        bool away = false;
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
-            const float to = fmaxf(m[c], top[c] - ATT_OFF), f = to == m[c] ? 1.f : fast_exp2(m[c] - to);
+            const float to = next_max(m[c], top[c]), f = to == m[c] ? 1.f : fast_exp2(m[c] - to);
             m[c] = to;
             l[c] *= f;
             const float g = f * u;
 #pragma unroll
             for (int db = 0; db < D / 32; ++db) o[c][db] *= g;
+            away |= is_far(m[c]);
+        }
+        far = __any(away);
+    }
+    if (__builtin_expect(far, 0)) {                          // from here on the scores are less the maximum
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = CB == 1 ? 0 : i;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[i][v] = rounded_product(s[i][v], sc[CB == 1 ? i : 0].qs) - (m[c] == -__builtin_inff() ? 0.f : m[c]);
         }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int c = CB == 1 ? 0 : i;
         const Scales& x = sc[CB == 1 ? i : 0];
-        const float up = x.more - (m[c] == -__builtin_inff() ? 0.f : m[c]);
+        const float qs = uniformf(far ? 1.f : x.qs), up = x.more - (far || m[c] == -__builtin_inff() ? 0.f : m[c]);
         float sum = 0.f;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-            const float w = fast_exp2(__builtin_fmaf(s[i][v], x.qs, up));
+            const float w = fast_exp2(__builtin_fmaf(s[i][v], qs, up));
             sum += w;
             p[i][v / 8][v % 8] = (_Float16)w;
         }
@@ -885,7 +924,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
             m[c] = -__builtin_inff();
             l[c] = 0.f;
         }
-        int unit = 0;
+        int unit = 0, far = 0;                               // far: some row's maximum is
         bool odd = false;                                    // this wave has left out NaN codes
         __syncthreads();                                     // the last piece's tiles are read
         fetch(t0, 0);
@@ -941,7 +980,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
                 }
                 f16x8 p[2][2];
                 __builtin_amdgcn_s_setprio(0);
-                wide_softmax<D, CB>(s, sc + (CB == 1 ? 0 : h), to_unit, unit, m, l, o, p);
+                wide_softmax<D, CB>(s, sc + (CB == 1 ? 0 : h), to_unit, unit, far, m, l, o, p);
                 __builtin_amdgcn_s_setprio(1);
                 const float f[2] = {factor_of(sc[CB == 1 ? 0 : h], unit), factor_of(sc[1], unit)};
                 wide_sums<D, CB>(vt, value_at(cur) + (uint32_t)(h * 32 * D), f, p, o);
