@@ -232,8 +232,9 @@ template <int STEP, int G> struct Places {
         if (page >= 0) {
             const size_t at = ((((size_t)page * a.hkv + hk) << a.page_shift) + (size_t)(j & ((1 << a.page_shift) - 1))) / G;
             if constexpr (STEP > G) {
-                sk = *reinterpret_cast<const uint32_t*>(a.sk + at);
-                sv = *reinterpret_cast<const uint32_t*>(a.sv + at);
+                const uint32_t own = end - j <= G ? 0xFFFFu : 0xFFFFFFFFu;   // what lies behind the last position is not the sequence's
+                sk = *reinterpret_cast<const uint32_t*>(a.sk + at) & own;
+                sv = *reinterpret_cast<const uint32_t*>(a.sv + at) & own;
             } else {
                 sk = a.sk[at] * 0x10001u;
                 sv = a.sv[at] * 0x10001u;
@@ -956,7 +957,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 3 : 2) void attend_wide(AttendArgs a
         for (; t < tw; ++t, cur ^= RAW) {
             Scales sc[2];
             sc[0].set(sk & 0xFFFFu, sv & 0xFFFFu, a.qscale, there);
-            sc[1].set(sk >> 16, sv >> 16, a.qscale, there || t * BN + 32 >= len);
+            sc[1].set(sk >> 16, sv >> 16, a.qscale, there);
             const int to_unit = unit_for(sc, unit);
             arrive(t, cur);
 #pragma unroll
