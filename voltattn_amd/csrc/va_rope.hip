@@ -90,8 +90,7 @@ __device__ __forceinline__ Rates rates_of(const RopeArgs& a, int d) {
     }
     return r;
 }
-__device__ __forceinline__ void set_turn(Turn& t, const RopeArgs& a, const Rates& r, int place) {
-    const double at = (double)place;
+__device__ __forceinline__ void set_turn(Turn& t, const RopeArgs& a, const Rates& r, double at) {
     const float sign = a.pairs || !r.lead ? a.scaling : -a.scaling;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -181,7 +180,7 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, int r, int j0, int
     const int oth = other(a, d);
     const Rates rates = rates_of(a, d);
     Turn t;
-    set_turn(t, a, rates, a.places ? a.places[r] : (int)p);
+    set_turn(t, a, rates, a.places ? (double)a.places[r] : (double)p);
     for (int jb = j0; jb < j1; jb += U) {
         u32x4 w[U], v[U];
 #pragma unroll
@@ -334,7 +333,7 @@ __device__ __forceinline__ void rope_block_few(const RopeArgs& a, int r, int j) 
         if (!is_k) return values8(w, x);
         u32x4 v = {0u, 0u, 0u, 0u};
         if (!a.pairs) v = *reinterpret_cast<const u32x4*>(s + oth);
-        set_turn(t, a, rates, a.places ? a.places[r + i] : (int)(p + i));
+        set_turn(t, a, rates, a.places ? (double)a.places[r + i] : (double)(p + i));
         turn8(t, rates.on, a.pairs, w, v, x);
     };
     float top = 0.f;
@@ -421,11 +420,12 @@ __device__ __forceinline__ void rope_block_many(const RopeArgs& a, int item, int
     float x[PASS][8], top = 0.f;                             // (rows past the last are that one again)
     if (is_k) {
         const Rates rates = rates_of(a, d);
+        const double first = (double)p;                      // (p may pass 32 bits: rows that are not written are turned all the same)
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
             Turn t;
             const int r = r0 + i * RP, rr = min(r, n - 1);
-            set_turn(t, a, rates, a.places ? a.places[begin + rr] : (int)(p + rr));
+            set_turn(t, a, rates, a.places ? (double)a.places[begin + rr] : first + (double)rr);
             turn8(t, rates.on, a.pairs, w[i], v[i], x[i]);
             if (a.k_out && r < n) *reinterpret_cast<u32x4*>(a.k_out + ((size_t)(begin + r) * a.hkv + hk) * D + d) = rates.on ? halves8(x[i]) : w[i];
         }
