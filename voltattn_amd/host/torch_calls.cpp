@@ -169,11 +169,14 @@ Tensor attend_paged(const Tensor& q, const Tensor& kp, const Tensor& vp, const T
     return out;
 }
 
-// Above the ops: inputs that require grad take the checked op, whose output's backward() raises.
+// Above the ops: inputs that require grad take the checked op, whose output's backward() raises, as do those with
+// a tangent (forward mode, which no_grad() leaves on), for which it raises itself.
 bool requires_grad(std::initializer_list<const Tensor*> ts) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor* t : ts)
-        if (t && t->requires_grad()) return true;
+    const bool backward = at::GradMode::is_enabled();
+    for (const Tensor* t : ts) {
+        if (!t || !t->unsafeGetTensorImpl()->autograd_meta()) continue;   // neither, as most are
+        if ((backward && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined()) return true;
+    }
     return false;
 }
 const Tensor* of(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }

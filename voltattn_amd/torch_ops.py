@@ -42,6 +42,7 @@ from pathlib import Path
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import (B8, TREE_MAX, Fmt, _AttendBufs, _Bufs, _PagedBufs, _PagedShape, _Pools, _PrefillBufs, _PrefillShape,
                _RopeBufs, _RopeShape, _TreeBufs, check, fmt_bits, lib, ws_bytes)
@@ -405,6 +406,13 @@ class _NoGradient(torch.autograd.Function):
         _fail(f"backward through voltattn::{ctx.name}, which has no gradient formula")
 
 
+def _no_tangents(name: str, args) -> None:
+    """Forward mode: an output without a tangent would be a wrong one."""
+    if torch._C._is_fwd_grad_enabled() and any(
+            isinstance(a, torch.Tensor) and a.is_floating_point() and _forward.unpack_dual(a).tangent is not None for a in args):
+        _fail(f"forward-mode gradient through voltattn::{name}, which has no gradient formula")
+
+
 def _op(schema: str, fake, computes: Optional[bool] = None, native: bool = False):
     """Registers the decorated function and its fake implementation; what it returns is the op.
     computes: whether its outputs are computed from its inputs (None: if it changes none in place).
@@ -424,6 +432,8 @@ def _op(schema: str, fake, computes: Optional[bool] = None, native: bool = False
         if "!" not in schema if computes is None else computes:
 
             def autograd(keys, *args):
+                if _forward._current_level >= 0:                # in a dual_level()
+                    _no_tangents(name, args)
                 grads = torch._C.is_grad_enabled() and torch._C._any_requires_grad(*args)
                 if not grads and keys.raw_repr() == _PLAIN:     # on a GPU: the dispatcher's second turn takes 3 us
                     return fn(*args)
