@@ -12,9 +12,14 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
+#include <torch/version.h>
 
 #include <optional>
 #include <tuple>
+
+// What the package looks for before it loads this library: it goes with one PyTorch.
+extern "C" __attribute__((used, visibility("default"))) const char va_torch_calls_for[] =
+    "voltattn calls for PyTorch " C10_STRINGIZE(TORCH_VERSION_MAJOR) "." C10_STRINGIZE(TORCH_VERSION_MINOR) "." C10_STRINGIZE(TORCH_VERSION_PATCH);
 
 namespace {
 

@@ -38,6 +38,8 @@ torch.compile.
 from __future__ import annotations
 
 import ctypes as C
+import re
+import warnings
 from pathlib import Path
 from typing import Optional
 
@@ -887,16 +889,25 @@ def row_format_bits(fmt: str) -> int:
     return _BITS[_fmt(fmt)]
 
 
-def _load_calls() -> None:
+def _load_calls(path: Path = Path(__file__).resolve().parent / "libvoltattn_torch.so") -> None:
     """host/torch_calls.cpp's plain calls: the C ABI's functions by their addresses in the library
-    that is loaded. Without a GPU nothing calls them, and the built file need not be there."""
-    path = Path(__file__).resolve().parent / "libvoltattn_torch.so"
-    if not path.exists():
-        if torch.cuda.device_count() > 0:
-            raise ImportError(f"{path} is not built; run `python voltattn_amd/build.py` (needs g++)")
-        return
-    torch.ops.load_library(str(path))
-    torch.ops.voltattn._bind([C.cast(f, C.c_void_p).value for f in (lib.va_append_rope, lib.va_attend_paged, lib.va_attend_ws_bytes)])
+    that is loaded. Where it was built without PyTorch, or for another one, these ops' plain calls go
+    through Python too, to the same kernels: said once, and nothing else changes. Without a GPU nothing
+    calls them."""
+    why = "is not built"
+    if path.exists():
+        if b"voltattn calls for PyTorch " + re.match(r"\d+\.\d+\.\d+", torch.__version__)[0].encode() + b"\0" not in path.read_bytes():
+            why = f"was built for another PyTorch than {torch.__version__}"
+        else:
+            try:
+                torch.ops.load_library(str(path))
+                torch.ops.voltattn._bind([C.cast(f, C.c_void_p).value for f in (lib.va_append_rope, lib.va_attend_paged, lib.va_attend_ws_bytes)])
+                return
+            except OSError as e:
+                why = f"does not load ({e})"
+    if torch.cuda.device_count() > 0:
+        warnings.warn(f"{path} {why}: append_rope and attend_paged take about 10 us more of host time a call; "
+                      "run `python voltattn_amd/build.py` (needs g++)", stacklevel=2)
 
 
 _load_calls()
