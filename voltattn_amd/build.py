@@ -163,13 +163,14 @@ def build_library(jobs: int = 8, out: Path = LIB, defines: tuple[str, ...] = (),
 
 
 def build_torch() -> Path | None:
-    """host/torch_calls.cpp against the installed PyTorch's headers and libraries; without PyTorch there is
-    nothing that would load it."""
+    """host/torch_calls.cpp against the installed PyTorch's headers and libraries; without a PyTorch for HIP
+    there is nothing that would load it."""
     out = PKG / "libvoltattn_torch.so"
     found = importlib.util.find_spec("torch")
-    if found is None or not found.origin:
+    torch = Path(found.origin).parent if found is not None and found.origin else None
+    if torch is None or not (torch / "lib" / "libc10_hip.so").exists():
+        out.unlink(missing_ok=True)
         return None
-    torch = Path(found.origin).parent
     rocm = Path(hipcc()).resolve().parent.parent
     tmp = out.with_suffix(".so.tmp")
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra", "-Werror",
@@ -207,10 +208,10 @@ def build_all(jobs: int = 8) -> None:
     with cf.ThreadPoolExecutor(max_workers=1) as ex:
         calls = ex.submit(build_torch)
         build_library(jobs, variants=tuple(VARIANTS))
-        calls.result()
     build_oracle()
     if (ROOT / "tests" / "cli" / "voltattn_cli.cpp").exists():
         build_cli()
+    calls.result()                           # raises what it met: nothing else waits for it
 
 
 if __name__ == "__main__":
