@@ -18,6 +18,7 @@
 // work-group w begins with, 2w + 1: the one it ends with) and attend_merge joins them.
 #pragma once
 #include "va_kernels.hpp"
+#include "va_shares.hpp"
 #include "va_wide.hpp"
 
 namespace va {
@@ -85,25 +86,13 @@ template <int BM, int BN> struct AttendBlock {
         size(a);
         return true;
     }
-    // The tiles ahead of unit first + x: in the numbering's proportion, the first tile with the first unit.
-    __device__ __forceinline__ int ahead(const AttendArgs& a, int x) const {
-        if (x >= units) return tiles;
-        if (x <= 0) return 0;
-        if (units == tiles << a.shift) return (x + (1 << a.shift) - 1) >> a.shift;   // the same, without the division
-        return (int)__builtin_ceil((double)x * tiles / units);
-    }
+    // The tiles ahead of unit first + x.
+    __device__ __forceinline__ int ahead(const AttendArgs& a, int x) const { return tiles_ahead(x, units, tiles, a.shift); }
 };
 
-// The numbering, by one wave: lane i has span from + i of the current 64. The work-groups of a CU do not
-// get on equally: its oldest waves go first. With equal shares of many rows those of 128-row blocks, three
-// to a CU, ended after 508, 650 and 752 us (10 prompts' chunks over up to 16 K positions), those of 256-row
-// blocks, two, after 3272 and 3977 (8 K tokens over 32 K positions); shares by age (10 : 8 : 6 and 8 : 6)
-// take these calls from 670 to 650 us and from 3900 to 3810. A launch fills the GPU in the order of its
-// blocks, an age after the other, eight XCDs in turn.
+// The numbering, by one wave: lane i has span from + i of the current 64.
 template <int BM, int BN> struct AttendPlan {
     using Block = AttendBlock<BM, BN>;
-    static constexpr int AGES = BM == 128 ? 3 : BM == 256 ? 2 : 1;
-    static constexpr int AGE[4] = {0, AGES == 3 ? 10 : 8, AGES == 3 ? 18 : 14, 24};   // what the work-groups up to an age take
     const AttendArgs& a;
     int from = -1, before = 0, prev = 0;         // before: units ahead of the 64; prev: the bound ahead of the next ones
     int begin = 0, n = 0, len = 0;
@@ -167,20 +156,7 @@ template <int BM, int BN> struct AttendPlan {
         b.size(a);
         return b;
     }
-    // The shares: units start(w) .. start(w + 1) - 1 are work-group w's.
-    __device__ __forceinline__ bool by_age() const { return AGES > 1 && a.nwg % (8 * AGES) == 0 && total >> (a.shift + 4) >= a.nwg; }
-    __device__ __forceinline__ int share() const {
-        const int x = (total + a.nwg - 1) / a.nwg, tile = 1 << a.shift;
-        return x >= 8 * tile ? x : (x + tile - 1) & -tile;   // whole tiles, where they are few
-    }
-    __device__ __forceinline__ int shares() const { return by_age() ? a.nwg : (total + share() - 1) / share(); }
-    __device__ __forceinline__ int start(int w) const {
-        if (!by_age()) return (int)min((long long)w * share(), (long long)total);
-        if (w >= a.nwg) return total;
-        const int per = a.nwg / 8, of = per / AGES, x = w / per, j = w - x * per, age = j / of;
-        const int p = (x * AGE[AGES] + AGE[age]) * of + (j - age * of) * (AGE[age + 1] - AGE[age]), all = 8 * AGE[AGES] * of;
-        return total / all * p + (int)((uint32_t)(total % all) * (uint32_t)p / (uint32_t)all);
-    }
+    __device__ __forceinline__ Shares<BM> shares() const { return Shares<BM>{total, a.nwg, a.shift}; }
 };
 
 // What attend_merge has to know of work-group w, behind the pieces in ws: whether it begins a block
@@ -202,14 +178,15 @@ template <int D, int BM, int BN> __device__ __forceinline__ void attend_write_no
 template <int D, int BM, int BN> struct AttendShare {
     int wg, at, end;
     __device__ __forceinline__ AttendShare(const AttendArgs& a, const AttendPlan<BM, BN>& plan) {
-        const int per = (plan.shares() + 7) >> 3, x = (int)blockIdx.x & 7, j = (int)blockIdx.x >> 3;   // neighbours on one XCD
+        const Shares<BM> shares = plan.shares();
+        const int per = (shares.shares() + 7) >> 3, x = (int)blockIdx.x & 7, j = (int)blockIdx.x >> 3;   // neighbours on one XCD
         wg = j < per ? x * per + j : 8 * per + x * ((int)(gridDim.x >> 3) - per) + j - per;
         if (wg < a.nwg && threadIdx.x == 0) {
             i32x4* to = reinterpret_cast<i32x4*>(attend_note<D, BM>(a, wg));
             to[0] = to[1] = i32x4{};
         }
-        at = j < per ? uniform(plan.start(wg)) : 0;
-        end = j < per ? uniform(plan.start(wg + 1)) : 0;
+        at = j < per ? uniform(shares.start(wg)) : 0;
+        end = j < per ? uniform(shares.start(wg + 1)) : 0;
     }
 };
 
