@@ -15,7 +15,9 @@ constexpr int SETUP = 2;
 // 16 sequences over 4 K with 16 rows to a head 40.3 and 42.3, with 24 52.2 and 43.7; with 32 rows and blocks of 32
 // 45.2, of 128 57.4; with 64 rows 83 (16), 61 (128). 2 x 4 K tokens over 8 K positions with blocks of 128 rows
 // 869, of 256 836, 8 K tokens over 32 K 3880 and 3615; with 2048 rows both take 306, and blocks of 128 waste less of
-// uneven batches. One launch for all of a batch: of a step with four chunks among 36 tokens two (16-row blocks
+// uneven batches. (All of batches whose sequences are alike: the mean says little of one long chunk beside many
+// tokens, whose rows then share the tokens' short blocks. 127 tokens and a chunk of 512 take 215 us, 111 and 71
+// apart.) One launch for all of a batch: of a step with four chunks among 36 tokens two (16-row blocks
 // for the tokens, 128-row blocks for the chunks) took 157 against 158.
 AttendForm attend_form(int B, int total, int hkv, int group, int cap, int cus) {
     AttendForm f;

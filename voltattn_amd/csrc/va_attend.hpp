@@ -347,7 +347,7 @@ __device__ __forceinline__ float next_max(float m, float top) {
 // rows; probed on MI355X). A lane's slots of the second product are the positions whose scores it
 // holds: 4h + 0..3 and 16 + 4h + 0..3.
 //
-// Bound by memory: 32 heads over 64 K positions (537 MB) 85.5 us, 6.3 TB/s of the 7.3 that plain reads reach; 64
+// Bound by memory: 32 heads over 64 K positions (537 MB) 85 us, 6.3 TB/s of the 7.3 that plain reads reach; 64
 // sequences over up to 8 K positions (303 MB) 56 us, where every work-group begins two blocks; one token over
 // 4 K positions 7 us, the chain of lengths, table, scales and tile. Three work-groups on a CU (161 registers,
 // one V tile ahead) do 64 K positions in 91 us.
@@ -646,7 +646,7 @@ __global__ __launch_bounds__(256, 2) void attend_few(AttendArgs a) {
 // us without, 3998 with it, before shares went by age).
 //
 // Bound by the matrix cores and what shares the issue port with them: those 8 K tokens (32 heads, 8 K/V
-// heads of 128 dimensions) take 3590 to 3690 us, 1050 TFLOP/s at the 1.9 GHz that the power allows; a
+// heads of 128 dimensions) take 3690 to 3780 us, 1020 to 1040 TFLOP/s at the 1.9 GHz that the power allows; a
 // large product of the library does 1173 to 1465.
 //
 // A lane has two score blocks of 32 positions at a time: both halves of a tile against one row (CB =
